@@ -561,6 +561,97 @@ int t2c_linear_allreduce(int wtype, const void *x, const void *w, const void *re
                          int64_t K, void *const *bufs, int rank, int tp, uint32_t *counter, int64_t n_max,
                          void *stream);
 
+/* ------------------------------------------- paged KV cache in 8 bits
+ * A pool of pages of int8 codes, k / v [num_pages][n_kv][page_size][head_dim] (element strides page_stride,
+ * head_stride, row_stride, multiples of 16, shared by k and v; unit stride along head_dim), with one fp16 scale
+ * for each `block` consecutive tokens of a KV head, k_scale / v_scale [num_pages][n_kv][page_size / block]
+ * (strides scale_page_stride, scale_head_stride; unit last).  A code c in -127..127 stands for c * scale.
+ * page_size: a power of two from 16 up; block: 16, 32 or 64, at most page_size; head_dim 64 or 128.
+ * block_table int32 [B, bt_width] (row stride bt_stride) maps a sequence's logical pages to physical ones; an
+ * entry outside [0, num_pages) is reported through t2c_device_status (T2C_EINVAL): writes skip those rows,
+ * attention and eviction read page 0 in their place, the read back gives zeros.
+ * The reference keeps fp16 caches only (kv_cache_write_f16.py:22-92); these entry points have no counterpart.
+ */
+typedef struct {
+    void *k, *v, *k_scale, *v_scale;
+    int64_t page_stride, head_stride, row_stride;
+    int64_t scale_page_stride, scale_head_stride;
+    int64_t num_pages, n_kv, page_size, head_dim, block;
+} t2c_q8_pages;
+
+/*
+ * Appends rows k / v [B, T, n_kv, head_dim] (fp16, element strides) at positions[b] .. positions[b] + T - 1;
+ * rows at negative positions are padding and skipped, rows past the table are skipped and reported.
+ * For each block that gets rows: scale = max(the scale it has, if it holds earlier rows; the least fp16 number
+ * >= max|new| / 127, at most 515.5), code = round-half-even(value / scale); when the scale grows, the earlier
+ * rows' codes become round-half-even(code * old / new).  A block given a non-finite value gets scale NaN and
+ * codes 0, and reads as NaN until its first row is written again.
+ */
+int t2c_kv_cache_write_q8(const t2c_q8_pages *pages, const void *k, int64_t k_sb, int64_t k_st, int64_t k_sh,
+                          const void *v, int64_t v_sb, int64_t v_st, int64_t v_sh, const int32_t *positions,
+                          const int32_t *block_table, int64_t bt_stride, int64_t bt_width, int64_t B, int64_t T,
+                          void *stream);
+/*
+ * Rows first[b] .. first[b] + T - 1 as fp16 values, k_out / v_out [B, T, n_kv, head_dim] contiguous (code * scale
+ * rounded once); rows before position 0 or from lengths[b] on are zero.
+ */
+int t2c_kv_cache_read_q8(const t2c_q8_pages *pages, void *k_out, void *v_out, const int32_t *first,
+                         const int32_t *lengths, const int32_t *block_table, int64_t bt_stride, int64_t bt_width,
+                         int64_t B, int64_t T, void *stream);
+/*
+ * Attention of T queries per sequence over the cache: query t of sequence b sees positions 0 .. positions[b] + t
+ * (its own row is already cached); grouped heads (NH % n_kv == 0, query head h reads KV head h / (NH / n_kv)).
+ *   out = softmax(scale * q k^T) v, lse = log sum exp of the scaled scores (natural log; NULL: not stored).
+ * A query that sees nothing (negative position) gives out 0 and lse -inf.
+ * q, out fp16 with element strides (multiples of 8, unit along head_dim); lse fp32 [B, NH, T].
+ * max_len > 0: no sequence has more than max_len positions (longer ones are cut to it and reported).
+ * splits: CTAs that share one sequence's keys, 0 = chosen by the library; workspace: at least
+ * t2c_attn_*_q8_workspace(...) floats for the same arguments (-1: arguments out of range).
+ * t2c_attn_decode_q8 is the T = 1 form.  Its weights_out (NULL: off) fp32 [B, n_kv, positions] (strides w_sb,
+ * w_sh, unit last) gets, for each position j the query sees, weights[j] (0 for j = positions[b], and everywhere
+ * when weights is NULL) plus the softmax probability of j summed over the heads of the group; weights and
+ * weights_out may be one tensor.
+ */
+int64_t t2c_attn_decode_q8_workspace(const t2c_q8_pages *pages, int64_t bt_width, int64_t B, int64_t NH,
+                                     int64_t max_len, int64_t splits, int with_weights);
+int t2c_attn_decode_q8(const t2c_q8_pages *pages, const void *q, int64_t q_sb, int64_t q_sh, void *out, int64_t o_sb,
+                       int64_t o_sh, float *lse, const int32_t *positions, const int32_t *block_table,
+                       int64_t bt_stride, int64_t bt_width, int64_t B, int64_t NH, float scale, int64_t max_len,
+                       int64_t splits, const float *weights, float *weights_out, int64_t w_sb, int64_t w_sh,
+                       float *workspace, int64_t workspace_floats, void *stream);
+int64_t t2c_attn_prefill_q8_workspace(const t2c_q8_pages *pages, int64_t bt_width, int64_t B, int64_t T, int64_t NH,
+                                      int64_t max_len, int64_t splits);
+int t2c_attn_prefill_q8(const t2c_q8_pages *pages, const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh, void *out,
+                        int64_t o_sb, int64_t o_st, int64_t o_sh, float *lse, const int32_t *positions,
+                        const int32_t *block_table, int64_t bt_stride, int64_t bt_width, int64_t B, int64_t T,
+                        int64_t NH, float scale, int64_t max_len, int64_t splits, float *workspace,
+                        int64_t workspace_floats, void *stream);
+/*
+ * The attention weight that T queries give each cached key: weights_out[b, kv head, j] = w + sum over the heads of
+ * the group and the queries t with j <= positions[b] + t of exp(scale * q_t . k_j - lse[b, h, t]), for the
+ * positions j the last query sees; w = weights[j] for j < positions[b], else 0 (0 everywhere when weights is
+ * NULL).  lse fp32 [B, NH, T] from t2c_attn_prefill_q8.  weights and weights_out may be one tensor.
+ */
+int t2c_attn_key_weights_q8(const t2c_q8_pages *pages, const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                            const float *lse, const int32_t *positions, const int32_t *block_table, int64_t bt_stride,
+                            int64_t bt_width, int64_t B, int64_t T, int64_t NH, float scale, int64_t max_len,
+                            const float *weights, float *weights_out, int64_t w_sb, int64_t w_sh, void *stream);
+/*
+ * Cuts every sequence to at most `keep` positions, for each KV head by itself: a sequence of n = lengths[b] <= keep
+ * positions keeps all; otherwise the first `sinks`, the last `recent` and, of the others, those with the largest
+ * weights[b, head, j] stay (equal weights: the lowest positions; NaN counts as the largest).  The kept rows move, in
+ * order, to positions 0 .. of out_table's pages; each block's new scale is the least fp16 number >= its
+ * max|code * scale| / 127, code' = round-half-even(code * scale / new scale).  out_table = block_table (one pointer)
+ * compacts in place (a sequence that keeps all is then left as it is); otherwise the tables' pages must be disjoint.
+ * kept int32 [B, n_kv, keep] gets the kept positions (ascending, then -1), new_lengths[b] = min(n, keep),
+ * weights_out[b, head, i] = the weight of kept position i (may be weights itself when in place).
+ */
+int t2c_kv_cache_evict_q8(const t2c_q8_pages *pages, const float *weights, int64_t w_sb, int64_t w_sh,
+                          const int32_t *lengths, const int32_t *block_table, int64_t bt_stride, int64_t bt_width,
+                          const int32_t *out_table, int64_t ot_stride, int64_t ot_width, int64_t B, int64_t keep,
+                          int64_t sinks, int64_t recent, float *weights_out, int64_t wo_sb, int64_t wo_sh,
+                          int32_t *kept, int32_t *new_lengths, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

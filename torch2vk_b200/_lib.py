@@ -106,10 +106,33 @@ _SIGNATURES: dict[str, list] = {
     "t2c_embedding_q8_0": [_vp, _vp, _vp, _i64, _i64, _i64, _vp],
     "t2c_ew_misc": [_i32, _vp, _i32, _vp, _i32, _vp, _i32, _i64, _i64, _f32, _vp],
     "t2c_row_mean_f32": [_vp, _vp, _i64, _i64, _vp],
+    "t2c_kv_cache_write_q8": [_vp] + [_vp, _i64, _i64, _i64] * 2 + [_vp, _vp] + [_i64] * 4 + [_vp],
+    "t2c_kv_cache_read_q8": [_vp] * 6 + [_i64] * 4 + [_vp],
+    "t2c_attn_decode_q8_workspace": [_vp] + [_i64] * 5 + [_i32],
+    "t2c_attn_decode_q8": [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _f32, _i64,
+                           _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp],
+    "t2c_attn_prefill_q8_workspace": [_vp] + [_i64] * 6,
+    "t2c_attn_prefill_q8": [_vp] + [_vp, _i64, _i64, _i64] * 2 + [_vp, _vp, _vp] + [_i64] * 5 + [_f32, _i64, _i64, _vp,
+                                                                                         _i64, _vp],
+    "t2c_attn_key_weights_q8": [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp] + [_i64] * 5 + [_f32, _i64, _vp, _vp, _i64,
+                                                                                       _i64, _vp],
+    "t2c_kv_cache_evict_q8": [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp] + [_i64] * 6 + [_vp, _i64, _i64, _vp,
+                                                                                          _vp, _vp],
 }
+
+
+class Q8PagesStruct(_c.Structure):
+    """t2c_q8_pages of include/t2c_sm100.h."""
+
+    _fields_ = [(n, _vp) for n in ("k", "v", "k_scale", "v_scale")] + [(n, _i64) for n in (
+        "page_stride", "head_stride", "row_stride", "scale_page_stride", "scale_head_stride", "num_pages", "n_kv",
+        "page_size", "head_dim", "block")]
+
+
 _RESTYPES = {"t2c_last_error": _c.c_char_p, "t2c_attn_decode_fused_workspace": _c.c_int64,
              "t2c_allreduce_buffer_bytes": _c.c_int64, "t2c_linear_f32_scratch_bytes": _c.c_int64,
-             "t2c_linear_allreduce_buffer_bytes": _c.c_int64}
+             "t2c_linear_allreduce_buffer_bytes": _c.c_int64, "t2c_attn_decode_q8_workspace": _c.c_int64,
+             "t2c_attn_prefill_q8_workspace": _c.c_int64}
 
 
 class T2CError(RuntimeError):

@@ -1,0 +1,110 @@
+// Paged KV cache in 8 bits: the device view of the pool and the code <-> value
+// helpers that the write, read, eviction and attention kernels share.
+//
+// A code c (int8, -127..127) of a block of `block` consecutive tokens of one
+// KV head stands for c * s, s the block's fp16 scale.  c * s has at most
+// 7 + 11 significant bits, so fp32 holds it exactly.  A NaN scale marks a block
+// that was given a non-finite value: all of it reads as NaN.
+#pragma once
+
+#include <math.h>
+
+#include "common.cuh"
+
+namespace t2c {
+
+struct KvPages {
+    int8_t *k, *v;
+    __half *ks, *vs;
+    int64_t page_stride, head_stride, row_stride;  // codes, in elements (= bytes)
+    int64_t s_page_stride, s_head_stride;          // scales, in elements
+    int num_pages, n_kv, page_log2, block_log2;
+};
+
+// Checks the pool's description; fills `out`.  `what` names the entry point in messages.
+int kv8_view(const t2c_q8_pages *pages, const char *what, KvPages &out);
+// Checks a block table against the pool: returns T2C_OK and the capacity in positions.
+int kv8_table(const t2c_q8_pages *pages, const int32_t *table, int64_t stride, int64_t width, const char *what,
+              int64_t &capacity);
+
+// Physical page of a position; an entry outside the pool is reported and becomes -1.
+__device__ __forceinline__ int kv8_page(const KvPages &pg, const int32_t *__restrict__ table, int64_t pos) {
+    const int page = table[pos >> pg.page_log2];
+    if (static_cast<unsigned>(page) < static_cast<unsigned>(pg.num_pages)) return page;
+    report_device_error(T2C_EINVAL);
+    return -1;
+}
+
+__device__ __forceinline__ int64_t kv8_row_offset(const KvPages &pg, int page, int head, int64_t pos) {
+    return page * pg.page_stride + head * pg.head_stride + (pos & ((1 << pg.page_log2) - 1)) * pg.row_stride;
+}
+
+__device__ __forceinline__ int64_t kv8_scale_offset(const KvPages &pg, int page, int head, int64_t pos) {
+    return page * pg.s_page_stride + head * pg.s_head_stride + ((pos & ((1 << pg.page_log2) - 1)) >> pg.block_log2);
+}
+
+// Four codes (one 32-bit word) as two half2, exactly: the biased byte c + 128 placed in the low mantissa
+// bits of 1024 gives 1152 + c, and the subtraction is exact.  even = codes 0 and 2, odd = codes 1 and 3.
+__device__ __forceinline__ void kv8_unpack(uint32_t w, __half2 &even, __half2 &odd) {
+    const uint32_t lo = (w & 0x00ff00ffu) ^ 0x64806480u;
+    const uint32_t hi = ((w >> 8) & 0x00ff00ffu) ^ 0x64806480u;
+    const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
+    even = __hsub2(*reinterpret_cast<const __half2 *>(&lo), bias);
+    odd = __hsub2(*reinterpret_cast<const __half2 *>(&hi), bias);
+}
+
+// Least fp16 scale with 127 * s >= top, at most 515.5 (127 * 515.5 is the largest such product that fp16
+// holds; the fp16 values above it still get code 127).  top / 127 in fp32 picks the right fp16 neighbour: the
+// quotient of an at most 18-bit number by 127 is either an fp16 number or differs from one by more than 2^-20
+// of itself.  top = +inf (a non-finite value was seen) gives NaN.
+__device__ __forceinline__ __half kv8_scale_for(float top) {
+    if (!(top < INFINITY)) return __ushort_as_half(0x7fff);
+    return __float2half_ru(fminf(__fdiv_rn(top, 127.0f), 515.5f));
+}
+
+// round-to-nearest-even of x / s as the low byte of the result.  inv = 1 / s.  y = x * inv is within a few
+// ulp; adding the exactly computed residual x - y * s once makes every representable quotient (the ties
+// k + 1/2 among them) exact, and no other x / s of an up-to-18-bit x and an 11-bit s lies within 2^-20 of a
+// tie.  1.5 * 2^23 then leaves the integer in the low mantissa bits.  |x / s| <= 127.
+__device__ __forceinline__ uint32_t kv8_code(float x, float s, float inv) {
+    float y = x * inv;
+    y = fmaf(fmaf(-y, s, x), inv, y);
+    return __float_as_uint(y + 12582912.0f);
+}
+
+__device__ __forceinline__ uint32_t kv8_pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// Largest |code| of a word's four codes, folded into a running u16x2 maximum.
+__device__ __forceinline__ uint32_t kv8_absmax(uint32_t w, uint32_t best) {
+    const uint32_t sign = (w >> 7) & 0x01010101u;
+    const uint32_t mag = (w ^ (sign * 0xffu)) + sign;  // codes are >= -127: no byte overflows
+    return __vmaxu2(best, __vmaxu2(mag & 0x00ff00ffu, (mag >> 8) & 0x00ff00ffu));
+}
+
+template <typename Kernel, typename... Args>
+int kv8_launch(const char *what, Kernel kernel, dim3 grid, dim3 block, size_t smem, unsigned cluster,
+               cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (err != cudaSuccess) return set_error(T2C_ECUDA, "%s launch: %s", what, cudaGetErrorString(err));
+    return T2C_OK;
+}
+
+inline bool kv8_aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+
+}  // namespace t2c
