@@ -237,6 +237,14 @@ __device__ __forceinline__ void split_range(int64_t n, int splits, int s, int64_
 
 __device__ __forceinline__ float key_weight(const float *x, const float *lse2, int group) {
     float sum = 0.0f;
+    if ((group & 3) == 0) {  // rows of scores are 16-byte aligned
+        for (int g = 0; g < group; g += 4) {
+            const float4 v = *reinterpret_cast<const float4 *>(x + g);
+            sum += exp2_approx(v.x - lse2[g]) + exp2_approx(v.y - lse2[g + 1]) + exp2_approx(v.z - lse2[g + 2]) +
+                   exp2_approx(v.w - lse2[g + 3]);
+        }
+        return sum;
+    }
     for (int g = 0; g < group; ++g) sum += exp2_approx(x[g] - lse2[g]);
     return sum;
 }
@@ -266,20 +274,22 @@ __global__ void __launch_bounds__(kDThreads, 4) attn8_decode_kernel(DecodeArgs p
     // ---- the lane's step of a window of 32: page and scales, looked up a window ahead of their use
     int page = 0;
     float kf = 0.0f, lv = 0.0f, iv = 0.0f;
-    const auto look_up = [&](int window) {
+    const auto step_key = [&](int i) { return k0 + 16 * (warp + static_cast<int64_t>(kDWarps) * i); };
+    const auto look_up_page = [&](int window) {
+        const int i = window * 32 + lane;
+        if (i < mine) page = max(kv8_page(a.pg, bt, step_key(i)), 0);
+    };
+    const auto look_up_scales = [&](int window) {
         const int i = window * 32 + lane;
         if (i >= mine) return;
-        const int64_t key = k0 + 16 * (warp + static_cast<int64_t>(kDWarps) * i);
-        page = kv8_page(a.pg, bt, key);
-        if (page < 0) page = 0;
-        const int64_t so = kv8_scale_offset(a.pg, page, head, key);
+        const int64_t so = kv8_scale_offset(a.pg, page, head, step_key(i));
         kf = __half2float(a.pg.ks[so]) * a.scale_log2;
         const float vs = __half2float(a.pg.vs[so]);
         // a block of scale 0 has values 0: any exponent adds nothing to O, the least scale's moves no reference
         lv = vs == 0.0f ? -24.0f : log2f(vs);
         iv = vs == 0.0f ? 16777216.0f : 1.0f / vs;
     };
-    look_up(0);
+    look_up_page(0);
 
     // ---- Q^T fragments: k step i, lane (g, t): head g, dims D/4 t + 4 i + {0, 2} and {1, 3}
     uint32_t qf[kWords][2];
@@ -299,7 +309,7 @@ __global__ void __launch_bounds__(kDThreads, 4) attn8_decode_kernel(DecodeArgs p
     constexpr int kRowsPerPass = 32 / Shape::kChunks;
     const auto load = [&](int i, int from) {  // step i of this warp, whose page lane `from` knows
         if (i < mine) {
-            const int64_t key = k0 + 16 * (warp + static_cast<int64_t>(kDWarps) * i);
+            const int64_t key = step_key(i);
             const int pg = __shfl_sync(0xffffffffu, page, from);
             const int64_t off = pg * a.pg.page_stride + head * a.pg.head_stride +
                                 ((key & row_in_page_mask) + my_row) * a.pg.row_stride + 16 * my_chunk;
@@ -319,12 +329,14 @@ __global__ void __launch_bounds__(kDThreads, 4) attn8_decode_kernel(DecodeArgs p
     float *xs = p.scores + ((static_cast<int64_t>(b) * a.pg.n_kv + head) * p.s_len) * group + 8 * chunk;
 #pragma unroll
     for (int i = 0; i < kDStages - 1; ++i) load(i, i);
+    look_up_scales(0);  // behind the first copies: their latencies overlap
     int next_page_lane = kDStages - 1;
     float cur_kf = kf, cur_lv = lv, cur_iv = iv;  // of the window being computed; kf, lv, iv: of the window being loaded
     for (int i = 0; i < mine; ++i) {
         if (next_page_lane == 32) {  // every page of the window has been used: look the next one up
             cur_kf = kf, cur_lv = lv, cur_iv = iv;
-            look_up((i + kDStages - 1) / 32);
+            look_up_page((i + kDStages - 1) / 32);
+            look_up_scales((i + kDStages - 1) / 32);
             next_page_lane = 0;
         }
         load(i + kDStages - 1, next_page_lane++);
@@ -335,7 +347,7 @@ __global__ void __launch_bounds__(kDThreads, 4) attn8_decode_kernel(DecodeArgs p
         const float lv_i = __shfl_sync(0xffffffffu, same_window ? lv : cur_lv, i & 31);
         const float iv_i = __shfl_sync(0xffffffffu, same_window ? iv : cur_iv, i & 31);
         const uint32_t ks = ring + (i % kDStages) * 2 * Shape::kStep, vs = ks + Shape::kStep;
-        const int64_t key = k0 + 16 * (warp + static_cast<int64_t>(kDWarps) * i);
+        const int64_t key = step_key(i);
         // S^T: rows g, g + 8 of K, the lane's D / 4 dims
         float s[4] = {};
 #pragma unroll
@@ -496,53 +508,63 @@ __global__ void __launch_bounds__(kDThreads, 4) attn8_decode_kernel(DecodeArgs p
     cluster.sync();  // no CTA leaves while another may read its shared memory
 }
 
-// Joins the splits of a (sequence, KV head): block 0 the output, the others 1024 keys' weights each.
+// Joins the splits of a (sequence, KV head).  Blocks 0 .. group - 1: one head's output, the splits dealt to the
+// block's quarters; the others: the weights of 1024 keys each.
+constexpr int kJoinThreads = 512;
+
 template <int D>
-__global__ void __launch_bounds__(128) attn8_join_kernel(DecodeArgs p) {
-    extern __shared__ float sm[];  // [group] reference, [group] sum, [group][splits] factors
+__global__ void __launch_bounds__(kJoinThreads) attn8_join_kernel(DecodeArgs p) {
+    extern __shared__ float sm[];  // [heads][splits] factors
+    __shared__ float ref[128], sum[128], quarter[kJoinThreads];
     const AttnArgs &a = p.a;
     const int head = blockIdx.y, b = blockIdx.z, group = a.NH / a.pg.n_kv;
-    float *ref = sm, *sum = sm + group, *fac = sm + 2 * group;
+    const bool is_out = static_cast<int>(blockIdx.x) < group;
     pdl_wait();
     pdl_trigger();
     const int64_t n = visible(a.positions, b, 0, a.max_len);
-    const int64_t w0 = static_cast<int64_t>(blockIdx.x - 1) * 1024;
-    if (blockIdx.x > 0 && w0 >= n) return;
-    const float *base = p.parts + (static_cast<int64_t>(b) * a.pg.n_kv + head) * p.head_chunks * p.splits * 8 * (D + 2);
+    const int64_t w0 = (static_cast<int64_t>(blockIdx.x) - group) * 1024;
+    if (!is_out && w0 >= n) return;
+    constexpr int64_t kPart = 8 * (D + 2);
+    const float *base = p.parts + (static_cast<int64_t>(b) * a.pg.n_kv + head) * p.head_chunks * p.splits * kPart;
     const int lane = threadIdx.x & 31;
-    for (int h = threadIdx.x >> 5; h < group; h += 4) {
-        const float *st = base + static_cast<int64_t>(h >> 3) * p.splits * 8 * (D + 2) + 8 * D + (h & 7);
+    const int first = is_out ? blockIdx.x : 0, last = is_out ? first + 1 : group;
+    for (int h = first + (threadIdx.x >> 5); h < last; h += kJoinThreads / 32) {
+        const float *st = base + static_cast<int64_t>(h >> 3) * p.splits * kPart + 8 * D + (h & 7);
         float top = kRefStart, s = 0.0f;
-        for (int i = lane; i < p.splits; i += 32) top = fmaxf(top, st[static_cast<int64_t>(i) * 8 * (D + 2)]);
+        for (int i = lane; i < p.splits; i += 32) top = fmaxf(top, st[i * kPart]);
         top = warp_max(top);
         for (int i = lane; i < p.splits; i += 32) {
-            const float f = exp2_approx(st[static_cast<int64_t>(i) * 8 * (D + 2)] - top);
-            fac[h * p.splits + i] = f;
-            s = fmaf(st[static_cast<int64_t>(i) * 8 * (D + 2) + 8], f, s);
+            const float f = exp2_approx(st[i * kPart] - top);
+            sm[(h - first) * p.splits + i] = f;
+            s = fmaf(st[i * kPart + 8], f, s);
         }
         s = warp_sum(s);
-        if (lane == 0) ref[h] = top + log2f(s), sum[h] = s;
+        if (lane == 0) ref[h - first] = top + log2f(s), sum[h - first] = s;
     }
     __syncthreads();
-    if (blockIdx.x > 0) {
+    if (!is_out) {
         const float *xs = p.scores + ((static_cast<int64_t>(b) * a.pg.n_kv + head) * p.s_len) * group;
-        for (int64_t key = w0 + threadIdx.x; key < w0 + 1024 && key < n; key += 128) {
+        for (int64_t key = w0 + threadIdx.x; key < w0 + 1024 && key < n; key += kJoinThreads) {
             const int64_t at = b * p.w_sb + head * p.w_sh + key;
             const float w = key_weight(xs + key * group, ref, group);
             p.w_out[at] = w + (p.w_in && key < n - 1 ? p.w_in[at] : 0.0f);
         }
         return;
     }
-    for (int i = threadIdx.x; i < group * D; i += 128) {
-        const int h = i / D, d = i % D;
-        const float *src = base + static_cast<int64_t>(h >> 3) * p.splits * 8 * (D + 2) + (h & 7) * D + d;
-        float acc = 0.0f;
-        for (int s = 0; s < p.splits; ++s) acc = fmaf(src[static_cast<int64_t>(s) * 8 * (D + 2)], fac[h * p.splits + s], acc);
-        a.out[b * a.o_sb + (head * group + h) * a.o_sh + d] = __float2half(n > 0 ? acc / sum[h] : 0.0f);
+    constexpr int kShare = kJoinThreads / D;
+    const int d = threadIdx.x % D, q = threadIdx.x / D, h = first;
+    const float *src = base + static_cast<int64_t>(h >> 3) * p.splits * kPart + (h & 7) * D + d;
+    float acc = 0.0f;
+#pragma unroll 8
+    for (int s = q; s < p.splits; s += kShare) acc = fmaf(src[s * kPart], sm[s], acc);
+    quarter[threadIdx.x] = acc;
+    __syncthreads();
+    if (threadIdx.x < D) {
+        for (int i = 1; i < kShare; ++i) acc += quarter[i * D + d];
+        a.out[b * a.o_sb + (head * group + h) * a.o_sh + d] = __float2half(n > 0 ? acc / sum[0] : 0.0f);
+        if (a.lse && d == 0)
+            a.lse[static_cast<int64_t>(b) * a.NH + head * group + h] = n > 0 ? ref[0] * 0.6931471805599453f : -INFINITY;
     }
-    if (a.lse && threadIdx.x < group)
-        a.lse[static_cast<int64_t>(b) * a.NH + head * group + threadIdx.x] =
-            n > 0 ? ref[threadIdx.x] * 0.6931471805599453f : -INFINITY;
 }
 
 int check(const t2c_q8_pages *pages, const char *what, KvPages &pg, const int32_t *table, int64_t bt_stride,
@@ -596,13 +618,13 @@ DecodePlan decode_plan(int64_t B, int64_t NH, int64_t NK, int64_t D, int64_t max
         s = s < least ? least : s;
         s = s > most ? most : s;
     }
-    const int64_t bound = 12288 / group - 2;  // the joining kernel's shared memory
+    const int64_t bound = 10240 / group;  // the joining kernel's shared memory
     s = s > 128 ? 128 : s;
     s = s > bound ? bound : s;
     s = s < 1 ? 1 : s;
     r.splits = static_cast<int>(s);
     r.join = s > 8 || (weights && r.head_chunks > 1);
-    r.part_floats = r.join ? units * s * 8 * (D + 2) : 0;
+    r.part_floats = r.join ? units * s * 8 * (D + 2) : 0;  // a multiple of 4: the scores behind stay aligned
     r.floats = r.part_floats + (weights ? B * NK * max_len * group : 0);
     return r;
 }
@@ -648,10 +670,12 @@ extern "C" int t2c_attn_decode_q8(const t2c_q8_pages *pages, const void *q, int6
     if (!strides_ok(q, q_sb, q_sh, 0) || !strides_ok(out, o_sb, o_sh, 0))
         return set_error(T2C_EINVAL, "attn_decode_q8: q and out rows must be 16-byte aligned");
     if (splits < 0) return set_error(T2C_EINVAL, "attn_decode_q8: splits %lld", (long long)splits);
-    const int64_t D = pages->head_dim;
+    const int64_t D = pages->head_dim, group = NH / a.pg.n_kv;
+    if (group > 128) return set_error(T2C_EUNSUPPORTED, "attn_decode_q8: group %lld", (long long)group);
     const DecodePlan plan = decode_plan(B, NH, a.pg.n_kv, D, max_len, splits, weights_out != nullptr);
     if (plan.floats > 0 && (!workspace || workspace_floats < plan.floats))
         return set_error(T2C_ESCRATCH, "attn_decode_q8: workspace needs %lld floats", (long long)plan.floats);
+    if (!kv8_aligned(workspace, 16)) return set_error(T2C_EINVAL, "attn_decode_q8: workspace must be 16-byte aligned");
     if (a.pg.n_kv * plan.head_chunks > 65535) return set_error(T2C_EINVAL, "attn_decode_q8: bad shape");
     a.q = static_cast<const __half *>(q), a.q_sb = q_sb, a.q_sh = q_sh;
     a.out = static_cast<__half *>(out), a.o_sb = o_sb, a.o_sh = o_sh;
@@ -674,10 +698,9 @@ extern "C" int t2c_attn_decode_q8(const t2c_q8_pages *pages, const void *q, int6
                     dim3(kDThreads), smem, p.join ? 1u : static_cast<unsigned>(p.splits), s, p);
     if (rc != T2C_OK || !p.join) return rc;
     const int64_t chunks = weights_out ? (max_len + 1023) / 1024 : 0;
-    const int64_t group = NH / a.pg.n_kv;
     return kv8_launch("attn_decode_q8 join", D == 128 ? attn8_join_kernel<128> : attn8_join_kernel<64>,
-                      dim3(static_cast<unsigned>(1 + chunks), static_cast<unsigned>(a.pg.n_kv), static_cast<unsigned>(B)),
-                      dim3(128), static_cast<size_t>(group * (p.splits + 2) * 4), 1, s, p);
+                      dim3(static_cast<unsigned>(group + chunks), static_cast<unsigned>(a.pg.n_kv), static_cast<unsigned>(B)),
+                      dim3(kJoinThreads), static_cast<size_t>((weights_out ? group : 1) * p.splits * 4), 1, s, p);
 }
 
 extern "C" int64_t t2c_attn_prefill_q8_workspace(const t2c_q8_pages *pages, int64_t bt_width, int64_t B, int64_t T,
