@@ -1,6 +1,7 @@
 // Attention over the paged KV cache in 8 bits: one warp per query row, one
 // lane per key for the scores, lanes across head_dim for the values.
 #include <cooperative_groups.h>
+#include <cudaTypedefs.h>
 
 #include "kv8.cuh"
 
@@ -137,52 +138,51 @@ __global__ void __launch_bounds__(32) attn8_weights_kernel(AttnArgs a, const flo
 }
 
 // ------------------------------------------------------------------ one token per sequence
-// A warp walks its share of a sequence's keys in steps of 16.  Codes arrive by 16-byte cp.async in a ring of
-// kDStages steps that only this warp reads (no CTA barrier in the loop); a step's 16 keys lie in one block, so one K
-// and one V scale serve it.  Both products run on mma.m16n8k16 with the up to 8 heads of a group as the n side, so
-// that a cached byte is expanded once for all of them:
+// Work is cut into tiles of 64 keys of one (sequence, KV head, 8 heads of the group); a fixed number of CTAs takes
+// equal runs of the list of tiles (whatever the sequences' lengths), so a run covers the end of one unit, whole
+// units, and the beginning of another: units that a CTA covers wholly it finishes itself, the others a second kernel
+// joins.  Short caches take one cluster per unit instead, joined in distributed shared memory by the same launch.
+// Inside a CTA a warp takes every fourth 16 keys, in a ring of kDStages steps of its own: TMA boxes of 16 rows
+// (swizzled, so that the fragment reads below hit each bank once), one mbarrier per stage, no CTA barrier in the
+// loop.  16 keys lie in one block of the cache, so one K and one V scale serve a step.  Both products run on
+// mma.m16n8k16 with the heads as the n side, so that a cached byte is expanded once for all heads of the group:
 //   S^T [16 keys x 8 heads] = K Q^T,   O^T [16 dims x 8 heads] += V^T P^T.
 // Codes become fp16 exactly.  The scales stay in fp32: x = s * (k scale * softmax scale * log2 e), and the V scale
 // joins the exponent, P = 2^(x + log2 vs - m), so that P q_v needs no scaled V; the softmax sum takes P / vs.  m is a
 // running reference per head, moved (and O, l rescaled) only when some exponent passes 14: P stays in fp16's range,
-// and its one rounding to fp16, shared with every attention kernel here, is the only one before the output.
-// What bounds it: HBM.
+// and its one rounding to fp16, which the tensor core asks for, is the only one before the output's.
 constexpr int kDWarps = 4;
 constexpr int kDStages = 3;
 constexpr int kDThreads = 32 * kDWarps;
+constexpr int kDTile = 16 * kDWarps;
 constexpr float kRefStart = -1e30f;  // below any finite score: the first step moves it
 constexpr float kRefTop = 14.0f;     // P <= 2^14
 constexpr float kRefDrop = 8.0f;     // a moved reference leaves the largest P at 2^8
 
 template <int D>
 struct DecodeShape {
-    static constexpr int kChunks = D / 16;                     // 16-byte chunks of a row
-    static constexpr int kStep = 16 * D;                       // bytes of K (or V) per step
+    static constexpr int kStep = 16 * D;  // bytes of K (or V) per step
     static constexpr int kRing = kDWarps * kDStages * 2 * kStep;
-    // 16-byte slot of chunk c of row r: the fragment reads below touch each bank once per 8 lanes
-    static __device__ __forceinline__ uint32_t slot(int r, int c) {
-        if constexpr (D == 128) {
-            return static_cast<uint32_t>(r * 8 + (c ^ (r & 7)));
-        } else {
-            const int j = r >> 1;
-            return static_cast<uint32_t>(j * 8 + ((c & 1) | (((c >> 1) ^ ((j >> 1) & 1)) << 1) | (((r ^ j) & 1) << 2)));
-        }
+    static constexpr int kPart = 8 * (D + 2);  // floats of a partial result: O, m, l of 8 heads
+    // byte offset of 16-byte chunk c of row r in a TMA box (128- or 64-byte swizzle); chunk c + 2 j is at ^ (32 j)
+    static __device__ __forceinline__ uint32_t at(int r, int c) {
+        return static_cast<uint32_t>(D == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
     }
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// Four 8 x 16-byte tiles, a row's address from each lane: lane (g, t) gets bytes 4t .. 4t + 3 of each tile's row g, or
+// transposed by byte pairs: bytes 2g, 2g + 1 of rows 2t and 2t + 1.
+__device__ __forceinline__ void ldsm(uint32_t v[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "r"(a)
+                 : "memory");
 }
-
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-    return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-    return v;
+__device__ __forceinline__ void ldsm_trans(uint32_t v[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "r"(a)
+                 : "memory");
 }
 
 __device__ __forceinline__ void mma16816(float c[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -217,23 +217,18 @@ __device__ __forceinline__ float exp2_approx(float x) {
 
 struct DecodeArgs {
     AttnArgs a;
-    int splits, head_chunks;      // CTAs per (sequence, KV head); chunks of 8 heads of a group
-    float *parts;                 // [B][n_kv * head_chunks][splits][8][D + 2]: O, m, l
-    float *scores;                // [B][n_kv][s_len][group] x in log2 units, where the weights are wanted
+    int splits;       // CTAs per unit in a cluster; 0: tile runs, joined by the second kernel
+    int head_chunks;  // chunks of 8 heads of a group
+    int ctas;         // of the tile runs
+    float *parts;     // [2 * ctas][kPart]
+    int2 *unit_ctas;  // [B * n_kv * head_chunks] first and last CTA of a unit's tiles
+    float *unit_lse;  // [B][NH] in log2 units, of units one CTA finished; where the weights are wanted
+    float *scores;    // [B][n_kv][s_len][group] x in log2 units, where the weights are wanted
     int64_t s_len;
     const float *w_in;
     float *w_out;
     int64_t w_sb, w_sh;
-    bool join;                    // a second kernel joins the splits
 };
-
-// The keys that CTA `s` of `splits` takes of n: multiples of 16, at least 64 a CTA.
-__device__ __forceinline__ void split_range(int64_t n, int splits, int s, int64_t &k0, int64_t &k1) {
-    int64_t chunk = (n + splits - 1) / splits;
-    chunk = chunk < 64 ? 64 : (chunk + 15) & ~int64_t(15);
-    k0 = s * chunk < n ? s * chunk : n;
-    k1 = k0 + chunk < n ? k0 + chunk : n;
-}
 
 __device__ __forceinline__ float key_weight(const float *x, const float *lse2, int group) {
     float sum = 0.0f;
@@ -249,302 +244,423 @@ __device__ __forceinline__ float key_weight(const float *x, const float *lse2, i
     return sum;
 }
 
+// Tiles of sequence b: an empty sequence keeps one, whose CTA writes its zeros.
+__device__ __forceinline__ int seq_tiles(const AttnArgs &a, int b) {
+    const int64_t n = min(static_cast<int64_t>(a.positions[b]) + 1, a.max_len);
+    return n <= kDTile ? 1 : static_cast<int>((n + kDTile - 1) / kDTile);
+}
+
 template <int D>
-__global__ void __launch_bounds__(kDThreads, 4) attn8_decode_kernel(DecodeArgs p) {
+__global__ void __launch_bounds__(kDThreads, 4) attn8_decode_kernel(const __grid_constant__ CUtensorMap k_map,
+                                                                    const __grid_constant__ CUtensorMap v_map,
+                                                                    const __grid_constant__ DecodeArgs p) {
     using Shape = DecodeShape<D>;
     constexpr int kWords = D / 16;  // K: 32-bit words per lane and row = k steps; V: m tiles
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ uint64_t full[kDWarps][kDStages];
+    __shared__ float4 metas[kDWarps][64];  // of two windows of 32 steps: K factor, log2 V scale, 1 / V scale, page
     __shared__ float st_m[kDWarps][8], st_l[kDWarps][8], cta_m[8], cta_l[8], lse2[8];
     const AttnArgs &a = p.a;
     cg::cluster_group cluster = cg::this_cluster();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x;
-    const int head = blockIdx.y / p.head_chunks, chunk = blockIdx.y % p.head_chunks;
-    const int b = blockIdx.z;
-    const int group = a.NH / a.pg.n_kv, heads = min(8, group - 8 * chunk), h0 = head * group + 8 * chunk;
+    const int group = a.NH / a.pg.n_kv;
+    const int units = a.pg.n_kv * p.head_chunks;  // of a sequence
+    if (threadIdx.x < kDWarps * kDStages) mbar_init(&full[0][0] + threadIdx.x, 1);
+    fence_mbar_init();
+    __syncthreads();
+    if (smem_u32(smem) & 1023u) {  // the swizzle needs it: report, compute nothing
+        if (threadIdx.x == 0) report_device_error(T2C_EUNSUPPORTED);
+        return;
+    }
     pdl_wait();
     pdl_trigger();
-    const int64_t n = visible(a.positions, b, 0, a.max_len);
-    int64_t k0, k1;
-    split_range(n, p.splits, split, k0, k1);
-    const int32_t *bt = a.table + b * a.t_stride;
-    const int steps = static_cast<int>((k1 - k0 + 15) >> 4);            // of the CTA
-    const int mine = steps > warp ? (steps - warp + kDWarps - 1) / kDWarps : 0;  // of this warp: warp, warp + 4, ..
 
-    // ---- the lane's step of a window of 32: page and scales, looked up a window ahead of their use
-    int page = 0;
-    float kf = 0.0f, lv = 0.0f, iv = 0.0f;
-    const auto step_key = [&](int i) { return k0 + 16 * (warp + static_cast<int64_t>(kDWarps) * i); };
-    const auto look_up_page = [&](int window) {
-        const int i = window * 32 + lane;
-        if (i < mine) page = max(kv8_page(a.pg, bt, step_key(i)), 0);
-    };
-    const auto look_up_scales = [&](int window) {
-        const int i = window * 32 + lane;
-        if (i >= mine) return;
-        const int64_t so = kv8_scale_offset(a.pg, page, head, step_key(i));
-        kf = __half2float(a.pg.ks[so]) * a.scale_log2;
-        const float vs = __half2float(a.pg.vs[so]);
-        // a block of scale 0 has values 0: any exponent adds nothing to O, the least scale's moves no reference
-        lv = vs == 0.0f ? -24.0f : log2f(vs);
-        iv = vs == 0.0f ? 16777216.0f : 1.0f / vs;
-    };
-    look_up_page(0);
-
-    // ---- Q^T fragments: k step i, lane (g, t): head g, dims D/4 t + 4 i + {0, 2} and {1, 3}
-    uint32_t qf[kWords][2];
-    {
-        const uint32_t *q = reinterpret_cast<const uint32_t *>(a.q + b * a.q_sb + (h0 + min(g, heads - 1)) * a.q_sh) + D / 8 * t;
+    // ---- this CTA's tiles: of its cluster's unit, or its run of all tiles
+    int b = 0, unit = 0, t0 = 0, left = 0, unit_tiles = 1;
+    if (p.splits > 0) {
+        b = blockIdx.z, unit = blockIdx.y;
+        unit_tiles = seq_tiles(a, b);
+        const int per = (unit_tiles + p.splits - 1) / p.splits;
+        t0 = min(per * static_cast<int>(blockIdx.x), unit_tiles);
+        left = min(per, unit_tiles - t0);
+    } else {
+        int total = 0;
+        for (int i = lane; i < a.B; i += 32) total += seq_tiles(a, i);
+        total = units * __reduce_add_sync(0xffffffffu, total);
+        const int ctas = min(p.ctas, total);  // each has a tile or more
+        const int c = blockIdx.x;
+        if (c >= ctas) return;
+        const int per = total / ctas, extra = total % ctas;
+        const int from = c * per + min(c, extra);
+        left = per + (c < extra ? 1 : 0);
+        // 32 sequences at a time: the one that holds tile `from`
+        int before = 0;
+        for (int base = 0; base < a.B; base += 32) {
+            const int mine = base + lane < a.B ? units * seq_tiles(a, base + lane) : 0;
+            int incl = mine;
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-            const uint32_t lo = g < heads ? q[2 * i] : 0u, hi = g < heads ? q[2 * i + 1] : 0u;
-            qf[i][0] = __byte_perm(lo, hi, 0x5410);
-            qf[i][1] = __byte_perm(lo, hi, 0x7632);
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, before + incl > from);
+            if (past) {
+                const int i = __ffs(past) - 1;
+                b = base + i;
+                unit_tiles = __shfl_sync(0xffffffffu, mine, i) / units;
+                const int local = from - (before + __shfl_sync(0xffffffffu, incl - mine, i));
+                unit = local / unit_tiles;
+                t0 = local % unit_tiles;
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, incl, 31);
         }
     }
 
     const uint32_t ring = smem_u32(smem) + warp * (kDStages * 2 * Shape::kStep);
-    const int64_t row_in_page_mask = (1 << a.pg.page_log2) - 1;
-    const int my_row = lane / Shape::kChunks, my_chunk = lane % Shape::kChunks;
-    constexpr int kRowsPerPass = 32 / Shape::kChunks;
-    const auto load = [&](int i, int from) {  // step i of this warp, whose page lane `from` knows
-        if (i < mine) {
-            const int64_t key = step_key(i);
-            const int pg = __shfl_sync(0xffffffffu, page, from);
-            const int64_t off = pg * a.pg.page_stride + head * a.pg.head_stride +
-                                ((key & row_in_page_mask) + my_row) * a.pg.row_stride + 16 * my_chunk;
-            const uint32_t st = ring + (i % kDStages) * 2 * Shape::kStep;
-#pragma unroll
-            for (int r = 0; r < 16 / kRowsPerPass; ++r) {
-                const uint32_t dst = st + 16 * Shape::slot(my_row + r * kRowsPerPass, my_chunk);
-                cp_async16(dst, a.pg.k + off + r * kRowsPerPass * a.pg.row_stride);
-                cp_async16(dst + Shape::kStep, a.pg.v + off + r * kRowsPerPass * a.pg.row_stride);
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
+    const int page_mask = (1 << a.pg.page_log2) - 1;
+    const uint32_t frag = Shape::at(lane & 15, lane >> 4);  // the lane's row of a fragment load: 16 rows, 2 chunks
+    uint32_t phases = 0;  // of this warp's stages
+    bool failed = false;
+    do {
+        const int head = unit / p.head_chunks, chunk = unit % p.head_chunks;
+        const int heads = min(8, group - 8 * chunk), h0 = head * group + 8 * chunk;
+        const int64_t n = visible(a.positions, b, 0, a.max_len);
+        const int t1 = min(t0 + left, unit_tiles);
+        const int64_t k0 = min(static_cast<int64_t>(t0) * kDTile, n), k1 = min(static_cast<int64_t>(t1) * kDTile, n);
+        const int32_t *bt = a.table + b * a.t_stride;
+        const int steps = static_cast<int>((k1 - k0 + 15) >> 4);                     // of the CTA
+        const int mine = steps > warp ? (steps - warp + kDWarps - 1) / kDWarps : 0;  // of this warp: warp, warp + 4, ..
+        const auto step_key = [&](int i) { return k0 + 16 * warp + static_cast<int64_t>(kDTile) * i; };
+        float4 *meta = metas[warp];
 
-    float o[kWords][4] = {};
-    float m[2] = {kRefStart, kRefStart}, l[2] = {0.0f, 0.0f};
-    float *xs = p.scores + ((static_cast<int64_t>(b) * a.pg.n_kv + head) * p.s_len) * group + 8 * chunk;
+        // pages and scales of 32 steps: page, then scales, then the factors, each a few steps after the one before
+        int next_page = 0;
+        __half next_ks, next_vs;
+        const auto look_page = [&](int window) {
+            const int i = window * 32 + lane;
+            next_page = i < mine ? max(kv8_page(a.pg, bt, step_key(i)), 0) : 0;
+        };
+        const auto look_scales = [&](int window) {
+            const int i = window * 32 + lane;
+            const int64_t so = i < mine ? kv8_scale_offset(a.pg, next_page, head, step_key(i)) : 0;
+            next_ks = a.pg.ks[so];
+            next_vs = a.pg.vs[so];
+        };
+        const auto store_meta = [&](int window) {
+            const float vs = __half2float(next_vs);
+            // a block of scale 0 has values 0: any exponent adds nothing to O, the least scale's moves no reference
+            meta[(window & 1) * 32 + lane] =
+                make_float4(__half2float(next_ks) * a.scale_log2, vs == 0.0f ? -24.0f : log2f(vs),
+                            vs == 0.0f ? 16777216.0f : 1.0f / vs, __int_as_float(next_page));
+            __syncwarp();
+        };
+        const auto load = [&](int i, int stage, int page) {  // by one lane
+            const uint32_t st = ring + stage * 2 * Shape::kStep;
+            mbar_arrive_expect_tx(&full[warp][stage], 2 * Shape::kStep);
+            const int row = static_cast<int>(step_key(i)) & page_mask;
+            tma_load_4d(st, &k_map, 0, row, head, page, &full[warp][stage]);
+            tma_load_4d(st + Shape::kStep, &v_map, 0, row, head, page, &full[warp][stage]);
+        };
+        look_page(0);
 #pragma unroll
-    for (int i = 0; i < kDStages - 1; ++i) load(i, i);
-    look_up_scales(0);  // behind the first copies: their latencies overlap
-    int next_page_lane = kDStages - 1;
-    float cur_kf = kf, cur_lv = lv, cur_iv = iv;  // of the window being computed; kf, lv, iv: of the window being loaded
-    for (int i = 0; i < mine; ++i) {
-        if (next_page_lane == 32) {  // every page of the window has been used: look the next one up
-            cur_kf = kf, cur_lv = lv, cur_iv = iv;
-            look_up_page((i + kDStages - 1) / 32);
-            look_up_scales((i + kDStages - 1) / 32);
-            next_page_lane = 0;
+        for (int i = 0; i < kDStages; ++i) {
+            const int page = __shfl_sync(0xffffffffu, next_page, i);
+            if (lane == 0 && i < mine) load(i, i, page);
         }
-        load(i + kDStages - 1, next_page_lane++);
-        asm volatile("cp.async.wait_group %0;" ::"n"(kDStages - 1) : "memory");
-        __syncwarp();
-        const bool same_window = (i + kDStages - 1) / 32 == i / 32;
-        const float kf_i = __shfl_sync(0xffffffffu, same_window ? kf : cur_kf, i & 31);
-        const float lv_i = __shfl_sync(0xffffffffu, same_window ? lv : cur_lv, i & 31);
-        const float iv_i = __shfl_sync(0xffffffffu, same_window ? iv : cur_iv, i & 31);
-        const uint32_t ks = ring + (i % kDStages) * 2 * Shape::kStep, vs = ks + Shape::kStep;
-        const int64_t key = step_key(i);
-        // S^T: rows g, g + 8 of K, the lane's D / 4 dims
-        float s[4] = {};
+        look_scales(0);
+
+        // ---- Q^T fragments: k step i, lane (g, t): head g, dims 16 i + 4 t + {0, 2} and {1, 3}
+        uint32_t qf[kWords][2];
+        {
+            const uint32_t *q = reinterpret_cast<const uint32_t *>(a.q + b * a.q_sb + (h0 + min(g, heads - 1)) * a.q_sh) + 2 * t;
 #pragma unroll
-        for (int c = 0; c < kWords / 4; ++c) {
-            const uint4 lo = lds128(ks + 16 * Shape::slot(g, kWords / 4 * t + c));
-            const uint4 hi = lds128(ks + 16 * Shape::slot(g + 8, kWords / 4 * t + c));
-            const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t a0, a1, a2, a3;
-                unpack_word(wl[j], a0, a2);
-                unpack_word(wh[j], a1, a3);
-                mma16816(s, a0, a1, a2, a3, qf[4 * c + j][0], qf[4 * c + j][1]);
+            for (int i = 0; i < kWords; ++i) {
+                const uint32_t lo = g < heads ? q[8 * i] : 0u, hi = g < heads ? q[8 * i + 1] : 0u;
+                qf[i][0] = __byte_perm(lo, hi, 0x5410);
+                qf[i][1] = __byte_perm(lo, hi, 0x7632);
             }
         }
-        // s[0], s[1]: key g, heads 2t, 2t + 1; s[2], s[3]: key g + 8
-        const bool in0 = key + g < k1, in1 = key + g + 8 < k1;
-        if (p.w_out) {
-            float *x0 = xs + (key + g) * group + 2 * t, *x1 = x0 + 8 * group;
-            if (in0 && 2 * t < heads) x0[0] = s[0] * kf_i;
-            if (in0 && 2 * t + 1 < heads) x0[1] = s[1] * kf_i;
-            if (in1 && 2 * t < heads) x1[0] = s[2] * kf_i;
-            if (in1 && 2 * t + 1 < heads) x1[1] = s[3] * kf_i;
+        store_meta(0);
+
+        float o[kWords][4] = {};
+        float m[2] = {kRefStart, kRefStart}, l[2] = {0.0f, 0.0f};
+        float *xs = p.scores + ((static_cast<int64_t>(b) * a.pg.n_kv + head) * p.s_len) * group + 8 * chunk;
+        float *xp = xs + (k0 + 16 * warp + g) * group + 2 * t;
+        int rem = static_cast<int>(k1 - k0) - 16 * warp - g;  // keys from this lane's first one to the end
+#pragma unroll 1
+        for (int i0 = 0; i0 < mine && !failed; i0 += kDStages) {
+#pragma unroll
+            for (int st = 0; st < kDStages; ++st) {
+                const int i = i0 + st;
+                if (i >= mine) break;
+                if ((i | 31) + 1 < mine) {  // the next window's look-ups, spread over this one's steps
+                    const int at = i & 31;
+                    if (at == 4) look_page(i / 32 + 1);
+                    if (at == 12) look_scales(i / 32 + 1);
+                    if (at == 20) store_meta(i / 32 + 1);
+                }
+                const bool arrived = mbar_wait(&full[warp][st], (phases >> st) & 1u);
+                if (!__all_sync(0xffffffffu, arrived)) {
+                    failed = true;
+                    break;
+                }
+                phases ^= 1u << st;
+                const float4 f = meta[i & 63];
+                const uint32_t ks = ring + st * 2 * Shape::kStep, vs = ks + Shape::kStep;
+                // S^T: 16 dims a k step; two chains
+                float s[4] = {}, s2[4] = {};
+#pragma unroll
+                for (int c = 0; c < kWords; c += 2) {
+                    uint32_t w[4], a0, a1, a2, a3;
+                    ldsm(w, ks + (frag ^ (16 * c)));
+                    unpack_word(w[0], a0, a2);
+                    unpack_word(w[1], a1, a3);
+                    mma16816(s, a0, a1, a2, a3, qf[c][0], qf[c][1]);
+                    unpack_word(w[2], a0, a2);
+                    unpack_word(w[3], a1, a3);
+                    mma16816(s2, a0, a1, a2, a3, qf[c + 1][0], qf[c + 1][1]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[e] += s2[e];
+                // s[0], s[1]: key g, heads 2t, 2t + 1; s[2], s[3]: key g + 8
+                const bool in0 = rem > 0, in1 = rem > 8;
+                if (p.w_out) {
+                    if (in0 && 2 * t < heads) xp[0] = s[0] * f.x;
+                    if (in0 && 2 * t + 1 < heads) xp[1] = s[1] * f.x;
+                    if (in1 && 2 * t < heads) xp[8 * group] = s[2] * f.x;
+                    if (in1 && 2 * t + 1 < heads) xp[8 * group + 1] = s[3] * f.x;
+                    xp += kDTile * group;
+                }
+                rem -= kDTile;
+                float y[4];
+                y[0] = in0 ? fmaf(s[0], f.x, f.y - m[0]) : -INFINITY;
+                y[1] = in0 ? fmaf(s[1], f.x, f.y - m[1]) : -INFINITY;
+                y[2] = in1 ? fmaf(s[2], f.x, f.y - m[0]) : -INFINITY;
+                y[3] = in1 ? fmaf(s[3], f.x, f.y - m[1]) : -INFINITY;
+                if (__any_sync(0xffffffffu, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) > kRefTop)) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float top = fmaxf(in0 ? fmaf(s[e], f.x, f.y) : -INFINITY, in1 ? fmaf(s[2 + e], f.x, f.y) : -INFINITY);
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        const float ref = top - m[e] > kRefTop ? top - kRefDrop : m[e];
+                        const float corr = exp2_approx(m[e] - ref);
+                        l[e] *= corr;
+#pragma unroll
+                        for (int w = 0; w < kWords; ++w) {
+                            o[w][e] *= corr;
+                            o[w][2 + e] *= corr;
+                        }
+                        m[e] = ref;
+                        y[e] = in0 ? fmaf(s[e], f.x, f.y - ref) : -INFINITY;
+                        y[2 + e] = in1 ? fmaf(s[2 + e], f.x, f.y - ref) : -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = exp2_approx(y[e]);
+                l[0] = fmaf(y[0] + y[2], f.z, l[0]);
+                l[1] = fmaf(y[1] + y[3], f.z, l[1]);
+                const uint32_t b0 = transpose8x8(half2_bits(__floats2half2_rn(y[0], y[1])));
+                const uint32_t b1 = transpose8x8(half2_bits(__floats2half2_rn(y[2], y[3])));
+                // O^T: m tile c, lane (g, t): dims 16 c + 2 g + {0, 1} of keys 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+                for (int c = 0; c < kWords; c += 2) {
+                    uint32_t w[4], a0, a1, a2, a3;
+                    ldsm_trans(w, vs + (frag ^ (16 * c)));
+                    unpack_word(w[0], a0, a1);
+                    unpack_word(w[1], a2, a3);
+                    mma16816(o[c], a0, a1, a2, a3, b0, b1);
+                    unpack_word(w[2], a0, a1);
+                    unpack_word(w[3], a2, a3);
+                    mma16816(o[c + 1], a0, a1, a2, a3, b0, b1);
+                }
+                __syncwarp();  // the stage is read before it is refilled
+                if (lane == 0 && i + kDStages < mine)
+                    load(i + kDStages, st, __float_as_int(meta[(i + kDStages) & 63].w));
+            }
         }
-        float y[4];
-        y[0] = in0 ? fmaf(s[0], kf_i, lv_i - m[0]) : -INFINITY;
-        y[1] = in0 ? fmaf(s[1], kf_i, lv_i - m[1]) : -INFINITY;
-        y[2] = in1 ? fmaf(s[2], kf_i, lv_i - m[0]) : -INFINITY;
-        y[3] = in1 ? fmaf(s[3], kf_i, lv_i - m[1]) : -INFINITY;
-        if (__any_sync(0xffffffffu, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) > kRefTop)) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
+            if (g == 0) {
+                st_m[warp][2 * t + e] = m[e];
+                st_l[warp][2 * t + e] = l[e];
+            }
+        }
+        failed = __syncthreads_or(failed);  // every warp is done with its ring
+        if (failed) {
+            if (threadIdx.x == 0) report_device_error(T2C_ETIMEOUT);
+            break;
+        }
+        // ---- the CTA's O [8 heads][D]: each warp's share at the common reference, summed
+        constexpr int kPitch = D + 4;  // floats per (warp, head) row
+        float *part = reinterpret_cast<float *>(smem);
+        if (threadIdx.x < 8) {
+            float top = kRefStart, sum = 0.0f;
+            for (int w = 0; w < kDWarps; ++w) top = fmaxf(top, st_m[w][threadIdx.x]);
+            for (int w = 0; w < kDWarps; ++w) sum += st_l[w][threadIdx.x] * exp2_approx(st_m[w][threadIdx.x] - top);
+            cta_m[threadIdx.x] = top;
+            cta_l[threadIdx.x] = sum;
+            lse2[threadIdx.x] = top + log2f(sum);
+        }
+        {
+            float top[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                float top = fmaxf(in0 ? fmaf(s[e], kf_i, lv_i) : -INFINITY, in1 ? fmaf(s[2 + e], kf_i, lv_i) : -INFINITY);
+                top[e] = kRefStart;
+                for (int w = 0; w < kDWarps; ++w) top[e] = fmaxf(top[e], st_m[w][2 * t + e]);
+                top[e] = exp2_approx(m[e] - top[e]);
+            }
 #pragma unroll
-                for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                const float ref = top - m[e] > kRefTop ? top - kRefDrop : m[e];
-                const float corr = exp2_approx(m[e] - ref);
-                l[e] *= corr;
-#pragma unroll
-                for (int w = 0; w < kWords; ++w) {
-                    o[w][e] *= corr;
-                    o[w][2 + e] *= corr;
-                }
-                m[e] = ref;
-                y[e] = in0 ? fmaf(s[e], kf_i, lv_i - ref) : -INFINITY;
-                y[2 + e] = in1 ? fmaf(s[2 + e], kf_i, lv_i - ref) : -INFINITY;
+            for (int w = 0; w < kWords; ++w) {
+                const int d = 16 * w + 2 * g;
+                float *r0 = part + (warp * 8 + 2 * t) * kPitch + d, *r1 = r0 + kPitch;
+                *reinterpret_cast<float2 *>(r0) = make_float2(o[w][0] * top[0], o[w][2] * top[0]);
+                *reinterpret_cast<float2 *>(r1) = make_float2(o[w][1] * top[1], o[w][3] * top[1]);
             }
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = exp2_approx(y[e]);
-        l[0] = fmaf(y[0] + y[2], iv_i, l[0]);
-        l[1] = fmaf(y[1] + y[3], iv_i, l[1]);
-        const uint32_t b0 = transpose8x8(half2_bits(__floats2half2_rn(y[0], y[1])));
-        const uint32_t b1 = transpose8x8(half2_bits(__floats2half2_rn(y[2], y[3])));
-        // O^T: lane (g, t) has dims D/8 g .. of keys 2t, 2t + 1, 2t + 8, 2t + 9
-        uint32_t v[4][kWords / 2];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = 2 * t + (r & 1) + 8 * (r >> 1);
-            if constexpr (D == 128) {
-                const uint4 x = lds128(vs + 16 * Shape::slot(row, g));
-                v[r][0] = x.x, v[r][1] = x.y, v[r][2] = x.z, v[r][3] = x.w;
-            } else {
-                const uint2 x = lds64(vs + 16 * Shape::slot(row, g >> 1) + 8 * (g & 1));
-                v[r][0] = x.x, v[r][1] = x.y;
-            }
-        }
-#pragma unroll
-        for (int w = 0; w < kWords / 2; ++w) {
-            uint32_t a0, a1, a2, a3;
-            unpack_word(__byte_perm(v[0][w], v[1][w], 0x5410), a0, a1);  // dim 4w: keys 2t, 2t + 1; dim 4w + 1
-            unpack_word(__byte_perm(v[2][w], v[3][w], 0x5410), a2, a3);
-            mma16816(o[2 * w], a0, a1, a2, a3, b0, b1);
-            unpack_word(__byte_perm(v[0][w], v[1][w], 0x7632), a0, a1);  // dims 4w + 2, 4w + 3
-            unpack_word(__byte_perm(v[2][w], v[3][w], 0x7632), a2, a3);
-            mma16816(o[2 * w + 1], a0, a1, a2, a3, b0, b1);
-        }
-        __syncwarp();  // the stage is read before it is refilled
-    }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
-        if (g == 0) {
-            st_m[warp][2 * t + e] = m[e];
-            st_l[warp][2 * t + e] = l[e];
-        }
-    }
-    __syncthreads();  // every warp is done with its ring
-    // ---- the CTA's O [8 heads][D]: each warp's share at its own reference, summed by dim
-    constexpr int kPitch = D + 4;  // floats per (warp, head) row
-    float *part = reinterpret_cast<float *>(smem);
-    if (threadIdx.x < 8) {
-        float top = kRefStart, sum = 0.0f;
-        for (int w = 0; w < kDWarps; ++w) top = fmaxf(top, st_m[w][threadIdx.x]);
-        for (int w = 0; w < kDWarps; ++w) sum += st_l[w][threadIdx.x] * exp2_approx(st_m[w][threadIdx.x] - top);
-        cta_m[threadIdx.x] = top;
-        cta_l[threadIdx.x] = sum;
-    }
-    __syncthreads();
-    const float f0 = exp2_approx(m[0] - cta_m[2 * t]), f1 = exp2_approx(m[1] - cta_m[2 * t + 1]);
-#pragma unroll
-    for (int w = 0; w < kWords; ++w) {
-        const int d = D / 8 * g + 2 * w;
-        float *r0 = part + (warp * 8 + 2 * t) * kPitch + d, *r1 = r0 + kPitch;
-        *reinterpret_cast<float2 *>(r0) = make_float2(o[w][0] * f0, o[w][2] * f0);
-        *reinterpret_cast<float2 *>(r1) = make_float2(o[w][1] * f1, o[w][3] * f1);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 8 * D; i += kDThreads) {
-        float *r = part + (i / D) * kPitch + i % D;
-        float sum = r[0];
-        for (int w = 1; w < kDWarps; ++w) sum += r[w * 8 * kPitch];
-        r[0] = sum;
-    }
-    if (p.join) {
-        float *dst = p.parts + ((static_cast<int64_t>(b) * gridDim.y + blockIdx.y) * p.splits + split) * 8 * (D + 2);
         __syncthreads();
-        for (int i = threadIdx.x; i < heads * D; i += kDThreads) dst[i] = part[(i / D) * kPitch + i % D];
-        if (threadIdx.x < heads) {
-            dst[8 * D + threadIdx.x] = cta_m[threadIdx.x];
-            dst[8 * D + 8 + threadIdx.x] = cta_l[threadIdx.x];
+        const bool whole = t0 == 0 && t1 == unit_tiles;  // and so finished here
+        const bool shared = p.splits > 1;
+        float *dst = p.parts + (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0 ? 1 : 0)) * Shape::kPart;
+        for (int i = threadIdx.x; i < heads * D; i += kDThreads) {
+            const int h = i / D, d = i % D;
+            float *r = part + h * kPitch + d;
+            float sum = r[0];
+            for (int w = 1; w < kDWarps; ++w) sum += r[w * 8 * kPitch];
+            if (shared)
+                r[0] = sum;
+            else if (whole)
+                a.out[b * a.o_sb + (h0 + h) * a.o_sh + d] = __float2half(n > 0 ? sum / cta_l[h] : 0.0f);
+            else
+                dst[i] = sum;
         }
-        return;
-    }
-    // ---- the cluster's CTAs hold all of the sequence's keys: join through distributed shared memory
-    cluster.sync();
+        if (!shared && threadIdx.x < heads) {
+            const int64_t row = static_cast<int64_t>(b) * a.NH + h0 + threadIdx.x;
+            if (whole) {
+                if (a.lse) a.lse[row] = n > 0 ? lse2[threadIdx.x] * 0.6931471805599453f : -INFINITY;
+                if (p.w_out && p.splits == 0) p.unit_lse[row] = lse2[threadIdx.x];
+            } else {
+                dst[8 * D + threadIdx.x] = cta_m[threadIdx.x];
+                dst[8 * D + 8 + threadIdx.x] = cta_l[threadIdx.x];
+            }
+        }
+        if (p.splits > 0) break;
+        if (threadIdx.x == 0) {
+            int2 *at = p.unit_ctas + static_cast<int64_t>(b) * units + unit;
+            if (t0 == 0) at->x = blockIdx.x;
+            if (t1 == unit_tiles) at->y = blockIdx.x;
+        }
+        // the next unit; its copies overwrite what the loop above read
+        left -= t1 - t0;
+        t0 = 0;
+        if (++unit == units && left > 0) {
+            unit = 0;
+            ++b;
+            unit_tiles = seq_tiles(a, b);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
+    } while (left > 0);
+    if (p.splits == 0) return;
+    // ---- the cluster's CTAs hold all of the unit's keys: join through distributed shared memory
+    const int head = unit / p.head_chunks, chunk = unit % p.head_chunks;
+    const int heads = min(8, group - 8 * chunk), h0 = head * group + 8 * chunk;
+    const int64_t n = visible(a.positions, b, 0, a.max_len);
     const int C = p.splits;
-    if (threadIdx.x < 8) {
-        float top = kRefStart, sum = 0.0f;
-        for (int r = 0; r < C; ++r) top = fmaxf(top, *cluster.map_shared_rank(&cta_m[threadIdx.x], r));
-        for (int r = 0; r < C; ++r)
-            sum += *cluster.map_shared_rank(&cta_l[threadIdx.x], r) *
-                   exp2_approx(*cluster.map_shared_rank(&cta_m[threadIdx.x], r) - top);
-        st_m[0][threadIdx.x] = top;
-        st_l[0][threadIdx.x] = sum;
-        lse2[threadIdx.x] = top + log2f(sum);
+    constexpr int kPitch = D + 4;
+    float *part = reinterpret_cast<float *>(smem);
+    if (C > 1) {
+        cluster.sync();
+        if (threadIdx.x < 8) {
+            float top = kRefStart, sum = 0.0f;
+            for (int r = 0; r < C; ++r) top = fmaxf(top, *cluster.map_shared_rank(&cta_m[threadIdx.x], r));
+            for (int r = 0; r < C; ++r) {
+                const float f = exp2_approx(*cluster.map_shared_rank(&cta_m[threadIdx.x], r) - top);
+                sum += *cluster.map_shared_rank(&cta_l[threadIdx.x], r) * f;
+                metas[r >> 2][8 * (r & 3) + threadIdx.x].x = f;  // factors [rank][head]
+            }
+            st_m[0][threadIdx.x] = sum;
+            lse2[threadIdx.x] = top + log2f(sum);
+        }
+        __syncthreads();
+        for (int i = blockIdx.x * kDThreads + threadIdx.x; i < heads * D; i += C * kDThreads) {
+            const int h = i / D, d = i % D;
+            float sum = 0.0f;
+            for (int r = 0; r < C; ++r)
+                sum = fmaf(*cluster.map_shared_rank(part + h * kPitch + d, r), metas[r >> 2][8 * (r & 3) + h].x, sum);
+            a.out[b * a.o_sb + (h0 + h) * a.o_sh + d] = __float2half(n > 0 ? sum / st_m[0][h] : 0.0f);
+        }
+        if (a.lse && blockIdx.x == 0 && threadIdx.x < heads)
+            a.lse[static_cast<int64_t>(b) * a.NH + h0 + threadIdx.x] =
+                n > 0 ? lse2[threadIdx.x] * 0.6931471805599453f : -INFINITY;
     }
-    __syncthreads();
-    for (int i = split * kDThreads + threadIdx.x; i < heads * D; i += C * kDThreads) {
-        const int h = i / D, d = i % D;
-        float sum = 0.0f;
-        for (int r = 0; r < C; ++r)
-            sum = fmaf(*cluster.map_shared_rank(part + h * kPitch + d, r),
-                       exp2_approx(*cluster.map_shared_rank(&cta_m[h], r) - st_m[0][h]), sum);
-        a.out[b * a.o_sb + (h0 + h) * a.o_sh + d] = __float2half(n > 0 ? sum / st_l[0][h] : 0.0f);
-    }
-    if (a.lse && split == 0 && threadIdx.x < heads)
-        a.lse[static_cast<int64_t>(b) * a.NH + h0 + threadIdx.x] = n > 0 ? lse2[threadIdx.x] * 0.6931471805599453f : -INFINITY;
-    if (p.w_out) {
-        for (int64_t key = k0 + threadIdx.x; key < k1; key += kDThreads) {
+    if (p.w_out) {  // one chunk of heads: this CTA's own scores
+        const float *xs = p.scores + ((static_cast<int64_t>(b) * a.pg.n_kv + head) * p.s_len) * group;
+        const int64_t end = min(static_cast<int64_t>(t0 + left) * kDTile, n);
+        for (int64_t key = static_cast<int64_t>(t0) * kDTile + threadIdx.x; key < end; key += kDThreads) {
             const int64_t at = b * p.w_sb + head * p.w_sh + key;
             const float sum = key_weight(xs + key * group, lse2, group);
             p.w_out[at] = sum + (p.w_in && key < n - 1 ? p.w_in[at] : 0.0f);
         }
     }
-    cluster.sync();  // no CTA leaves while another may read its shared memory
+    if (C > 1) cluster.sync();  // no CTA leaves while another may read its shared memory
 }
 
-// Joins the splits of a (sequence, KV head).  Blocks 0 .. group - 1: one head's output, the splits dealt to the
-// block's quarters; the others: the weights of 1024 keys each.
+// Joins the runs.  Blocks 0 .. group - 1 of a (sequence, KV head): one head's output, the parts dealt to the block's
+// quarters; the others: the weights of 4096 keys each.
 constexpr int kJoinThreads = 512;
+constexpr int kJoinKeys = 4096;
 
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads) attn8_join_kernel(DecodeArgs p) {
-    extern __shared__ float sm[];  // [heads][splits] factors
-    __shared__ float ref[128], sum[128], quarter[kJoinThreads];
+__global__ void __launch_bounds__(kJoinThreads) attn8_join_kernel(const __grid_constant__ DecodeArgs p) {
+    extern __shared__ float factor[];  // [parts] of the block's head
+    __shared__ float ref[128], sum, quarter[kJoinThreads];
+    constexpr int kPart = DecodeShape<D>::kPart;
     const AttnArgs &a = p.a;
     const int head = blockIdx.y, b = blockIdx.z, group = a.NH / a.pg.n_kv;
     const bool is_out = static_cast<int>(blockIdx.x) < group;
+    const int lane = threadIdx.x & 31;
     pdl_wait();
     pdl_trigger();
-    const int64_t n = visible(a.positions, b, 0, a.max_len);
-    const int64_t w0 = (static_cast<int64_t>(blockIdx.x) - group) * 1024;
+    const int64_t n = min(static_cast<int64_t>(a.positions[b]) + 1, a.max_len);
+    const int64_t w0 = (static_cast<int64_t>(blockIdx.x) - group) * kJoinKeys;
     if (!is_out && w0 >= n) return;
-    constexpr int64_t kPart = 8 * (D + 2);
-    const float *base = p.parts + (static_cast<int64_t>(b) * a.pg.n_kv + head) * p.head_chunks * p.splits * kPart;
-    const int lane = threadIdx.x & 31;
+    const int2 *ctas = p.unit_ctas + (static_cast<int64_t>(b) * a.pg.n_kv + head) * p.head_chunks;
+    // part i of a unit whose tiles begin in CTA c0: that CTA's last one, then the others' first
+    const auto part_of = [&](int c0, int i) { return p.parts + (2 * static_cast<int64_t>(c0 + i) + (i == 0 ? 1 : 0)) * kPart; };
     const int first = is_out ? blockIdx.x : 0, last = is_out ? first + 1 : group;
+    const int2 own = ctas[first >> 3];
+    if (is_out && own.x == own.y) return;  // its CTA wrote it
     for (int h = first + (threadIdx.x >> 5); h < last; h += kJoinThreads / 32) {
-        const float *st = base + static_cast<int64_t>(h >> 3) * p.splits * kPart + 8 * D + (h & 7);
+        const int2 c = ctas[h >> 3];
+        const int parts = c.y - c.x + 1;
+        if (parts == 1) {
+            if (lane == 0) ref[h] = p.unit_lse[static_cast<int64_t>(b) * a.NH + head * group + h];
+            continue;
+        }
         float top = kRefStart, s = 0.0f;
-        for (int i = lane; i < p.splits; i += 32) top = fmaxf(top, st[i * kPart]);
+        for (int i = lane; i < parts; i += 32) top = fmaxf(top, part_of(c.x, i)[8 * D + (h & 7)]);
         top = warp_max(top);
-        for (int i = lane; i < p.splits; i += 32) {
-            const float f = exp2_approx(st[i * kPart] - top);
-            sm[(h - first) * p.splits + i] = f;
-            s = fmaf(st[i * kPart + 8], f, s);
+        for (int i = lane; i < parts; i += 32) {
+            const float f = exp2_approx(part_of(c.x, i)[8 * D + (h & 7)] - top);
+            if (is_out) factor[i] = f;
+            s = fmaf(part_of(c.x, i)[8 * D + 8 + (h & 7)], f, s);
         }
         s = warp_sum(s);
-        if (lane == 0) ref[h - first] = top + log2f(s), sum[h - first] = s;
+        if (lane == 0) {
+            ref[h] = top + log2f(s);
+            if (is_out) sum = s;
+        }
     }
     __syncthreads();
     if (!is_out) {
         const float *xs = p.scores + ((static_cast<int64_t>(b) * a.pg.n_kv + head) * p.s_len) * group;
-        for (int64_t key = w0 + threadIdx.x; key < w0 + 1024 && key < n; key += kJoinThreads) {
+        const int64_t end = w0 + kJoinKeys < n ? w0 + kJoinKeys : n;
+#pragma unroll 4
+        for (int64_t key = w0 + threadIdx.x; key < end; key += kJoinThreads) {
             const int64_t at = b * p.w_sb + head * p.w_sh + key;
             const float w = key_weight(xs + key * group, ref, group);
             p.w_out[at] = w + (p.w_in && key < n - 1 ? p.w_in[at] : 0.0f);
@@ -552,18 +668,16 @@ __global__ void __launch_bounds__(kJoinThreads) attn8_join_kernel(DecodeArgs p) 
         return;
     }
     constexpr int kShare = kJoinThreads / D;
-    const int d = threadIdx.x % D, q = threadIdx.x / D, h = first;
-    const float *src = base + static_cast<int64_t>(h >> 3) * p.splits * kPart + (h & 7) * D + d;
+    const int d = threadIdx.x % D, q = threadIdx.x / D, count = own.y - own.x + 1;
     float acc = 0.0f;
 #pragma unroll 8
-    for (int s = q; s < p.splits; s += kShare) acc = fmaf(src[s * kPart], sm[s], acc);
+    for (int i = q; i < count; i += kShare) acc = fmaf(part_of(own.x, i)[(first & 7) * D + d], factor[i], acc);
     quarter[threadIdx.x] = acc;
     __syncthreads();
     if (threadIdx.x < D) {
         for (int i = 1; i < kShare; ++i) acc += quarter[i * D + d];
-        a.out[b * a.o_sb + (head * group + h) * a.o_sh + d] = __float2half(n > 0 ? acc / sum[0] : 0.0f);
-        if (a.lse && d == 0)
-            a.lse[static_cast<int64_t>(b) * a.NH + head * group + h] = n > 0 ? ref[0] * 0.6931471805599453f : -INFINITY;
+        a.out[b * a.o_sb + (head * group + first) * a.o_sh + d] = __float2half(acc / sum);
+        if (a.lse && d == 0) a.lse[static_cast<int64_t>(b) * a.NH + head * group + first] = ref[first] * 0.6931471805599453f;
     }
 }
 
@@ -598,34 +712,29 @@ bool strides_ok(const void *p, int64_t a, int64_t b, int64_t c) {
 }
 
 struct DecodePlan {
-    int splits, head_chunks;
-    bool join;
-    int64_t part_floats, floats;
+    int splits, head_chunks, ctas;
+    int64_t part_floats, unit_floats, lse_floats, floats;
 };
 
-// CTAs per sequence and head: four per SM in all, but at least 64 keys each and at most 2048.  Up to 8 join within
-// their cluster; more (and groups of more than 8 heads whose weights are wanted, which no one CTA holds) in a
-// second kernel.
+// A cluster of one 64-key tile per CTA where the longest sequence has at most 8 tiles and one wave of CTAs holds
+// them all (a group of more than 8 heads whose weights are wanted is in no one CTA's hands, so it takes the runs);
+// else runs of tiles, four CTAs per SM.
 DecodePlan decode_plan(int64_t B, int64_t NH, int64_t NK, int64_t D, int64_t max_len, int64_t splits, bool weights) {
     DecodePlan r = {};
     const int64_t group = NH / NK;
     r.head_chunks = static_cast<int>((group + 7) / 8);
-    const int64_t units = B * NK * r.head_chunks;
-    int64_t s = splits;
-    if (s == 0) {
-        s = 4 * sm_count() / units;
-        const int64_t most = (max_len + 63) / 64, least = (max_len + 2047) / 2048;
-        s = s < least ? least : s;
-        s = s > most ? most : s;
+    const int64_t units = B * NK * r.head_chunks, tiles = (max_len + kDTile - 1) / kDTile, wave = 4 * sm_count();
+    if (splits == 0 && tiles <= 8 && units * tiles <= wave && !(weights && r.head_chunks > 1)) {
+        r.splits = static_cast<int>(tiles);
+    } else {
+        const int64_t most = units * tiles;
+        int64_t ctas = splits > 0 ? (splits < most / units ? splits * units : most) : (wave < most ? wave : most);
+        r.ctas = static_cast<int>(ctas < 8192 ? ctas : 8192);
+        r.part_floats = 2 * r.ctas * 8 * (D + 2);  // a multiple of 4: what lies behind stays aligned
+        r.unit_floats = (2 * units + 3) / 4 * 4;
+        r.lse_floats = weights ? (B * NH + 3) / 4 * 4 : 0;
     }
-    const int64_t bound = 10240 / group;  // the joining kernel's shared memory
-    s = s > 128 ? 128 : s;
-    s = s > bound ? bound : s;
-    s = s < 1 ? 1 : s;
-    r.splits = static_cast<int>(s);
-    r.join = s > 8 || (weights && r.head_chunks > 1);
-    r.part_floats = r.join ? units * s * 8 * (D + 2) : 0;  // a multiple of 4: the scores behind stay aligned
-    r.floats = r.part_floats + (weights ? B * NK * max_len * group : 0);
+    r.floats = r.part_floats + r.unit_floats + r.lse_floats + (weights ? B * NK * max_len * group : 0);
     return r;
 }
 
@@ -676,31 +785,40 @@ extern "C" int t2c_attn_decode_q8(const t2c_q8_pages *pages, const void *q, int6
     if (plan.floats > 0 && (!workspace || workspace_floats < plan.floats))
         return set_error(T2C_ESCRATCH, "attn_decode_q8: workspace needs %lld floats", (long long)plan.floats);
     if (!kv8_aligned(workspace, 16)) return set_error(T2C_EINVAL, "attn_decode_q8: workspace must be 16-byte aligned");
-    if (a.pg.n_kv * plan.head_chunks > 65535) return set_error(T2C_EINVAL, "attn_decode_q8: bad shape");
+    if (a.pg.n_kv * plan.head_chunks > 65535 || B * a.pg.n_kv * plan.head_chunks * ((max_len + kDTile - 1) / kDTile) > INT32_MAX)
+        return set_error(T2C_EINVAL, "attn_decode_q8: bad shape");
     a.q = static_cast<const __half *>(q), a.q_sb = q_sb, a.q_sh = q_sh;
     a.out = static_cast<__half *>(out), a.o_sb = o_sb, a.o_sh = o_sh;
     a.lse = lse;
     a.positions = positions, a.table = block_table, a.t_stride = bt_stride, a.max_len = max_len;
     a.B = static_cast<int>(B), a.T = 1, a.NH = static_cast<int>(NH);
     a.scale_log2 = scale * 1.4426950408889634f;
-    p.splits = plan.splits, p.head_chunks = plan.head_chunks, p.join = plan.join;
+    p.splits = plan.splits, p.head_chunks = plan.head_chunks, p.ctas = plan.ctas;
     p.parts = workspace;
-    p.scores = workspace + plan.part_floats;
+    p.unit_ctas = reinterpret_cast<int2 *>(workspace + plan.part_floats);
+    p.unit_lse = workspace + plan.part_floats + plan.unit_floats;
+    p.scores = workspace + plan.part_floats + plan.unit_floats + plan.lse_floats;
     p.s_len = max_len;
     p.w_in = weights, p.w_out = weights_out, p.w_sb = w_sb, p.w_sh = w_sh;
+    CUtensorMap k_map, v_map;
+    if (!kv8_maps(pages, 16, k_map, v_map))
+        return set_error(T2C_ECUDA, "attn_decode_q8: cuTensorMapEncodeTiled failed");
     const cudaStream_t s = as_stream(stream);
     const auto kern = D == 128 ? attn8_decode_kernel<128> : attn8_decode_kernel<64>;
     const int smem = D == 128 ? DecodeShape<128>::kRing : DecodeShape<64>::kRing;
     rc = configure(kern, smem, D == 128 ? 0 : 1, "attn_decode_q8");
     if (rc != T2C_OK) return rc;
-    rc = kv8_launch("attn_decode_q8", kern,
-                    dim3(static_cast<unsigned>(p.splits), static_cast<unsigned>(a.pg.n_kv * p.head_chunks), static_cast<unsigned>(B)),
-                    dim3(kDThreads), smem, p.join ? 1u : static_cast<unsigned>(p.splits), s, p);
-    if (rc != T2C_OK || !p.join) return rc;
-    const int64_t chunks = weights_out ? (max_len + 1023) / 1024 : 0;
+    const bool clusters = p.splits > 0;
+    const dim3 grid = clusters ? dim3(static_cast<unsigned>(p.splits), static_cast<unsigned>(a.pg.n_kv * p.head_chunks),
+                                      static_cast<unsigned>(B))
+                               : dim3(static_cast<unsigned>(p.ctas));
+    rc = kv8_launch("attn_decode_q8", kern, grid, dim3(kDThreads), smem, clusters ? static_cast<unsigned>(p.splits) : 1u, s, k_map,
+                    v_map, p);
+    if (rc != T2C_OK || clusters) return rc;
+    const int64_t chunks = weights_out ? (max_len + kJoinKeys - 1) / kJoinKeys : 0;
     return kv8_launch("attn_decode_q8 join", D == 128 ? attn8_join_kernel<128> : attn8_join_kernel<64>,
                       dim3(static_cast<unsigned>(group + chunks), static_cast<unsigned>(a.pg.n_kv), static_cast<unsigned>(B)),
-                      dim3(kJoinThreads), static_cast<size_t>((weights_out ? group : 1) * p.splits * 4), 1, s, p);
+                      dim3(kJoinThreads), static_cast<size_t>(p.ctas * 4), 1, s, p);
 }
 
 extern "C" int64_t t2c_attn_prefill_q8_workspace(const t2c_q8_pages *pages, int64_t bt_width, int64_t B, int64_t T,

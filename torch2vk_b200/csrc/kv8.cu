@@ -51,6 +51,33 @@ int kv8_table(const t2c_q8_pages *p, const int32_t *table, int64_t stride, int64
     return T2C_OK;
 }
 
+bool kv8_maps(const t2c_q8_pages *p, int rows, CUtensorMap &k_map, CUtensorMap &v_map) {
+    static PFN_cuTensorMapEncodeTiled encode = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled>(fn);
+    }();
+    if (!encode) return false;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p->head_dim), static_cast<cuuint64_t>(p->page_size),
+                                static_cast<cuuint64_t>(p->n_kv), static_cast<cuuint64_t>(p->num_pages)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(p->row_stride), static_cast<cuuint64_t>(p->head_stride),
+                                   static_cast<cuuint64_t>(p->page_stride)};
+    const cuuint32_t box[4] = {static_cast<cuuint32_t>(p->head_dim), static_cast<cuuint32_t>(rows), 1, 1};
+    const cuuint32_t es[4] = {1, 1, 1, 1};
+    const CUtensorMapSwizzle swizzle = p->head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+    CUtensorMap *maps[2] = {&k_map, &v_map};
+    void *bases[2] = {p->k, p->v};
+    for (int i = 0; i < 2; ++i)
+        if (encode(maps[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, bases[i], dims, strides, box, es,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return false;
+    return true;
+}
+
 namespace {
 
 // ------------------------------------------------------------------ write

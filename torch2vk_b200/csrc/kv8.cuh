@@ -7,6 +7,7 @@
 // that was given a non-finite value: all of it reads as NaN.
 #pragma once
 
+#include <cudaTypedefs.h>
 #include <math.h>
 
 #include "common.cuh"
@@ -26,6 +27,19 @@ int kv8_view(const t2c_q8_pages *pages, const char *what, KvPages &out);
 // Checks a block table against the pool: returns T2C_OK and the capacity in positions.
 int kv8_table(const t2c_q8_pages *pages, const int32_t *table, int64_t stride, int64_t width, const char *what,
               int64_t &capacity);
+
+// Tensor maps of the codes as (dim, row of page, KV head, page), boxes of `rows` rows of one head in the swizzle that
+// is as wide as a row (128 or 64 bytes).  False when the driver refuses.
+bool kv8_maps(const t2c_q8_pages *pages, int rows, CUtensorMap &k_map, CUtensorMap &v_map);
+
+// A box of the codes at (row, head, page) into shared memory (no multicast).
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
+            "r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
 
 // Physical page of a position; an entry outside the pool is reported and becomes -1.
 __device__ __forceinline__ int kv8_page(const KvPages &pg, const int32_t *__restrict__ table, int64_t pos) {
