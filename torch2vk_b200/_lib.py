@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -120,14 +121,8 @@ _SIGNATURES: dict[str, list] = {
                                                                                           _vp, _vp],
 }
 
-
-class Q8PagesStruct(_c.Structure):
-    """t2c_q8_pages of include/t2c_sm100.h."""
-
-    _fields_ = [(n, _vp) for n in ("k", "v", "k_scale", "v_scale")] + [(n, _i64) for n in (
-        "page_stride", "head_stride", "row_stride", "scale_page_stride", "scale_head_stride", "num_pages", "n_kv",
-        "page_size", "head_dim", "block")]
-
+# t2c_q8_pages of include/t2c_sm100.h: four pointers, ten int64
+Q8_PAGES = struct.Struct("@4P10q")
 
 _RESTYPES = {"t2c_last_error": _c.c_char_p, "t2c_attn_decode_fused_workspace": _c.c_int64,
              "t2c_allreduce_buffer_bytes": _c.c_int64, "t2c_linear_f32_scratch_bytes": _c.c_int64,
@@ -190,8 +185,9 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def stream_ptr(stream: torch.cuda.Stream | None = None) -> int:
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    if stream is None:  # the raw handle, without building a Stream object
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return stream.cuda_stream
 
 
 def ptr_array(values) -> ctypes.Array:

@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(32) attn8_weights_kernel(AttnArgs a, const flo
 // running reference per head, moved (and O, l rescaled) only when some exponent passes 14: P stays in fp16's range,
 // and its one rounding to fp16, which the tensor core asks for, is the only one before the output's.
 constexpr int kDWarps = 4;
-constexpr int kDStages = 3;
+constexpr int kDStages = 2;
 constexpr int kDThreads = 32 * kDWarps;
 constexpr int kDTile = 16 * kDWarps;
 constexpr float kRefStart = -1e30f;  // below any finite score: the first step moves it
@@ -610,7 +610,8 @@ __global__ void __launch_bounds__(kDThreads, 4) attn8_decode_kernel(const __grid
 }
 
 // Joins the runs.  Blocks 0 .. group - 1 of a (sequence, KV head): one head's output, the parts dealt to the block's
-// quarters; the others: the weights of 4096 keys each.
+// quarters; the others: the weights of 4096 keys each.  What does not depend on the softmax statistics is loaded
+// beside them: a block is three dependent trips to memory long.
 constexpr int kJoinThreads = 512;
 constexpr int kJoinKeys = 4096;
 
@@ -622,32 +623,46 @@ __global__ void __launch_bounds__(kJoinThreads) attn8_join_kernel(const __grid_c
     const AttnArgs &a = p.a;
     const int head = blockIdx.y, b = blockIdx.z, group = a.NH / a.pg.n_kv;
     const bool is_out = static_cast<int>(blockIdx.x) < group;
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_wait();
     pdl_trigger();
-    const int64_t n = min(static_cast<int64_t>(a.positions[b]) + 1, a.max_len);
-    const int64_t w0 = (static_cast<int64_t>(blockIdx.x) - group) * kJoinKeys;
-    if (!is_out && w0 >= n) return;
     const int2 *ctas = p.unit_ctas + (static_cast<int64_t>(b) * a.pg.n_kv + head) * p.head_chunks;
-    // part i of a unit whose tiles begin in CTA c0: that CTA's last one, then the others' first
-    const auto part_of = [&](int c0, int i) { return p.parts + (2 * static_cast<int64_t>(c0 + i) + (i == 0 ? 1 : 0)) * kPart; };
     const int first = is_out ? blockIdx.x : 0, last = is_out ? first + 1 : group;
     const int2 own = ctas[first >> 3];
-    if (is_out && own.x == own.y) return;  // its CTA wrote it
-    for (int h = first + (threadIdx.x >> 5); h < last; h += kJoinThreads / 32) {
+    const int64_t n = min(static_cast<int64_t>(a.positions[b]) + 1, a.max_len);
+    const int64_t w0 = (static_cast<int64_t>(blockIdx.x) - group) * kJoinKeys;
+    if (is_out ? own.x == own.y : w0 >= n) return;  // a unit of one CTA is written
+    // part i of a unit whose tiles begin in CTA c0: that CTA's last one, then the others' first
+    const auto part_of = [&](int c0, int i) { return p.parts + (2 * static_cast<int64_t>(c0 + i) + (i == 0 ? 1 : 0)) * kPart; };
+
+    constexpr int kShare = kJoinThreads / D, kAhead = 4;
+    const int d = threadIdx.x % D, q = threadIdx.x / D, count = own.y - own.x + 1;
+    float ahead[kAhead];
+    if (is_out) {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+            ahead[k] = q + kShare * k < count ? part_of(own.x, q + kShare * k)[(first & 7) * D + d] : 0.0f;
+    }
+    for (int h = first + warp; h < last; h += kJoinThreads / 32) {
         const int2 c = ctas[h >> 3];
         const int parts = c.y - c.x + 1;
         if (parts == 1) {
             if (lane == 0) ref[h] = p.unit_lse[static_cast<int64_t>(b) * a.NH + head * group + h];
             continue;
         }
-        float top = kRefStart, s = 0.0f;
-        for (int i = lane; i < parts; i += 32) top = fmaxf(top, part_of(c.x, i)[8 * D + (h & 7)]);
+        float top = kRefStart, s = 0.0f, m0 = kRefStart, l0 = 0.0f;
+        if (lane < parts) {
+            const float *st = part_of(c.x, lane) + 8 * D + (h & 7);
+            top = m0 = st[0];
+            l0 = st[8];
+        }
+        for (int i = lane + 32; i < parts; i += 32) top = fmaxf(top, part_of(c.x, i)[8 * D + (h & 7)]);
         top = warp_max(top);
         for (int i = lane; i < parts; i += 32) {
-            const float f = exp2_approx(part_of(c.x, i)[8 * D + (h & 7)] - top);
+            const float *st = part_of(c.x, i) + 8 * D + (h & 7);
+            const float f = exp2_approx((i == lane ? m0 : st[0]) - top);
             if (is_out) factor[i] = f;
-            s = fmaf(part_of(c.x, i)[8 * D + 8 + (h & 7)], f, s);
+            s = fmaf(i == lane ? l0 : st[8], f, s);
         }
         s = warp_sum(s);
         if (lane == 0) {
@@ -655,23 +670,45 @@ __global__ void __launch_bounds__(kJoinThreads) attn8_join_kernel(const __grid_c
             if (is_out) sum = s;
         }
     }
-    __syncthreads();
     if (!is_out) {
-        const float *xs = p.scores + ((static_cast<int64_t>(b) * a.pg.n_kv + head) * p.s_len) * group;
-        const int64_t end = w0 + kJoinKeys < n ? w0 + kJoinKeys : n;
-#pragma unroll 4
-        for (int64_t key = w0 + threadIdx.x; key < end; key += kJoinThreads) {
-            const int64_t at = b * p.w_sb + head * p.w_sh + key;
-            const float w = key_weight(xs + key * group, ref, group);
-            p.w_out[at] = w + (p.w_in && key < n - 1 ? p.w_in[at] : 0.0f);
+        const float *xs = p.scores + ((static_cast<int64_t>(b) * a.pg.n_kv + head) * p.s_len + w0) * group;
+        const int64_t at = b * p.w_sb + head * p.w_sh + w0;
+        const int end = static_cast<int>(n - w0 < kJoinKeys ? n - w0 : kJoinKeys), old = static_cast<int>(n - 1 - w0);
+        if (group == 4) {  // scores of eight keys a thread, all in flight before the statistics are known
+            constexpr int kKeys = kJoinKeys / kJoinThreads;
+            float4 x[kKeys];
+            float w[kKeys];
+#pragma unroll
+            for (int k = 0; k < kKeys; ++k) {
+                const int key = threadIdx.x + kJoinThreads * k;
+                if (key < end) x[k] = *reinterpret_cast<const float4 *>(xs + 4 * key);
+                w[k] = p.w_in && key < end && key < old ? p.w_in[at + key] : 0.0f;
+            }
+            __syncthreads();
+            const float4 r = make_float4(ref[0], ref[1], ref[2], ref[3]);
+#pragma unroll
+            for (int k = 0; k < kKeys; ++k) {
+                const int key = threadIdx.x + kJoinThreads * k;
+                if (key < end)
+                    p.w_out[at + key] = w[k] + exp2_approx(x[k].x - r.x) + exp2_approx(x[k].y - r.y) +
+                                        exp2_approx(x[k].z - r.z) + exp2_approx(x[k].w - r.w);
+            }
+            return;
+        }
+        __syncthreads();
+        for (int key = threadIdx.x; key < end; key += kJoinThreads) {
+            const float w = key_weight(xs + static_cast<int64_t>(key) * group, ref, group);
+            p.w_out[at + key] = w + (p.w_in && key < old ? p.w_in[at + key] : 0.0f);
         }
         return;
     }
-    constexpr int kShare = kJoinThreads / D;
-    const int d = threadIdx.x % D, q = threadIdx.x / D, count = own.y - own.x + 1;
+    __syncthreads();
     float acc = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+        if (q + kShare * k < count) acc = fmaf(ahead[k], factor[q + kShare * k], acc);
 #pragma unroll 8
-    for (int i = q; i < count; i += kShare) acc = fmaf(part_of(own.x, i)[(first & 7) * D + d], factor[i], acc);
+    for (int i = q + kShare * kAhead; i < count; i += kShare) acc = fmaf(part_of(own.x, i)[(first & 7) * D + d], factor[i], acc);
     quarter[threadIdx.x] = acc;
     __syncthreads();
     if (threadIdx.x < D) {

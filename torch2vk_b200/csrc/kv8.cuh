@@ -60,8 +60,9 @@ __device__ __forceinline__ int64_t kv8_scale_offset(const KvPages &pg, int page,
 // Four codes (one 32-bit word) as two half2, exactly: the biased byte c + 128 placed in the low mantissa
 // bits of 1024 gives 1152 + c, and the subtraction is exact.  even = codes 0 and 2, odd = codes 1 and 3.
 __device__ __forceinline__ void kv8_unpack(uint32_t w, __half2 &even, __half2 &odd) {
-    const uint32_t lo = (w & 0x00ff00ffu) ^ 0x64806480u;
-    const uint32_t hi = ((w >> 8) & 0x00ff00ffu) ^ 0x64806480u;
+    uint32_t lo, hi;
+    asm("{\n .reg .b32 m, x;\n mov.b32 m, 0x00ff00ff;\n mov.b32 x, 0x64806480;\n lop3.b32 %0, %1, m, x, 0x6a;\n}\n" : "=r"(lo) : "r"(w));
+    asm("{\n .reg .b32 m, x;\n mov.b32 m, 0x00ff00ff;\n mov.b32 x, 0x64806480;\n lop3.b32 %0, %1, m, x, 0x6a;\n}\n" : "=r"(hi) : "r"(w >> 8));
     const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
     even = __hsub2(*reinterpret_cast<const __half2 *>(&lo), bias);
     odd = __hsub2(*reinterpret_cast<const __half2 *>(&hi), bias);

@@ -10,6 +10,7 @@ Weights are the GGUF packed tensors in the reference's physical dtypes
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -813,31 +814,33 @@ class Q8Pages:
     consecutive tokens of a KV head, k_scale / v_scale [num_pages, n_kv, page_size / block].  A code stands for
     code * scale."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "block", "struct", "ref")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "n_kv", "page_size", "head_dim", "block", "ref")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
         shape, strides = k.shape, k.stride()
-        if k.dtype != torch.int8 or v.dtype != torch.int8 or k.dim() != 4 or v.shape != shape or v.stride() != strides:
+        if k.dtype != torch.int8 or v.dtype != torch.int8 or len(shape) != 4 or v.shape != shape or v.stride() != strides:
             raise ValueError("k / v must be int8 [num_pages, n_kv, page_size, head_dim] of one layout")
         s_shape, s_strides = k_scale.shape, k_scale.stride()
-        if (k_scale.dtype != torch.float16 or v_scale.dtype != torch.float16 or k_scale.dim() != 3
+        if (k_scale.dtype != torch.float16 or v_scale.dtype != torch.float16 or len(s_shape) != 3
                 or v_scale.shape != s_shape or v_scale.stride() != s_strides or s_shape[:2] != shape[:2]
                 or s_shape[2] == 0 or shape[2] % s_shape[2]):
             raise ValueError("k_scale / v_scale must be float16 [num_pages, n_kv, page_size / block] of one layout")
         if strides[3] != 1 or (s_strides[2] != 1 and s_shape[2] > 1):
             raise ValueError("codes and scales must have unit last stride")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.block = shape[2] // s_shape[2]
-        self.struct = _lib.Q8PagesStruct(_lib.ptr(k), _lib.ptr(v), _lib.ptr(k_scale), _lib.ptr(v_scale), strides[0],
-                                         strides[1], strides[2], s_strides[0], s_strides[1], shape[0], shape[1], shape[2],
-                                         shape[3], self.block)
-        self.ref = ctypes.addressof(self.struct)
+        pages, self.n_kv, self.page_size, self.head_dim = shape
+        self.block = self.page_size // s_shape[2]
+        # the C description; its pointers stay valid as long as this object holds the tensors
+        self.ref = _lib.Q8_PAGES.pack(_lib.ptr(k), _lib.ptr(v), _lib.ptr(k_scale), _lib.ptr(v_scale), strides[0], strides[1],
+                                      strides[2], s_strides[0], s_strides[1], pages, self.n_kv, self.page_size,
+                                      self.head_dim, self.block)
 
 
 def _q8_table(table: torch.Tensor, batch: int) -> tuple[int, int, int]:
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] < batch or table.stride(1) != 1:
+    shape = table.shape
+    if table.dtype != torch.int32 or len(shape) != 2 or shape[0] < batch or table.stride(1) != 1:
         raise ValueError("block_table must be int32 [sequences, pages] with unit last stride")
-    return _lib.ptr(table), table.stride(0), table.shape[1]
+    return _lib.ptr(table), table.stride(0), shape[1]
 
 
 def _q8_index(t: torch.Tensor, batch: int, name: str) -> int:
@@ -848,7 +851,8 @@ def _q8_index(t: torch.Tensor, batch: int, name: str) -> int:
 
 def _q8_rows(x: torch.Tensor, name: str, heads: int | None, head_dim: int) -> tuple[int, ...]:
     """Pointer and (batch, token, head) strides of an fp16 [B, T, heads, head_dim] tensor."""
-    if x.dtype != torch.float16 or x.dim() != 4 or x.shape[3] != head_dim or (heads is not None and x.shape[2] != heads):
+    shape = x.shape
+    if x.dtype != torch.float16 or len(shape) != 4 or shape[3] != head_dim or (heads is not None and shape[2] != heads):
         raise ValueError(f"{name} must be float16 [batch, tokens, {heads or 'heads'}, {head_dim}]")
     sb, st, sh, sd = x.stride()
     if sd != 1:
@@ -862,11 +866,11 @@ def kv_cache_write_q8(pages: Q8Pages, k: torch.Tensor, v: torch.Tensor, position
 
     A block's scale only grows: earlier rows of a block are rescaled when a new row needs a larger scale.  Rows at
     negative positions are padding.  A block given a non-finite value reads as NaN."""
-    heads, dim = pages.k.shape[1], pages.k.shape[3]
-    if k.shape != v.shape:
+    shape = k.shape
+    if shape != v.shape:
         raise ValueError("k and v must have one shape")
-    kp, vp = _q8_rows(k, "k", heads, dim), _q8_rows(v, "v", heads, dim)
-    batch, tokens = k.shape[:2]
+    kp, vp = _q8_rows(k, "k", pages.n_kv, pages.head_dim), _q8_rows(v, "v", pages.n_kv, pages.head_dim)
+    batch, tokens = shape[0], shape[1]
     _lib.lib().call("t2c_kv_cache_write_q8", pages.ref, *kp, *vp, _q8_index(positions, batch, "positions"),
                     *_q8_table(block_table, batch), batch, tokens, _lib.stream_ptr())
 
@@ -876,23 +880,23 @@ def kv_cache_read_q8(pages: Q8Pages, first: torch.Tensor, lengths: torch.Tensor,
                      v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows first[b] .. first[b] + tokens - 1 as fp16 k, v [B, tokens, n_kv, head_dim]; zero from lengths[b] on."""
     batch = first.numel()
-    shape = (batch, tokens, pages.k.shape[1], pages.k.shape[3])
-    outs = []
+    shape = (batch, tokens, pages.n_kv, pages.head_dim)
+    if k_out is None:
+        k_out = pages.k_scale.new_empty(shape)
+    if v_out is None:
+        v_out = torch.empty_like(k_out)
     for t in (k_out, v_out):
-        if t is None:
-            t = torch.empty(shape, dtype=torch.float16, device=pages.k.device)
-        elif t.dtype != torch.float16 or t.shape != shape or not t.is_contiguous():
+        if t.dtype != torch.float16 or t.shape != shape or not t.is_contiguous():
             raise ValueError(f"k_out / v_out must be contiguous float16 {shape}")
-        outs.append(t)
-    _lib.lib().call("t2c_kv_cache_read_q8", pages.ref, _lib.ptr(outs[0]), _lib.ptr(outs[1]),
+    _lib.lib().call("t2c_kv_cache_read_q8", pages.ref, _lib.ptr(k_out), _lib.ptr(v_out),
                     _q8_index(first, batch, "first"), _q8_index(lengths, batch, "lengths"),
                     *_q8_table(block_table, batch), batch, tokens, _lib.stream_ptr())
-    return outs[0], outs[1]
+    return k_out, v_out
 
 
 def _q8_out(q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=torch.float16, device=q.device)
+        return torch.empty_like(q)
     if out.dtype != torch.float16 or out.shape != q.shape or out.stride(-1) != 1:
         raise ValueError("out must be float16 of q's shape with unit last stride")
     return out
@@ -909,16 +913,16 @@ def _q8_weights(weights: torch.Tensor | None, weights_out: torch.Tensor, batch: 
     return (None if weights is None else _lib.ptr(weights)), _lib.ptr(weights_out), *weights_out.stride()[:2]
 
 
-def _q8_lse(lse: torch.Tensor | None, want: bool, shape: tuple[int, ...], device: torch.device) -> torch.Tensor | None:
+def _q8_lse(lse: torch.Tensor | None, want: bool, shape: tuple[int, ...], like: torch.Tensor) -> torch.Tensor | None:
     if lse is None:
-        return torch.empty(shape, dtype=torch.float32, device=device) if want else None
+        return like.new_empty(shape, dtype=torch.float32) if want else None
     if lse.dtype != torch.float32 or lse.shape != shape or not lse.is_contiguous():
         raise ValueError(f"lse must be contiguous float32 {shape}")
     return lse
 
 
 def _q8_max_len(max_len: int | None, table: torch.Tensor, pages: Q8Pages) -> int:
-    capacity = table.shape[1] * pages.k.shape[2]
+    capacity = table.shape[1] * pages.page_size
     if max_len is None:
         return capacity
     if not 0 < max_len <= capacity:
@@ -926,12 +930,21 @@ def _q8_max_len(max_len: int | None, table: torch.Tensor, pages: Q8Pages) -> int
     return max_len
 
 
-def _q8_workspace(workspace: torch.Tensor | None, need: int, device: torch.device) -> tuple[torch.Tensor | None, int]:
+@functools.lru_cache(maxsize=1024)
+def _q8_workspace_floats(name: str, n_kv: int, head_dim: int, page_size: int, *args: int) -> int:
+    """The library's answer for a pool of this shape (it depends on nothing else)."""
+    ref = _lib.Q8_PAGES.pack(0, 0, 0, 0, 0, 0, 0, 0, 0, 1, n_kv, page_size, head_dim, 16)
+    return int(_lib.lib().raw(name)(ref, *args))
+
+
+def _q8_workspace(workspace: torch.Tensor | None, like: torch.Tensor, pages: Q8Pages, name: str,
+                  *args: int) -> tuple[torch.Tensor | None, int]:
     if workspace is None:
+        need = _q8_workspace_floats(name, pages.n_kv, pages.head_dim, pages.page_size, *args)
         if need <= 0:
             return None, 0
-        workspace = torch.empty(need, dtype=torch.float32, device=device)
-    elif workspace.dtype != torch.float32 or not workspace.is_contiguous():
+        return like.new_empty(need, dtype=torch.float32), need
+    if workspace.dtype != torch.float32 or not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous float32")
     return workspace, workspace.numel()
 
@@ -939,9 +952,9 @@ def _q8_workspace(workspace: torch.Tensor | None, need: int, device: torch.devic
 def attn_decode_q8_workspace(pages: Q8Pages, block_table: torch.Tensor, *, batch: int, n_heads: int,
                              max_len: int | None = None, splits: int = 0, with_weights: bool = False) -> int:
     """Floats of workspace that attn_decode_q8 needs with these arguments."""
-    return int(_lib.lib().raw("t2c_attn_decode_q8_workspace")(
-        pages.ref, block_table.shape[1], batch, n_heads, _q8_max_len(max_len, block_table, pages), splits,
-        1 if with_weights else 0))
+    return _q8_workspace_floats("t2c_attn_decode_q8_workspace", pages.n_kv, pages.head_dim, pages.page_size,
+                                block_table.shape[1], batch, n_heads, _q8_max_len(max_len, block_table, pages), splits,
+                                1 if with_weights else 0)
 
 
 def attn_decode_q8(q: torch.Tensor, pages: Q8Pages, positions: torch.Tensor, block_table: torch.Tensor, *,
@@ -954,27 +967,25 @@ def attn_decode_q8(q: torch.Tensor, pages: Q8Pages, positions: torch.Tensor, blo
     max_len: a bound on positions[b] + 1 (default: the block table's capacity).  weights_out [B, n_kv, positions]
     fp32 gets weights plus each key's probability summed over the heads of its group (the key at positions[b]
     starts from zero; without weights every key does); pass one tensor as both to accumulate.  lse [B, heads] fp32."""
-    heads, dim = pages.k.shape[1], pages.k.shape[3]
-    if q.dtype != torch.float16 or q.dim() != 3 or q.shape[2] != dim or q.stride(2) != 1:
+    heads, dim, shape, strides = pages.n_kv, pages.head_dim, q.shape, q.stride()
+    if q.dtype != torch.float16 or len(shape) != 3 or shape[2] != dim or strides[2] != 1:
         raise ValueError(f"q must be float16 [batch, heads, {dim}] with unit last stride")
-    batch, n_heads = q.shape[:2]
+    batch, n_heads = shape[0], shape[1]
     out = _q8_out(q, out)
+    o_strides = out.stride()
     max_len = _q8_max_len(max_len, block_table, pages)
     wargs: tuple = (None, None, 0, 0)
     if weights_out is not None:
         wargs = _q8_weights(weights, weights_out, batch, heads, max_len)
     elif weights is not None:
         raise ValueError("weights without weights_out")
-    lse = _q8_lse(lse, False, (batch, n_heads), q.device)
-    if workspace is None:
-        need = int(_lib.lib().raw("t2c_attn_decode_q8_workspace")(pages.ref, block_table.shape[1], batch, n_heads, max_len,
-                                                                  splits, 1 if weights_out is not None else 0))
-    else:
-        need = 0
-    workspace, floats = _q8_workspace(workspace, need, q.device)
-    _lib.lib().call("t2c_attn_decode_q8", pages.ref, _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(out), out.stride(0),
-                    out.stride(1), _lib.ptr(lse), _q8_index(positions, batch, "positions"),
-                    *_q8_table(block_table, batch), batch, n_heads, dim ** -0.5 if scale is None else float(scale),
+    if lse is not None:
+        _q8_lse(lse, False, (batch, n_heads), q)
+    workspace, floats = _q8_workspace(workspace, q, pages, "t2c_attn_decode_q8_workspace", block_table.shape[1], batch,
+                                      n_heads, max_len, splits, 0 if weights_out is None else 1)
+    _lib.lib().call("t2c_attn_decode_q8", pages.ref, _lib.ptr(q), strides[0], strides[1], _lib.ptr(out), o_strides[0],
+                    o_strides[1], _lib.ptr(lse), _q8_index(positions, batch, "positions"),
+                    *_q8_table(block_table, batch), batch, n_heads, dim ** -0.5 if scale is None else scale,
                     max_len, splits, *wargs, _lib.ptr(workspace), floats, _lib.stream_ptr())
     return out
 
@@ -982,8 +993,8 @@ def attn_decode_q8(q: torch.Tensor, pages: Q8Pages, positions: torch.Tensor, blo
 def attn_prefill_q8_workspace(pages: Q8Pages, block_table: torch.Tensor, *, batch: int, tokens: int, n_heads: int,
                               max_len: int | None = None, splits: int = 0) -> int:
     """Floats of workspace that attn_prefill_q8 needs with these arguments."""
-    return int(_lib.lib().raw("t2c_attn_prefill_q8_workspace")(
-        pages.ref, block_table.shape[1], batch, tokens, n_heads, _q8_max_len(max_len, block_table, pages), splits))
+    return _q8_workspace_floats("t2c_attn_prefill_q8_workspace", pages.n_kv, pages.head_dim, pages.page_size,
+                                block_table.shape[1], batch, tokens, n_heads, _q8_max_len(max_len, block_table, pages), splits)
 
 
 def attn_prefill_q8(q: torch.Tensor, pages: Q8Pages, positions: torch.Tensor, block_table: torch.Tensor, *,
@@ -993,21 +1004,18 @@ def attn_prefill_q8(q: torch.Tensor, pages: Q8Pages, positions: torch.Tensor, bl
     """Causal attention of q [B, T, heads, head_dim] (already cached tokens): query t of sequence b sees positions
     0..positions[b] + t (none when that is negative: zeros).  With return_lse (or an lse tensor) also the
     log-sum-exp of the scaled scores, fp32 [B, heads, T]."""
-    dim = pages.k.shape[3]
+    dim, shape = pages.head_dim, q.shape
     qp = _q8_rows(q, "q", None, dim)
-    batch, tokens, n_heads = q.shape[:3]
+    batch, tokens, n_heads = shape[0], shape[1], shape[2]
     out = _q8_out(q, out)
+    o_strides = out.stride()
     max_len = _q8_max_len(max_len, block_table, pages)
-    lse = _q8_lse(lse, return_lse, (batch, n_heads, tokens), q.device)
-    if workspace is None:
-        need = int(_lib.lib().raw("t2c_attn_prefill_q8_workspace")(pages.ref, block_table.shape[1], batch, tokens,
-                                                                   n_heads, max_len, splits))
-    else:
-        need = 0
-    workspace, floats = _q8_workspace(workspace, need, q.device)
-    _lib.lib().call("t2c_attn_prefill_q8", pages.ref, *qp, _lib.ptr(out), *out.stride()[:3], _lib.ptr(lse),
-                    _q8_index(positions, batch, "positions"), *_q8_table(block_table, batch), batch, tokens, n_heads,
-                    dim ** -0.5 if scale is None else float(scale), max_len, splits, _lib.ptr(workspace), floats,
+    lse = _q8_lse(lse, return_lse, (batch, n_heads, tokens), q)
+    workspace, floats = _q8_workspace(workspace, q, pages, "t2c_attn_prefill_q8_workspace", block_table.shape[1], batch,
+                                      tokens, n_heads, max_len, splits)
+    _lib.lib().call("t2c_attn_prefill_q8", pages.ref, *qp, _lib.ptr(out), o_strides[0], o_strides[1], o_strides[2],
+                    _lib.ptr(lse), _q8_index(positions, batch, "positions"), *_q8_table(block_table, batch), batch, tokens,
+                    n_heads, dim ** -0.5 if scale is None else scale, max_len, splits, _lib.ptr(workspace), floats,
                     _lib.stream_ptr())
     return out if lse is None else (out, lse)
 
@@ -1018,15 +1026,15 @@ def attn_key_weights_q8(q: torch.Tensor, lse: torch.Tensor, pages: Q8Pages, posi
     """The attention weight that queries q [B, T, heads, head_dim] (log-sum-exps lse [B, heads, T] from
     attn_prefill_q8) give each cached key, summed over queries and the heads of a group and added to weights for
     positions before positions[b]; weights_out fp32 [B, n_kv, positions] is written up to the last query's key."""
-    heads, dim = pages.k.shape[1], pages.k.shape[3]
+    heads, dim, shape = pages.n_kv, pages.head_dim, q.shape
     qp = _q8_rows(q, "q", None, dim)
-    batch, tokens, n_heads = q.shape[:3]
+    batch, tokens, n_heads = shape[0], shape[1], shape[2]
     max_len = _q8_max_len(max_len, block_table, pages)
-    lse = _q8_lse(lse, False, (batch, n_heads, tokens), q.device)
+    _q8_lse(lse, False, (batch, n_heads, tokens), q)
     wargs = _q8_weights(weights, weights_out, batch, heads, max_len)
     _lib.lib().call("t2c_attn_key_weights_q8", pages.ref, *qp, _lib.ptr(lse), _q8_index(positions, batch, "positions"),
                     *_q8_table(block_table, batch), batch, tokens, n_heads,
-                    dim ** -0.5 if scale is None else float(scale), max_len, *wargs, _lib.stream_ptr())
+                    dim ** -0.5 if scale is None else scale, max_len, *wargs, _lib.stream_ptr())
     return weights_out
 
 
@@ -1039,26 +1047,25 @@ def kv_cache_evict_q8(pages: Q8Pages, weights: torch.Tensor, lengths: torch.Tens
     positions 0.. of out_table's pages (default: block_table's own, in place; another table's pages must be
     disjoint from them), their weights to weights_out (default in place: weights itself).
     Returns (kept positions int32 [B, n_kv, keep], ascending then -1; new lengths int32 [B])."""
-    heads = pages.k.shape[1]
+    heads = pages.n_kv
     batch = lengths.numel()
-    capacity = block_table.shape[1] * pages.k.shape[2]
+    capacity = block_table.shape[1] * pages.page_size
     if weights.dtype != torch.float32 or weights.dim() != 3 or weights.stride(2) != 1 or weights.shape[0] < batch \
             or weights.shape[1] != heads or weights.shape[2] < capacity:
         raise ValueError(f"weights must be float32 [batch, {heads}, at least {capacity}] with unit last stride")
     if out_table is None:
         out_table = block_table
     if weights_out is None:
-        weights_out = weights if out_table is block_table else torch.empty(batch, heads, keep, dtype=torch.float32,
-                                                                           device=weights.device)
+        weights_out = weights if out_table is block_table else weights.new_empty((batch, heads, keep))
     if weights_out.dtype != torch.float32 or weights_out.dim() != 3 or weights_out.stride(2) != 1 \
             or weights_out.shape[0] < batch or weights_out.shape[1] != heads or weights_out.shape[2] < keep:
         raise ValueError(f"weights_out must be float32 [batch, {heads}, at least {keep}] with unit last stride")
     if kept is None:
-        kept = torch.empty(batch, heads, keep, dtype=torch.int32, device=weights.device)
+        kept = lengths.new_empty((batch, heads, keep))
     elif kept.dtype != torch.int32 or kept.shape != (batch, heads, keep) or not kept.is_contiguous():
         raise ValueError(f"kept must be contiguous int32 {(batch, heads, keep)}")
     if new_lengths is None:
-        new_lengths = torch.empty(batch, dtype=torch.int32, device=weights.device)
+        new_lengths = torch.empty_like(lengths)
     _lib.lib().call("t2c_kv_cache_evict_q8", pages.ref, _lib.ptr(weights), weights.stride(0), weights.stride(1),
                     _q8_index(lengths, batch, "lengths"), *_q8_table(block_table, batch), *_q8_table(out_table, batch),
                     batch, keep, sinks, recent, _lib.ptr(weights_out), weights_out.stride(0), weights_out.stride(1),
