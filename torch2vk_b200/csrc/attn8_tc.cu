@@ -1,0 +1,552 @@
+// Attention of many query tokens over the paged 8-bit KV cache on tcgen05.
+//
+// CTA = two query tiles of one (sequence, KV head) and a run of its key tiles.  A query tile is 128 rows: TT =
+// 128 / group tokens times the group's heads, so that one expansion of a key tile serves the whole group; row r is
+// token r / group, head r % group, and TMEM lane r.  Per 128-key tile j and query tile i:
+//   S_i = Q_i K_j^T     tcgen05.mma kind::f16, M = 128 rows, N = 128 keys, K = D, fp32 in TMEM
+//   P_i = 2^(S_i kf_j + log2 vs_j - m)   fp16 over S_i's columns in TMEM (A operand of the next product)
+//   O_i += P_i V_j      N = D, K = 128 keys, V as an MN-major operand
+// Roles: warps 0-3 and 4-7 the softmax of the two query tiles (a thread one row), warps 8-11 expand the int8 codes
+// to fp16 operand tiles (loads a tile ahead in registers), warp 12 issues the MMAs.  The tensor core runs
+// P V and the next S of one query tile while the other tile's softmax runs.
+//
+// Codes become fp16 exactly.  The scales stay in fp32 in the exponent: kf = k scale * softmax scale * log2 e; the V
+// scale joins as log2 vs, and the softmax sum takes P / vs.  One reference m per row serves all tiles until the P of
+// 16 keys sum to more than 2^14: then the row's m moves to its maximum - 8 and O, l are rescaled.  So no pass looks
+// for the maximum; P's rounding to fp16 (what the tensor core takes) is the only one before the output's.
+//
+// Within groups of four dims K and Q rows are held in the order 0, 2, 1, 3 (as the expansion leaves them; the product
+// does not see it), V's columns too, which the epilogue undoes.
+#include <type_traits>
+
+#include "kv8.cuh"
+#include "umma.cuh"
+
+namespace t2c {
+namespace {
+
+constexpr int kPRows = 128;   // rows of a query tile
+constexpr int kPKeys = 128;   // keys of a tile
+constexpr int kPThreads = 13 * 32;
+constexpr float kPRefStart = -1e30f;
+constexpr float kPSumTop = 16384.0f;  // sum of 16 P that moves the reference
+constexpr float kPRefDrop = 8.0f;
+
+template <int D>
+struct PrefillShape {
+    static constexpr int kTile = 128 * D * 2;          // bytes of a 128-row fp16 tile: D / 64 chunks of 16 KB
+    static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + 2 * kTile, kMeta = kV + 2 * kTile;
+    static constexpr int kBars = kMeta + 4 * 8 * 16;   // meta: ring of 4 tiles x 8 groups of 16 keys
+    static constexpr int kSmem = kBars + 256;
+};
+
+struct PrefillArgs {
+    KvPages pg;
+    const __half *q;
+    int64_t q_sb, q_st, q_sh;
+    __half *out;
+    int64_t o_sb, o_st, o_sh;
+    float *lse;
+    const int32_t *positions, *table;
+    int64_t t_stride, max_len;
+    int B, T, NH, pairs, splits;
+    float scale_log2;
+    float *parts;  // [B][n_kv][pairs][splits][256][D + 2]: O rows, then m and l of 256 rows
+};
+
+__device__ __forceinline__ uint32_t ph_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
+
+// byte offset of 16-byte unit u of row r of a tile: 64-value chunks of 16 KB, 128-byte swizzle
+__device__ __forceinline__ uint32_t unit_at(int r, int u) {
+    return static_cast<uint32_t>((u >> 3) * 16384 + r * 128 + (((u & 7) ^ (r & 7)) << 4));
+}
+
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+__device__ __forceinline__ float p_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __grid_constant__ PrefillArgs a) {
+    using S = PrefillShape<D>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t base = smem_u32(smem);
+    float4 *meta = reinterpret_cast<float4 *>(smem + S::kMeta);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kBars);
+    uint64_t *k_full = bars, *v_full = bars + 2, *k_free = bars + 4, *v_free = bars + 6, *s_ready = bars + 8,
+             *p_ready = bars + 10, *q_full = bars + 12, *o_done = bars + 13, *meta_full = bars + 14;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 18);
+    volatile int *stop = reinterpret_cast<volatile int *>(bars + 19);
+    if (base & 1023u) {  // the swizzle atoms need it: report, compute nothing
+        if (threadIdx.x == 0) report_device_error(T2C_EUNSUPPORTED);
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        for (int i = 0; i < 4; ++i) mbar_init(bars + i, 128);       // k_full, v_full: the expanding threads
+        for (int i = 4; i < 10; ++i) mbar_init(bars + i, 1);        // commits
+        mbar_init(p_ready, 128);
+        mbar_init(p_ready + 1, 128);
+        mbar_init(q_full, 256);
+        mbar_init(o_done, 1);
+        for (int i = 0; i < 4; ++i) mbar_init(meta_full + i, 1);
+        *stop = 0;
+        fence_mbar_init();
+    }
+    if (warp == 12) tmem_alloc(tmem_slot, 512);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(tmem_slot);
+    pdl_wait();
+    pdl_trigger();
+
+    // ---- this CTA's item: the pairs with most keys first
+    const int group = a.NH / a.pg.n_kv, TT = kPRows / group;
+    int item = blockIdx.x;
+    const int split = item % a.splits;
+    item /= a.splits;
+    const int head = item % a.pg.n_kv;
+    item /= a.pg.n_kv;
+    const int b = item % a.B;
+    const int pair = a.pairs - 1 - item / a.B;
+    const int64_t p0 = a.positions[b];
+    const int t_first = pair * 2 * TT, t_last = min(t_first + 2 * TT, a.T) - 1;
+    int64_t n = p0 + t_last + 1;  // keys the last query sees
+    if (n > a.max_len) {
+        if (tid == 0) report_device_error(T2C_EINVAL);
+        n = a.max_len;
+    }
+    if (n < 0) n = 0;
+    const int all_tiles = static_cast<int>((n + kPKeys - 1) / kPKeys);
+    const int per = (all_tiles + a.splits - 1) / a.splits;
+    const int tile0 = min(split * per, all_tiles), tiles = min(per, all_tiles - tile0);
+
+    if (tiles > 0) {
+        if (warp < 8) {
+            // ================================================== softmax: tile `qi`, row `row`
+            const int qi = warp >> 2, row = tid & 127;
+            const int t = t_first + qi * TT + row / group, h = head * group + row % group;
+            const bool real = row < TT * group && t < a.T;
+            {
+                const __half *q = a.q + b * a.q_sb + static_cast<int64_t>(t) * a.q_st + h * a.q_sh;
+                const uint32_t at = base + S::kQ + qi * S::kTile;
+#pragma unroll
+                for (int u = 0; u < D / 8; ++u) {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (real) v = ldg_nc_v4(q + 8 * u);
+                    sts128(at + unit_at(row, u), __byte_perm(v.x, v.y, 0x5410), __byte_perm(v.x, v.y, 0x7632),
+                           __byte_perm(v.z, v.w, 0x5410), __byte_perm(v.z, v.w, 0x7632));
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(q_full);
+            }
+            // last key of this row, and of the tile's first token: rows past the end follow the last real token
+            const int64_t limit = min(p0 + min(t, a.T - 1), n - 1);
+            const int64_t least = min(p0 + min(t_first + qi * TT, a.T - 1), n - 1);
+            const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
+            const uint32_t s_at = lanes + 128 * qi, o_at = lanes + 256 + D * qi;
+            float m = kPRefStart, l = 0.0f;
+            bool ok = true;
+            for (int j = 0; j < tiles; ++j) {
+                ok = mbar_wait_or(&s_ready[qi], j & 1, stop);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                mbar_wait_or(&meta_full[j & 3], (j >> 2) & 1, stop);  // complete: S was made after it
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const int64_t k0 = static_cast<int64_t>(tile0 + j) * kPKeys;
+                const bool masked = k0 + kPKeys - 1 > least;
+                const int last = static_cast<int>(max(min(limit - k0, static_cast<int64_t>(kPKeys)), static_cast<int64_t>(-1)));
+                const float4 *f = meta + (j & 3) * 8;
+                uint32_t p[kPKeys / 2];
+                float lt;
+                bool high;
+                const auto exponents = [&](auto hide) {
+                    lt = 0.0f;
+                    high = false;
+                    uint32_t s[2][32];
+                    tmem_ld32(s_at, s[0]);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        tmem_ld_wait();
+                        if (c < 3) tmem_ld32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float4 k = f[2 * c + e];
+                            const float shift = k.y - m;
+                            float y[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                y[i] = fmaf(__uint_as_float(s[c & 1][16 * e + i]), k.x, shift);
+                                if (hide && 32 * c + 16 * e + i > last) y[i] = -INFINITY;
+                            }
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) y[i] = p_exp2(y[i]);
+                            float sum[4] = {y[0], y[1], y[2], y[3]};
+#pragma unroll
+                            for (int i = 4; i < 16; ++i) sum[i & 3] += y[i];
+                            const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                            high |= total > kPSumTop;
+                            lt = fmaf(total, k.z, lt);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) p[16 * c + 8 * e + i] = ph_bits(__floats2half2_rn(y[2 * i], y[2 * i + 1]));
+                        }
+                    }
+                };
+                for (int pass = 0;; ++pass) {
+                    if (masked)
+                        exponents(std::true_type{});
+                    else
+                        exponents(std::false_type{});
+                    if (pass > 0 || !__any_sync(0xffffffffu, high)) break;
+                    // ---- rare: the reference of the rows that ask for it moves to their maximum - 8
+                    float top = -INFINITY;
+#pragma unroll 1
+                    for (int c = 0; c < 8; ++c) {
+                        uint32_t v[16];
+                        tmem_ld16(s_at + 16 * c, v);
+                        tmem_ld_wait();
+                        const float4 k = f[c];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float x = fmaf(__uint_as_float(v[i]), k.x, k.y);
+                            if (!masked || 16 * c + i <= last) top = fmaxf(top, x);
+                        }
+                    }
+                    const float ref = high ? top - kPRefDrop : m;
+                    const float corr = p_exp2(m - ref);
+                    m = ref;
+                    l *= corr;
+                    if (j > 0) {  // S being ready says that P V of the tile before is too
+#pragma unroll 1
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t v[16];
+                            tmem_ld16(o_at + 16 * c, v);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
+                            tmem_st16(o_at + 16 * c, v);
+                        }
+                    }
+                }
+                l += lt;
+                tmem_st32(s_at, p);
+                tmem_st32(s_at + 32, p + 32);
+                tmem_st_wait();
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                mbar_arrive(&p_ready[qi]);
+            }
+            ok = mbar_wait_or(o_done, 0, stop);
+            if (__all_sync(0xffffffffu, ok)) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const bool seen = limit >= 0;
+                if (a.splits > 1) {
+                    float *part = a.parts + (((static_cast<int64_t>(b) * a.pg.n_kv + head) * a.pairs + pair) * a.splits + split) *
+                                                (256 * (D + 2));
+                    float *dst = part + (qi * 128 + row) * D;
+#pragma unroll 1
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t v[16];
+                        tmem_ld16(o_at + 16 * c, v);
+                        tmem_ld_wait();
+                        if (real) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                reinterpret_cast<uint4 *>(dst)[4 * c + i] = make_uint4(v[4 * i], v[4 * i + 2], v[4 * i + 1], v[4 * i + 3]);
+                        }
+                    }
+                    part[256 * D + qi * 128 + row] = m;
+                    part[256 * (D + 1) + qi * 128 + row] = l;
+                } else {
+                    const float inv = seen ? 1.0f / l : 0.0f;
+                    __half *o = a.out + b * a.o_sb + static_cast<int64_t>(t) * a.o_st + h * a.o_sh;
+#pragma unroll 1
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t v[16];
+                        tmem_ld16(o_at + 16 * c, v);
+                        tmem_ld_wait();
+                        float x[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[i] = seen ? __uint_as_float(v[i]) * inv : 0.0f;
+                        if (real) {
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+                                reinterpret_cast<uint4 *>(o)[2 * c + i] =
+                                    make_uint4(ph_bits(__floats2half2_rn(x[8 * i], x[8 * i + 2])),
+                                               ph_bits(__floats2half2_rn(x[8 * i + 1], x[8 * i + 3])),
+                                               ph_bits(__floats2half2_rn(x[8 * i + 4], x[8 * i + 6])),
+                                               ph_bits(__floats2half2_rn(x[8 * i + 5], x[8 * i + 7])));
+                        }
+                    }
+                    if (real && a.lse)
+                        a.lse[(static_cast<int64_t>(b) * a.NH + h) * a.T + t] =
+                            seen ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+                }
+            }
+        } else if (warp < 12) {
+            // ================================================== expansion: 16-byte unit `c` of rows r0, r0 + kStep, ..
+            constexpr int kPerRow = D / 16, kStep = 128 / kPerRow, kPasses = 128 / kStep;
+            const int et = tid - 256, c = et % kPerRow, r0 = et / kPerRow;
+            const int32_t *bt = a.table + b * a.t_stride;
+            const int slice = lane & 7;  // the lane's 16 keys of a tile: their page and scales
+            int page = 0;
+            const auto look = [&](int j) {
+                const int64_t key = static_cast<int64_t>(tile0 + j) * kPKeys + 16 * slice;
+                page = j < tiles && key < n ? max(kv8_page(a.pg, bt, key), 0) : 0;
+            };
+            const auto fetch = [&](const int8_t *codes, int j, uint4 *x) {
+                const int64_t k0 = static_cast<int64_t>(tile0 + j) * kPKeys;
+#pragma unroll
+                for (int i = 0; i < kPasses; ++i) {
+                    const int r = r0 + i * kStep;
+                    const int pg = __shfl_sync(0xffffffffu, page, r >> 4);
+                    x[i] = make_uint4(0, 0, 0, 0);  // keys past the end: value 0, and hidden
+                    if (j < tiles && k0 + r < n) x[i] = ldg_nc_v4(codes + kv8_row_offset(a.pg, pg, head, k0 + r) + 16 * c);
+                }
+            };
+            // Eight lanes of a row write units 2c and 2c + 1 of both chunks: half of them the odd one first, so that
+            // a store instruction touches every bank once
+            const bool odd_first = D == 128 && c >= 4;
+            const auto expand = [&](uint32_t tile, const uint4 *x) {
+#pragma unroll
+                for (int i = 0; i < kPasses; ++i) {
+                    const int r = r0 + i * kStep;
+                    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                    uint32_t v[8];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        __half2 even, odd;
+                        kv8_unpack(w[e], even, odd);
+                        v[2 * e] = ph_bits(even);
+                        v[2 * e + 1] = ph_bits(odd);
+                    }
+                    const uint32_t at0 = tile + unit_at(r, 2 * c), at1 = tile + unit_at(r, 2 * c + 1);
+                    const bool f = odd_first;
+                    sts128(f ? at1 : at0, f ? v[4] : v[0], f ? v[5] : v[1], f ? v[6] : v[2], f ? v[7] : v[3]);
+                    sts128(f ? at0 : at1, f ? v[0] : v[4], f ? v[1] : v[5], f ? v[2] : v[6], f ? v[3] : v[7]);
+                }
+            };
+            uint4 kx[kPasses], vx[kPasses];
+            look(0);
+            fetch(a.pg.k, 0, kx);
+            fetch(a.pg.v, 0, vx);
+            for (int j = 0; j < tiles; ++j) {
+                const int st = j & 1;
+                // the factors of the tile's 8 groups of 16 keys (the ring of 4 outlives their readers)
+                if (et < 8) {
+                    const int64_t key = static_cast<int64_t>(tile0 + j) * kPKeys + 16 * slice;
+                    float4 f = make_float4(0.0f, -24.0f, 0.0f, 0.0f);
+                    if (key < n) {
+                        const int64_t so = kv8_scale_offset(a.pg, page, head, key);
+                        const float vs = __half2float(a.pg.vs[so]);
+                        // a block of scale 0 has values 0: the least scale's exponent moves no reference
+                        f = make_float4(__half2float(a.pg.ks[so]) * a.scale_log2, vs == 0.0f ? -24.0f : log2f(vs),
+                                        vs == 0.0f ? 16777216.0f : 1.0f / vs, 0.0f);
+                    }
+                    meta[(j & 3) * 8 + slice] = f;
+                }
+                if (warp == 8) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&meta_full[j & 3]);
+                }
+                look(j + 1);
+                bool ok = j < 2 || mbar_wait_or(&k_free[st], ((j >> 1) - 1) & 1, stop);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                expand(base + S::kK + st * S::kTile, kx);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(&k_full[st]);
+                fetch(a.pg.k, j + 1, kx);
+                ok = j < 2 || mbar_wait_or(&v_free[st], ((j >> 1) - 1) & 1, stop);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                expand(base + S::kV + st * S::kTile, vx);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(&v_full[st]);
+                fetch(a.pg.v, j + 1, vx);
+            }
+        } else if (lane == 0) {
+            // ================================================== MMA
+            const uint32_t idesc_s = umma_idesc(128, 128, false), idesc_o = umma_idesc(128, D, true);
+            const auto scores = [&](int qi, int st) {
+                const uint32_t q = base + S::kQ + qi * S::kTile, k = base + S::kK + st * S::kTile;
+#pragma unroll
+                for (int s = 0; s < D / 16; ++s) {
+                    const uint32_t off = static_cast<uint32_t>((s >> 2) * 16384 + 32 * (s & 3));
+                    umma_ss(tmem + 128 * qi, umma_desc_k(q + off), umma_desc_k(k + off), idesc_s, s > 0);
+                }
+                umma_commit(&s_ready[qi]);
+            };
+            const auto values = [&](int qi, int st, bool acc) {
+                const uint32_t v = base + S::kV + st * S::kTile;
+#pragma unroll
+                for (int s = 0; s < kPKeys / 16; ++s)
+                    umma_ts(tmem + 256 + D * qi, tmem + 128 * qi + 8 * s, umma_desc_mn(v + 2048 * s, 16384), idesc_o, acc || s > 0);
+            };
+            bool ok = mbar_wait_or(q_full, 0, stop) && mbar_wait_or(&k_full[0], 0, stop);
+            if (ok) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                scores(0, 0);
+                scores(1, 0);
+                umma_commit(&k_free[0]);
+            }
+            for (int j = 0; j < tiles && ok; ++j) {
+                const int st = j & 1, next = st ^ 1;
+                const bool more = j + 1 < tiles;
+                ok = mbar_wait_or(&v_full[st], (j >> 1) & 1, stop) &&
+                     (!more || mbar_wait_or(&k_full[next], ((j + 1) >> 1) & 1, stop));
+#pragma unroll
+                for (int qi = 0; qi < 2; ++qi) {
+                    ok = ok && mbar_wait_or(&p_ready[qi], j & 1, stop);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    values(qi, st, j > 0);
+                    if (qi == 1) umma_commit(&v_free[st]);
+                    if (more) scores(qi, next);
+                }
+                if (ok && more) umma_commit(&k_free[next]);
+            }
+            umma_commit(o_done);
+            mbar_wait_or(o_done, 0, nullptr);  // nothing of this CTA is in flight when it frees its TMEM
+        }
+    } else if (warp < 8 && a.splits == 1) {
+        // no query of the pair sees a key: zeros
+        const int qi = warp >> 2, row = tid & 127;
+        const int t = t_first + qi * TT + row / group, h = head * group + row % group;
+        if (row < TT * group && t < a.T) {
+            uint4 *o = reinterpret_cast<uint4 *>(a.out + b * a.o_sb + static_cast<int64_t>(t) * a.o_st + h * a.o_sh);
+            for (int i = 0; i < D / 8; ++i) o[i] = make_uint4(0, 0, 0, 0);
+            if (a.lse) a.lse[(static_cast<int64_t>(b) * a.NH + h) * a.T + t] = -INFINITY;
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (tid == 0 && *stop) report_device_error(T2C_ETIMEOUT);
+    if (warp == 12) {
+        __syncwarp();
+        tmem_free(tmem, 512);
+    }
+}
+
+// Joins the splits, a warp per query row.
+template <int D>
+__global__ void __launch_bounds__(256) attn8_prefill_join_kernel(const __grid_constant__ PrefillArgs a) {
+    const int lane = threadIdx.x & 31;
+    const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    pdl_wait();
+    pdl_trigger();
+    if (w >= static_cast<int64_t>(a.B) * a.T * a.NH) return;
+    const int h = static_cast<int>(w % a.NH), t = static_cast<int>(w / a.NH % a.T), b = static_cast<int>(w / a.NH / a.T);
+    const int group = a.NH / a.pg.n_kv, TT = kPRows / group, head = h / group;
+    const int pair = t / (2 * TT), in_pair = t % (2 * TT);
+    const int row = in_pair / TT * 128 + in_pair % TT * group + h % group;
+    const int64_t p0 = a.positions[b];
+    const int64_t n = min(p0 + min(pair * 2 * TT + 2 * TT, a.T), a.max_len);  // as the CTA had it
+    const int tiles = n > 0 ? static_cast<int>((n + kPKeys - 1) / kPKeys) : 0;
+    const int per = (tiles + a.splits - 1) / a.splits, used = per > 0 ? (tiles + per - 1) / per : 0;
+    const float *base = a.parts + ((static_cast<int64_t>(b) * a.pg.n_kv + head) * a.pairs + pair) * a.splits * (256 * (D + 2));
+    const bool seen = p0 + t >= 0;
+    constexpr int kPer = D / 32;
+    float acc[kPer] = {}, top = kPRefStart, sum = 0.0f;
+    for (int s = lane; s < used; s += 32) top = fmaxf(top, base[static_cast<int64_t>(s) * 256 * (D + 2) + 256 * D + row]);
+    top = warp_max(top);
+#pragma unroll 4
+    for (int s = 0; s < used; ++s) {
+        const float *part = base + static_cast<int64_t>(s) * 256 * (D + 2);
+        const float f = p_exp2(part[256 * D + row] - top);
+        sum = fmaf(part[256 * (D + 1) + row], f, sum);
+        const float *o = part + row * D + kPer * lane;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) acc[i] = fmaf(o[i], f, acc[i]);
+    }
+    const float inv = seen ? 1.0f / sum : 0.0f;
+    __half2 *out = reinterpret_cast<__half2 *>(a.out + b * a.o_sb + static_cast<int64_t>(t) * a.o_st + h * a.o_sh) + kPer / 2 * lane;
+#pragma unroll
+    for (int i = 0; i < kPer / 2; ++i)
+        out[i] = seen ? __floats2half2_rn(acc[2 * i] * inv, acc[2 * i + 1] * inv) : __float2half2_rn(0.0f);
+    if (a.lse && lane == 0)
+        a.lse[(static_cast<int64_t>(b) * a.NH + h) * a.T + t] = seen ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+}
+
+}  // namespace
+
+cudaError_t status_attn8_tc(unsigned int *bits, int clear, cudaStream_t s) { return read_tu_status(bits, clear, s); }
+
+}  // namespace t2c
+
+using namespace t2c;
+
+namespace {
+
+struct PrefillPlan {
+    int pairs, splits;
+    int64_t floats;
+};
+
+// One CTA per SM: the keys of a pair of query tiles are split while CTAs would be missing, at least two tiles each.
+PrefillPlan prefill_plan(int64_t B, int64_t T, int64_t NH, int64_t NK, int64_t D, int64_t max_len, int64_t splits) {
+    PrefillPlan r = {};
+    const int64_t tokens = 2 * (kPRows / (NH / NK));
+    r.pairs = static_cast<int>((T + tokens - 1) / tokens);
+    const int64_t items = B * NK * r.pairs, tiles = (max_len + kPKeys - 1) / kPKeys;
+    int64_t s = splits;
+    if (s == 0) {
+        s = sm_count() / items;
+        s = s > tiles / 2 ? tiles / 2 : s;
+    }
+    s = s > 64 ? 64 : s;
+    r.splits = static_cast<int>(s < 1 ? 1 : s);
+    r.floats = r.splits > 1 ? items * r.splits * 256 * (D + 2) : 0;
+    return r;
+}
+
+}  // namespace
+
+extern "C" int64_t t2c_attn_prefill_q8_workspace(const t2c_q8_pages *pages, int64_t bt_width, int64_t B, int64_t T,
+                                                 int64_t NH, int64_t max_len, int64_t splits) {
+    if (!pages || pages->n_kv <= 0 || NH <= 0 || NH % pages->n_kv || NH / pages->n_kv > kPRows || B <= 0 || T <= 0 ||
+        splits < 0 || bt_width <= 0)
+        return -1;
+    const int64_t capacity = bt_width * pages->page_size;
+    if (max_len <= 0 || max_len > capacity) max_len = capacity;
+    return prefill_plan(B, T, NH, pages->n_kv, pages->head_dim, max_len, splits).floats;
+}
+
+extern "C" int t2c_attn_prefill_q8(const t2c_q8_pages *pages, const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                                   void *out, int64_t o_sb, int64_t o_st, int64_t o_sh, float *lse,
+                                   const int32_t *positions, const int32_t *block_table, int64_t bt_stride,
+                                   int64_t bt_width, int64_t B, int64_t T, int64_t NH, float scale, int64_t max_len,
+                                   int64_t splits, float *workspace, int64_t workspace_floats, void *stream) {
+    PrefillArgs a = {};
+    int rc = kv8_attn_check(pages, "attn_prefill_q8", a.pg, block_table, bt_stride, bt_width, positions, B, T, NH, max_len);
+    if (rc != T2C_OK) return rc;
+    if (!kv8_strides(q, q_sb, q_st, q_sh) || !kv8_strides(out, o_sb, o_st, o_sh))
+        return set_error(T2C_EINVAL, "attn_prefill_q8: q and out rows must be 16-byte aligned");
+    if (splits < 0) return set_error(T2C_EINVAL, "attn_prefill_q8: splits %lld", (long long)splits);
+    const int64_t D = pages->head_dim;
+    if (NH / a.pg.n_kv > kPRows) return set_error(T2C_EUNSUPPORTED, "attn_prefill_q8: group %lld", (long long)(NH / a.pg.n_kv));
+    const PrefillPlan plan = prefill_plan(B, T, NH, a.pg.n_kv, D, max_len, splits);
+    if (plan.floats > 0 && (!workspace || workspace_floats < plan.floats))
+        return set_error(T2C_ESCRATCH, "attn_prefill_q8: workspace needs %lld floats", (long long)plan.floats);
+    if (!kv8_aligned(workspace, 16)) return set_error(T2C_EINVAL, "attn_prefill_q8: workspace must be 16-byte aligned");
+    a.q = static_cast<const __half *>(q), a.q_sb = q_sb, a.q_st = q_st, a.q_sh = q_sh;
+    a.out = static_cast<__half *>(out), a.o_sb = o_sb, a.o_st = o_st, a.o_sh = o_sh;
+    a.lse = lse;
+    a.positions = positions, a.table = block_table, a.t_stride = bt_stride, a.max_len = max_len;
+    a.B = static_cast<int>(B), a.T = static_cast<int>(T), a.NH = static_cast<int>(NH);
+    a.pairs = plan.pairs, a.splits = plan.splits;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.parts = workspace;
+    const int64_t ctas = B * a.pg.n_kv * plan.pairs * plan.splits, rows = B * T * NH;
+    if (ctas > INT32_MAX) return set_error(T2C_EINVAL, "attn_prefill_q8: bad shape");
+    const cudaStream_t s = as_stream(stream);
+    const auto kern = D == 128 ? attn8_prefill_kernel<128> : attn8_prefill_kernel<64>;
+    const int smem = D == 128 ? PrefillShape<128>::kSmem : PrefillShape<64>::kSmem;
+    rc = kv8_configure(kern, smem, D == 128 ? 2 : 3, "attn_prefill_q8");
+    if (rc == T2C_OK) rc = kv8_launch("attn_prefill_q8", kern, dim3(static_cast<unsigned>(ctas)), dim3(kPThreads), smem, 1, s, a);
+    if (rc != T2C_OK || plan.splits == 1) return rc;
+    return kv8_launch("attn_prefill_q8 join", D == 128 ? attn8_prefill_join_kernel<128> : attn8_prefill_join_kernel<64>,
+                      dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, 1, s, a);
+}

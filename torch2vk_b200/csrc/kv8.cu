@@ -51,6 +51,19 @@ int kv8_table(const t2c_q8_pages *p, const int32_t *table, int64_t stride, int64
     return T2C_OK;
 }
 
+int kv8_attn_check(const t2c_q8_pages *pages, const char *what, KvPages &pg, const int32_t *table, int64_t bt_stride,
+          int64_t bt_width, const int32_t *positions, int64_t B, int64_t T, int64_t NH, int64_t &max_len) {
+    int64_t capacity = 0;
+    int rc = kv8_view(pages, what, pg);
+    if (rc == T2C_OK) rc = kv8_table(pages, table, bt_stride, bt_width, what, capacity);
+    if (rc != T2C_OK) return rc;
+    if (!positions) return set_error(T2C_EINVAL, "%s: NULL positions", what);
+    if (B <= 0 || T <= 0 || NH <= 0 || NH % pg.n_kv || B > 65535 || B * T * NH > INT32_MAX)
+        return set_error(T2C_EINVAL, "%s: bad shape", what);
+    if (max_len <= 0 || max_len > capacity) max_len = capacity;
+    return T2C_OK;
+}
+
 bool kv8_maps(const t2c_q8_pages *p, int rows, CUtensorMap &k_map, CUtensorMap &v_map) {
     static PFN_cuTensorMapEncodeTiled encode = [] {
         void *fn = nullptr;

@@ -28,6 +28,10 @@ int kv8_view(const t2c_q8_pages *pages, const char *what, KvPages &out);
 int kv8_table(const t2c_q8_pages *pages, const int32_t *table, int64_t stride, int64_t width, const char *what,
               int64_t &capacity);
 
+// What the attention entry points check alike; max_len becomes the bound in positions.
+int kv8_attn_check(const t2c_q8_pages *pages, const char *what, KvPages &pg, const int32_t *table, int64_t bt_stride,
+                   int64_t bt_width, const int32_t *positions, int64_t B, int64_t T, int64_t NH, int64_t &max_len);
+
 // Tensor maps of the codes as (dim, row of page, KV head, page), boxes of `rows` rows of one head in the swizzle that
 // is as wide as a row (128 or 64 bytes).  False when the driver refuses.
 bool kv8_maps(const t2c_q8_pages *pages, int rows, CUtensorMap &k_map, CUtensorMap &v_map);
@@ -120,6 +124,25 @@ int kv8_launch(const char *what, Kernel kernel, dim3 grid, dim3 block, size_t sm
     return T2C_OK;
 }
 
+// Raises a kernel's shared-memory limit once per device; `slot` numbers the kernel.
+template <typename Kernel>
+int kv8_configure(Kernel kern, int smem, int slot, const char *what) {
+    static bool done[16][64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+    if (!done[slot][dev]) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+            return set_error(T2C_ECUDA, "%s: cudaFuncSetAttribute failed", what);
+        done[slot][dev] = true;
+    }
+    return T2C_OK;
+}
+
 inline bool kv8_aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+
+// An fp16 tensor whose rows are 16-byte aligned.
+inline bool kv8_strides(const void *p, int64_t a, int64_t b, int64_t c) {
+    return p && kv8_aligned(p, 16) && a % 8 == 0 && b % 8 == 0 && c % 8 == 0;
+}
 
 }  // namespace t2c
