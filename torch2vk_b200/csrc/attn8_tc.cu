@@ -6,8 +6,8 @@
 //   S_i = Q_i K_j^T     tcgen05.mma kind::f16, M = 128 rows, N = 128 keys, K = D, fp32 in TMEM
 //   P_i = 2^(S_i kf_j + log2 vs_j - m)   fp16 over S_i's columns in TMEM (A operand of the next product)
 //   O_i += P_i V_j      N = D, K = 128 keys, V as an MN-major operand
-// Roles: warps 0-3 and 4-7 the softmax of the two query tiles (a thread one row), warps 8-11 expand the int8 codes
-// to fp16 operand tiles (loads a tile ahead in registers), warp 12 issues the MMAs.  The tensor core runs
+// Roles: warps 0-3 and 4-7 the softmax of the two query tiles (a thread one row), warps 8-15 expand the int8 codes
+// to fp16 operand tiles (loads a tile ahead in registers), warp 16 issues the MMAs.  The tensor core runs
 // P V and the next S of one query tile while the other tile's softmax runs.
 //
 // Codes become fp16 exactly.  The scales stay in fp32 in the exponent: kf = k scale * softmax scale * log2 e; the V
@@ -27,7 +27,7 @@ namespace {
 
 constexpr int kPRows = 128;   // rows of a query tile
 constexpr int kPKeys = 128;   // keys of a tile
-constexpr int kPThreads = 13 * 32;
+constexpr int kPThreads = 640;
 constexpr float kPRefStart = -1e30f;
 constexpr float kPSumTop = 16384.0f;  // sum of 16 P that moves the reference
 constexpr float kPRefDrop = 8.0f;
@@ -71,6 +71,38 @@ __device__ __forceinline__ float p_exp2(float x) {
     return y;
 }
 
+// Two fp32 values in a register pair, and the packed operations on them.
+__device__ __forceinline__ uint64_t pair2(float x, float y) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ float2 unpair2(uint64_t v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+
+// Registers of the roles, of the 640 x 96 the CTA has: 2 x 144 + 2 x 72 + 48 = 5 x 96.
+template <int R>
+__device__ __forceinline__ void more_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
+}
+template <int R>
+__device__ __forceinline__ void fewer_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
+}
+
 template <int D>
 __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __grid_constant__ PrefillArgs a) {
     using S = PrefillShape<D>;
@@ -88,17 +120,17 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
     }
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
-        for (int i = 0; i < 4; ++i) mbar_init(bars + i, 128);       // k_full, v_full: the expanding threads
+        for (int i = 0; i < 4; ++i) mbar_init(bars + i, 8);         // k_full, v_full: the expanding warps
         for (int i = 4; i < 10; ++i) mbar_init(bars + i, 1);        // commits
         mbar_init(p_ready, 128);
         mbar_init(p_ready + 1, 128);
         mbar_init(q_full, 256);
         mbar_init(o_done, 1);
-        for (int i = 0; i < 4; ++i) mbar_init(meta_full + i, 1);
+        for (int i = 0; i < 4; ++i) mbar_init(meta_full + i, 8);
         *stop = 0;
         fence_mbar_init();
     }
-    if (warp == 12) tmem_alloc(tmem_slot, 512);
+    if (warp == 16) tmem_alloc(tmem_slot, 512);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -130,6 +162,7 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
     if (tiles > 0) {
         if (warp < 8) {
             // ================================================== softmax: tile `qi`, row `row`
+            more_registers<144>();
             const int qi = warp >> 2, row = tid & 127;
             const int t = t_first + qi * TT + row / group, h = head * group + row % group;
             const bool real = row < TT * group && t < a.T;
@@ -168,33 +201,33 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                 const auto exponents = [&](auto hide) {
                     lt = 0.0f;
                     high = false;
-                    uint32_t s[2][32];
-                    tmem_ld32(s_at, s[0]);
+                    uint32_t s[2][16];
+                    tmem_ld16(s_at, s[0]);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                    for (int c = 0; c < 8; ++c) {
                         tmem_ld_wait();
-                        if (c < 3) tmem_ld32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
+                        if (c < 7) tmem_ld16(s_at + 16 * (c + 1), s[(c + 1) & 1]);
+                        const float4 k = f[c];
+                        const uint64_t kk = pair2(k.x, k.x), shift = pair2(k.y - m, k.y - m);
+                        uint64_t sum[2];
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float4 k = f[2 * c + e];
-                            const float shift = k.y - m;
-                            float y[16];
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                y[i] = fmaf(__uint_as_float(s[c & 1][16 * e + i]), k.x, shift);
-                                if (hide && 32 * c + 16 * e + i > last) y[i] = -INFINITY;
+                        for (int i = 0; i < 8; ++i) {
+                            const uint32_t *x = s[c & 1] + 2 * i;
+                            float2 y = unpair2(fma2(pair2(__uint_as_float(x[0]), __uint_as_float(x[1])), kk, shift));
+                            if (hide) {
+                                const int at = 16 * c + 2 * i;
+                                y.x = at > last ? -INFINITY : y.x;
+                                y.y = at + 1 > last ? -INFINITY : y.y;
                             }
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) y[i] = p_exp2(y[i]);
-                            float sum[4] = {y[0], y[1], y[2], y[3]};
-#pragma unroll
-                            for (int i = 4; i < 16; ++i) sum[i & 3] += y[i];
-                            const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                            high |= total > kPSumTop;
-                            lt = fmaf(total, k.z, lt);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) p[16 * c + 8 * e + i] = ph_bits(__floats2half2_rn(y[2 * i], y[2 * i + 1]));
+                            y.x = p_exp2(y.x);
+                            y.y = p_exp2(y.y);
+                            sum[i & 1] = i < 2 ? pair2(y.x, y.y) : add2(sum[i & 1], pair2(y.x, y.y));
+                            p[8 * c + i] = ph_bits(__floats2half2_rn(y.x, y.y));
                         }
+                        const float2 both = unpair2(add2(sum[0], sum[1]));
+                        const float total = both.x + both.y;
+                        high |= total > kPSumTop;
+                        lt = fmaf(total, k.z, lt);
                     }
                 };
                 for (int pass = 0;; ++pass) {
@@ -287,34 +320,33 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                             seen ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
                 }
             }
-        } else if (warp < 12) {
-            // ================================================== expansion: 16-byte unit `c` of rows r0, r0 + kStep, ..
-            constexpr int kPerRow = D / 16, kStep = 128 / kPerRow, kPasses = 128 / kStep;
-            const int et = tid - 256, c = et % kPerRow, r0 = et / kPerRow;
+        } else if (warp < 16) {
+            // ================================================== expansion: a warp 16 keys, so one page and one scale
+            fewer_registers<72>();
+            constexpr int kPerRow = D / 16, kRows = 32 / kPerRow, kPasses = 16 / kRows;
+            const int slice = warp - 8;
+            // Eight lanes write a unit of two rows' quarters: every bank once per store instruction
+            const int c = D == 128 ? (lane & 3) + 4 * ((lane >> 3) & 1) : lane & 3;
+            const int r0 = D == 128 ? ((lane >> 2) & 1) + 2 * (lane >> 4) : lane >> 2;
             const int32_t *bt = a.table + b * a.t_stride;
-            const int slice = lane & 7;  // the lane's 16 keys of a tile: their page and scales
-            int page = 0;
-            const auto look = [&](int j) {
-                const int64_t key = static_cast<int64_t>(tile0 + j) * kPKeys + 16 * slice;
-                page = j < tiles && key < n ? max(kv8_page(a.pg, bt, key), 0) : 0;
-            };
-            const auto fetch = [&](const int8_t *codes, int j, uint4 *x) {
-                const int64_t k0 = static_cast<int64_t>(tile0 + j) * kPKeys;
+            const int64_t lane_off = head * a.pg.head_stride + r0 * a.pg.row_stride + 16 * c;
+            const int page_mask = (1 << a.pg.page_log2) - 1;
+            int64_t key = static_cast<int64_t>(tile0) * kPKeys + 16 * slice;  // the slice's first key
+            const auto look = [&](int64_t k) { return k < n ? max(kv8_page(a.pg, bt, k), 0) : 0; };
+            const auto fetch = [&](const int8_t *codes, int64_t k, int page, uint4 *x) {
+                const int8_t *at = codes + page * a.pg.page_stride + (static_cast<int>(k) & page_mask) * a.pg.row_stride + lane_off;
+                const int64_t left = n - k - r0;  // keys past the end: value 0, and hidden
 #pragma unroll
                 for (int i = 0; i < kPasses; ++i) {
-                    const int r = r0 + i * kStep;
-                    const int pg = __shfl_sync(0xffffffffu, page, r >> 4);
-                    x[i] = make_uint4(0, 0, 0, 0);  // keys past the end: value 0, and hidden
-                    if (j < tiles && k0 + r < n) x[i] = ldg_nc_v4(codes + kv8_row_offset(a.pg, pg, head, k0 + r) + 16 * c);
+                    x[i] = make_uint4(0, 0, 0, 0);
+                    if (i * kRows < left) x[i] = ldg_nc_v4(at);
+                    at += kRows * a.pg.row_stride;
                 }
             };
-            // Eight lanes of a row write units 2c and 2c + 1 of both chunks: half of them the odd one first, so that
-            // a store instruction touches every bank once
-            const bool odd_first = D == 128 && c >= 4;
+            const uint32_t at0 = unit_at(16 * slice + r0, 2 * c), at1 = unit_at(16 * slice + r0, 2 * c + 1);
             const auto expand = [&](uint32_t tile, const uint4 *x) {
 #pragma unroll
                 for (int i = 0; i < kPasses; ++i) {
-                    const int r = r0 + i * kStep;
                     const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
                     uint32_t v[8];
 #pragma unroll
@@ -324,21 +356,19 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                         v[2 * e] = ph_bits(even);
                         v[2 * e + 1] = ph_bits(odd);
                     }
-                    const uint32_t at0 = tile + unit_at(r, 2 * c), at1 = tile + unit_at(r, 2 * c + 1);
-                    const bool f = odd_first;
-                    sts128(f ? at1 : at0, f ? v[4] : v[0], f ? v[5] : v[1], f ? v[6] : v[2], f ? v[7] : v[3]);
-                    sts128(f ? at0 : at1, f ? v[0] : v[4], f ? v[1] : v[5], f ? v[2] : v[6], f ? v[3] : v[7]);
+                    // kRows rows on: for D = 128 the swizzle's row bits change with every second pass
+                    const uint32_t flip = D == 128 ? static_cast<uint32_t>((4 * i) & 4) << 4 : 0u;
+                    sts128(tile + (at0 ^ flip) + i * kRows * 128, v[0], v[1], v[2], v[3]);
+                    sts128(tile + (at1 ^ flip) + i * kRows * 128, v[4], v[5], v[6], v[7]);
                 }
             };
             uint4 kx[kPasses], vx[kPasses];
-            look(0);
-            fetch(a.pg.k, 0, kx);
-            fetch(a.pg.v, 0, vx);
+            int page = look(key);
+            fetch(a.pg.k, key, page, kx);
+            fetch(a.pg.v, key, page, vx);
             for (int j = 0; j < tiles; ++j) {
                 const int st = j & 1;
-                // the factors of the tile's 8 groups of 16 keys (the ring of 4 outlives their readers)
-                if (et < 8) {
-                    const int64_t key = static_cast<int64_t>(tile0 + j) * kPKeys + 16 * slice;
+                if (lane == 0) {  // the factors of these 16 keys (the ring of 4 outlives their readers)
                     float4 f = make_float4(0.0f, -24.0f, 0.0f, 0.0f);
                     if (key < n) {
                         const int64_t so = kv8_scale_offset(a.pg, page, head, key);
@@ -348,42 +378,46 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                                         vs == 0.0f ? 16777216.0f : 1.0f / vs, 0.0f);
                     }
                     meta[(j & 3) * 8 + slice] = f;
+                    mbar_arrive(&meta_full[j & 3]);
                 }
-                if (warp == 8) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&meta_full[j & 3]);
-                }
-                look(j + 1);
+                key += kPKeys;
+                if (j + 1 < tiles) page = look(key);
                 bool ok = j < 2 || mbar_wait_or(&k_free[st], ((j >> 1) - 1) & 1, stop);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 expand(base + S::kK + st * S::kTile, kx);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&k_full[st]);
-                fetch(a.pg.k, j + 1, kx);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&k_full[st]);
+                if (j + 1 < tiles) fetch(a.pg.k, key, page, kx);
                 ok = j < 2 || mbar_wait_or(&v_free[st], ((j >> 1) - 1) & 1, stop);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 expand(base + S::kV + st * S::kTile, vx);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&v_full[st]);
-                fetch(a.pg.v, j + 1, vx);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&v_full[st]);
+                if (j + 1 < tiles) fetch(a.pg.v, key, page, vx);
             }
-        } else if (lane == 0) {
+        } else {
+            fewer_registers<48>();
+            if (warp == 16 && lane == 0) {
             // ================================================== MMA
             const uint32_t idesc_s = umma_idesc(128, 128, false), idesc_o = umma_idesc(128, D, true);
             const auto scores = [&](int qi, int st) {
-                const uint32_t q = base + S::kQ + qi * S::kTile, k = base + S::kK + st * S::kTile;
+                uint32_t q = umma_desc_lo(base + S::kQ + qi * S::kTile), k = umma_desc_lo(base + S::kK + st * S::kTile);
+                asm volatile("" : "+r"(q), "+r"(k));  // the sums below are made here, not kept in registers across tiles
 #pragma unroll
                 for (int s = 0; s < D / 16; ++s) {
-                    const uint32_t off = static_cast<uint32_t>((s >> 2) * 16384 + 32 * (s & 3));
-                    umma_ss(tmem + 128 * qi, umma_desc_k(q + off), umma_desc_k(k + off), idesc_s, s > 0);
+                    const uint32_t off = static_cast<uint32_t>((s >> 2) * 1024 + 2 * (s & 3));  // 16-byte units
+                    umma_ss(tmem + 128 * qi, q + off, k + off, idesc_s, s > 0);
                 }
                 umma_commit(&s_ready[qi]);
             };
             const auto values = [&](int qi, int st, bool acc) {
-                const uint32_t v = base + S::kV + st * S::kTile;
+                uint32_t v = umma_desc_lo(base + S::kV + st * S::kTile, 16384), t = tmem;
+                asm volatile("" : "+r"(v), "+r"(t));
 #pragma unroll
                 for (int s = 0; s < kPKeys / 16; ++s)
-                    umma_ts(tmem + 256 + D * qi, tmem + 128 * qi + 8 * s, umma_desc_mn(v + 2048 * s, 16384), idesc_o, acc || s > 0);
+                    umma_ts(t + 256 + D * qi, t + 128 * qi + 8 * s, v + 128 * s, idesc_o, acc || s > 0);
             };
             bool ok = mbar_wait_or(q_full, 0, stop) && mbar_wait_or(&k_full[0], 0, stop);
             if (ok) {
@@ -410,6 +444,7 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
             }
             umma_commit(o_done);
             mbar_wait_or(o_done, 0, nullptr);  // nothing of this CTA is in flight when it frees its TMEM
+            }
         }
     } else if (warp < 8 && a.splits == 1) {
         // no query of the pair sees a key: zeros
@@ -424,7 +459,7 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (tid == 0 && *stop) report_device_error(T2C_ETIMEOUT);
-    if (warp == 12) {
+    if (warp == 16) {
         __syncwarp();
         tmem_free(tmem, 512);
     }

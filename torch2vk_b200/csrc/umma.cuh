@@ -6,37 +6,34 @@
 
 namespace t2c {
 
-// K-major operand, 128-byte swizzle: 8-row groups 1024 B apart.
-__device__ __forceinline__ uint64_t umma_desc_k(uint32_t saddr) {
-    return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(1u) << 16) |
-           (static_cast<uint64_t>(1024u >> 4) << 32) | (static_cast<uint64_t>(1u) << 46) | (static_cast<uint64_t>(2u) << 61);
+// Low word of the descriptor of a 128-byte-swizzled operand: its address and leading offset in 16-byte units.  Adding n
+// moves the start by 16 n bytes.  K-major operands ignore the leading offset (1); MN-major ones have their 64-value
+// atoms along MN `chunk` bytes apart.  The high word is the same for all: 8-row groups 1024 B apart.
+__device__ __forceinline__ uint32_t umma_desc_lo(uint32_t saddr, uint32_t chunk = 16) {
+    return ((saddr >> 4) & 0x3FFFu) | ((chunk >> 4) << 16);
 }
-
-// MN-major operand, 128-byte swizzle: 64-value atoms along MN `chunk` bytes apart (leading), 8-row K groups 1024 B
-// apart (stride).
-__device__ __forceinline__ uint64_t umma_desc_mn(uint32_t saddr, uint32_t chunk) {
-    return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(chunk >> 4) << 16) |
-           (static_cast<uint64_t>(1024u >> 4) << 32) | (static_cast<uint64_t>(1u) << 46) | (static_cast<uint64_t>(2u) << 61);
-}
+constexpr uint32_t kUmmaDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 
 // kind::f16, fp16 operands, fp32 accumulators, M x N; b_mn: B is MN-major.
 __device__ __forceinline__ uint32_t umma_idesc(int m, int n, bool b_mn) {
     return (1u << 4) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-// D[tmem] (+)= A B, both in shared memory.
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+// D[tmem] (+)= A B, both in shared memory (descriptors' low words).
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc ? 1u : 0u)
+        "{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %5, 0;\n mov.b64 x, {%1, %3};\n mov.b64 y, {%2, %3};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(kUmmaDescHi), "r"(idesc), "r"(acc ? 1u : 0u)
         : "memory");
 }
 
 // D[tmem] (+)= A B, A [128 lanes][two fp16 per column] in TMEM.
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc ? 1u : 0u)
+        "{\n .reg .pred p;\n .reg .b64 y;\n setp.ne.b32 p, %5, 0;\n mov.b64 y, {%2, %3};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(kUmmaDescHi), "r"(idesc), "r"(acc ? 1u : 0u)
         : "memory");
 }
 
