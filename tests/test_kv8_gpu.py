@@ -375,6 +375,27 @@ def test_attention_ignores_what_is_not_seen():
     assert torch.equal(out[1][:, keep], was[0][1][:, keep]) and torch.equal(out[0], was[0][0])
 
 
+def test_attention_rows_before_a_poisoned_block():
+    """A NaN block makes the rows that see it NaN, and no row before it."""
+    from torch2vk_b200 import kernels
+
+    NH, NK, dim, page, block = 8, 2, 64, 32, 16
+    cache, table, g, _ = attention_case(1, NH, NK, dim, page, block, 10, 65)
+    pages, bt = device_pages(cache), table.cuda()
+    T = 200
+    q = torch.randn(1, T, NH, dim, generator=g).half()
+    want = ref.attention(cache, q, [40], table, dim ** -0.5)
+    for scale in (pages.k_scale, pages.v_scale):
+        keep = scale.clone()
+        scale[bt[0, 144 // page].long(), :, 144 % page // block] = math.nan  # keys 144 .. 159, seen from query 104 on
+        out, lse = kernels.attn_prefill_q8(q.cuda(), pages, i32([40]), bt, return_lse=True)
+        clean()
+        assert bool(torch.isnan(out[:, 104:]).all())
+        part = {n: (x[:, :104] if n in ("out", "spread") else x[:, :, :104]) for n, x in want.items() if n != "probs"}
+        check_attention(out[:, :104], lse[:, :, :104], part)
+        scale.copy_(keep)
+
+
 def test_attention_reports_bad_entries_and_lengths():
     from torch2vk_b200 import kernels
 

@@ -7,13 +7,15 @@
 //   P_i = 2^(S_i kf_j + log2 vs_j - m)   fp16 over S_i's columns in TMEM (A operand of the next product)
 //   O_i += P_i V_j      N = D, K = 128 keys, V as an MN-major operand
 // Roles: warps 0-3 and 4-7 the softmax of the two query tiles (a thread one row), warps 8-15 expand the int8 codes
-// to fp16 operand tiles (loads a tile ahead in registers), warp 16 issues the MMAs.  The tensor core runs
-// P V and the next S of one query tile while the other tile's softmax runs.
+// to fp16 operand tiles (loads a tile ahead in registers), warp 16 issues the MMAs.
+//
+// The tensor core's work for one query tile runs under the other tile's softmax.
 //
 // Codes become fp16 exactly.  The scales stay in fp32 in the exponent: kf = k scale * softmax scale * log2 e; the V
 // scale joins as log2 vs, and the softmax sum takes P / vs.  One reference m per row serves all tiles until the P of
-// 16 keys sum to more than 2^14: then the row's m moves to its maximum - 8 and O, l are rescaled.  So no pass looks
-// for the maximum; P's rounding to fp16 (what the tensor core takes) is the only one before the output's.
+// 16 keys sum to more than 2^14: then the row's m moves to those keys' maximum - 8 (a whole number, so that rescaling
+// by 2^(old - new) is exact) and O, l and the tile's P are rescaled.  So no pass looks for the maximum; P's rounding
+// to fp16 (what the tensor core takes) is the only one before the output's.
 //
 // Within groups of four dims K and Q rows are held in the order 0, 2, 1, 3 (as the expansion leaves them; the product
 // does not see it), V's columns too, which the epilogue undoes.
@@ -29,14 +31,15 @@ constexpr int kPRows = 128;   // rows of a query tile
 constexpr int kPKeys = 128;   // keys of a tile
 constexpr int kPThreads = 640;
 constexpr float kPRefStart = -1e30f;
-constexpr float kPSumTop = 16384.0f;  // sum of 16 P that moves the reference
+constexpr float kPSumTop = 16384.0f;  // sum of 16 P that moves the reference; 16 P of 2^10 do not
+constexpr float kPRefMove = 10.0f;
 constexpr float kPRefDrop = 8.0f;
 
 template <int D>
 struct PrefillShape {
     static constexpr int kTile = 128 * D * 2;          // bytes of a 128-row fp16 tile: D / 64 chunks of 16 KB
     static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + 2 * kTile, kMeta = kV + 2 * kTile;
-    static constexpr int kBars = kMeta + 4 * 8 * 16;   // meta: ring of 4 tiles x 8 groups of 16 keys
+    static constexpr int kBars = kMeta + 4 * 8 * 20;   // meta: ring of 4 tiles x 8 groups of 16 keys
     static constexpr int kSmem = kBars + 256;
 };
 
@@ -93,7 +96,7 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return v;
 }
 
-// Registers of the roles, of the 640 x 96 the CTA has: 2 x 144 + 2 x 72 + 48 = 5 x 96.
+// Registers of the roles, of the 640 x 96 the CTA has: 2 x 136 + 2 x 72 + 64 = 5 x 96.
 template <int R>
 __device__ __forceinline__ void more_registers() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
@@ -108,24 +111,24 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
     using S = PrefillShape<D>;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = smem_u32(smem);
-    float4 *meta = reinterpret_cast<float4 *>(smem + S::kMeta);
+    // per group of 16 keys: (K factor twice, log2 V scale twice), and 1 / V scale
+    ulonglong2 *meta = reinterpret_cast<ulonglong2 *>(smem + S::kMeta);
+    float *inv_vs = reinterpret_cast<float *>(smem + S::kMeta + 4 * 8 * 16);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kBars);
     uint64_t *k_full = bars, *v_full = bars + 2, *k_free = bars + 4, *v_free = bars + 6, *s_ready = bars + 8,
-             *p_ready = bars + 10, *q_full = bars + 12, *o_done = bars + 13, *meta_full = bars + 14;
+             *o_done = bars + 10, *p_ready = bars + 11, *q_full = bars + 13, *meta_full = bars + 14;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 18);
-    volatile int *stop = reinterpret_cast<volatile int *>(bars + 19);
+    volatile int *stop = reinterpret_cast<volatile int *>(bars + 19), *stop_last = stop + 1;
     if (base & 1023u) {  // the swizzle atoms need it: report, compute nothing
         if (threadIdx.x == 0) report_device_error(T2C_EUNSUPPORTED);
         return;
     }
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
-        for (int i = 0; i < 4; ++i) mbar_init(bars + i, 8);         // k_full, v_full: the expanding warps
-        for (int i = 4; i < 10; ++i) mbar_init(bars + i, 1);        // commits
-        mbar_init(p_ready, 128);
-        mbar_init(p_ready + 1, 128);
+        for (int i = 0; i < 4; ++i) mbar_init(k_full + i, 8);  // k_full, v_full: the expanding warps
+        for (int i = 4; i < 11; ++i) mbar_init(bars + i, 1);   // commits
+        for (int i = 0; i < 2; ++i) mbar_init(p_ready + i, 4);
         mbar_init(q_full, 256);
-        mbar_init(o_done, 1);
         for (int i = 0; i < 4; ++i) mbar_init(meta_full + i, 8);
         *stop = 0;
         fence_mbar_init();
@@ -162,19 +165,31 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
     if (tiles > 0) {
         if (warp < 8) {
             // ================================================== softmax: tile `qi`, row `row`
-            more_registers<144>();
+            more_registers<136>();
             const int qi = warp >> 2, row = tid & 127;
             const int t = t_first + qi * TT + row / group, h = head * group + row % group;
             const bool real = row < TT * group && t < a.T;
-            {
-                const __half *q = a.q + b * a.q_sb + static_cast<int64_t>(t) * a.q_st + h * a.q_sh;
+            {   // a warp its 32 rows, neighbouring lanes neighbouring units of a row, eight loads in flight
+                constexpr int kUnits = D / 8, kRowsPer = 32 / kUnits;
                 const uint32_t at = base + S::kQ + qi * S::kTile;
+                const int u = lane % kUnits;
+#pragma unroll 1
+                for (int i0 = 0; i0 < 32 / kRowsPer; i0 += 8) {
+                    uint4 v[8];
 #pragma unroll
-                for (int u = 0; u < D / 8; ++u) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (real) v = ldg_nc_v4(q + 8 * u);
-                    sts128(at + unit_at(row, u), __byte_perm(v.x, v.y, 0x5410), __byte_perm(v.x, v.y, 0x7632),
-                           __byte_perm(v.z, v.w, 0x5410), __byte_perm(v.z, v.w, 0x7632));
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = 32 * (warp & 3) + (i0 + i) * kRowsPer + lane / kUnits;
+                        const int tr = t_first + qi * TT + r / group, hr = head * group + r % group;
+                        v[i] = make_uint4(0, 0, 0, 0);
+                        if (r < TT * group && tr < a.T)
+                            v[i] = *reinterpret_cast<const uint4 *>(a.q + b * a.q_sb + static_cast<int64_t>(tr) * a.q_st + hr * a.q_sh + 8 * u);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = 32 * (warp & 3) + (i0 + i) * kRowsPer + lane / kUnits;
+                        sts128(at + unit_at(r, u), __byte_perm(v[i].x, v[i].y, 0x5410), __byte_perm(v[i].x, v[i].y, 0x7632),
+                               __byte_perm(v[i].z, v[i].w, 0x5410), __byte_perm(v[i].z, v[i].w, 0x7632));
+                    }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(q_full);
@@ -185,96 +200,156 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
             const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
             const uint32_t s_at = lanes + 128 * qi, o_at = lanes + 256 + D * qi;
             float m = kPRefStart, l = 0.0f;
-            bool ok = true;
             for (int j = 0; j < tiles; ++j) {
-                ok = mbar_wait_or(&s_ready[qi], j & 1, stop);
-                if (!__all_sync(0xffffffffu, ok)) break;
-                mbar_wait_or(&meta_full[j & 3], (j >> 2) & 1, stop);  // complete: S was made after it
+                mbar_wait_or(&meta_full[j & 3], (j >> 2) & 1, stop);
+                const ulonglong2 *f = meta + (j & 3) * 8;
+                const float *fi = inv_vs + (j & 3) * 8;
+                // the factors come to registers before S is there: shared memory is slow to answer under the MMAs' reads
+                float kf[8], lv[8], iv[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const float4 x = reinterpret_cast<const float4 *>(f)[c];
+                    kf[c] = x.x, lv[c] = x.z, iv[c] = fi[c];
+                }
+                mbar_wait_or(&s_ready[qi], j & 1, stop);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const int64_t k0 = static_cast<int64_t>(tile0 + j) * kPKeys;
                 const bool masked = k0 + kPKeys - 1 > least;
+
+                // 32 keys at a time, three stages deep: exponents of chunk r (its S loaded before), 2^, sums and fp16 of
+                // chunk r - 1, check and store of chunk r - 2.  P of chunk c goes over S columns 16 c .. 16 c + 15, all
+                // read by then.  Returns the group of 16 keys from which another reference is needed, or 8.
                 const int last = static_cast<int>(max(min(limit - k0, static_cast<int64_t>(kPKeys)), static_cast<int64_t>(-1)));
-                const float4 *f = meta + (j & 3) * 8;
-                uint32_t p[kPKeys / 2];
-                float lt;
-                bool high;
-                const auto exponents = [&](auto hide) {
-                    lt = 0.0f;
-                    high = false;
-                    uint32_t s[2][16];
-                    tmem_ld16(s_at, s[0]);
+                const auto fast = [&](auto hide) -> int {
+                    uint32_t s[32], p[2][16];
+                    uint64_t y[2][16];
+                    float total[2][2];
+                    tmem_ld32(s_at, s);
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        tmem_ld_wait();
-                        if (c < 7) tmem_ld16(s_at + 16 * (c + 1), s[(c + 1) & 1]);
-                        const float4 k = f[c];
-                        const uint64_t kk = pair2(k.x, k.x), shift = pair2(k.y - m, k.y - m);
-                        uint64_t sum[2];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const uint32_t *x = s[c & 1] + 2 * i;
-                            float2 y = unpair2(fma2(pair2(__uint_as_float(x[0]), __uint_as_float(x[1])), kk, shift));
-                            if (hide) {
-                                const int at = 16 * c + 2 * i;
-                                y.x = at > last ? -INFINITY : y.x;
-                                y.y = at + 1 > last ? -INFINITY : y.y;
+                    for (int r = 0; r < 6; ++r) {
+                        if (r >= 2) {
+                            const int c = r - 2;
+                            if (__any_sync(0xffffffffu, fmaxf(total[c & 1][0], total[c & 1][1]) > kPSumTop)) {
+                                tmem_ld_wait();  // the load ahead
+                                return 2 * c;
                             }
-                            y.x = p_exp2(y.x);
-                            y.y = p_exp2(y.y);
-                            sum[i & 1] = i < 2 ? pair2(y.x, y.y) : add2(sum[i & 1], pair2(y.x, y.y));
-                            p[8 * c + i] = ph_bits(__floats2half2_rn(y.x, y.y));
+                            if (!hide || 32 * c <= last) l = fmaf(total[c & 1][0], iv[2 * c], l);  // an unseen block may have any scale
+                            if (!hide || 32 * c + 16 <= last) l = fmaf(total[c & 1][1], iv[2 * c + 1], l);
+                            tmem_st16(s_at + 16 * c, p[c & 1]);
                         }
-                        const float2 both = unpair2(add2(sum[0], sum[1]));
-                        const float total = both.x + both.y;
-                        high |= total > kPSumTop;
-                        lt = fmaf(total, k.z, lt);
+                        if (r < 4) {
+                            tmem_ld_wait32(s);
+                            const uint64_t k0 = pair2(kf[2 * r], kf[2 * r]), k1 = pair2(kf[2 * r + 1], kf[2 * r + 1]);
+                            const float h0 = lv[2 * r] - m, h1 = lv[2 * r + 1] - m;
+                            const uint64_t shift0 = pair2(h0, h0), shift1 = pair2(h1, h1);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                y[r & 1][i] = fma2(pair2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), i < 8 ? k0 : k1,
+                                                   i < 8 ? shift0 : shift1);
+                                if (hide) {
+                                    const float2 v = unpair2(y[r & 1][i]);
+                                    y[r & 1][i] = pair2(32 * r + 2 * i > last ? -INFINITY : v.x, 32 * r + 2 * i + 1 > last ? -INFINITY : v.y);
+                                }
+                            }
+                            if (r < 3) tmem_ld32(s_at + 32 * (r + 1), s);
+                        }
+                        if (r >= 1 && r < 5) {
+                            const int c = (r - 1) & 1;
+                            uint64_t sum[4];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const float2 v = unpair2(y[c][i]);
+                                const float e0 = p_exp2(v.x), e1 = p_exp2(v.y);
+                                const int k = (i >> 3) * 2 + (i & 1);
+                                sum[k] = (i & 7) < 2 ? pair2(e0, e1) : add2(sum[k], pair2(e0, e1));
+                                p[c][i] = ph_bits(__floats2half2_rn(e0, e1));
+                            }
+                            const float2 t0 = unpair2(add2(sum[0], sum[1])), t1 = unpair2(add2(sum[2], sum[3]));
+                            total[c][0] = t0.x + t0.y;
+                            total[c][1] = t1.x + t1.y;
+                        }
                     }
+                    return 8;
                 };
-                for (int pass = 0;; ++pass) {
-                    if (masked)
-                        exponents(std::true_type{});
-                    else
-                        exponents(std::false_type{});
-                    if (pass > 0 || !__any_sync(0xffffffffu, high)) break;
-                    // ---- rare: the reference of the rows that ask for it moves to their maximum - 8
+                // Moves the reference of the rows that need it to the maximum of groups c0 .. 7, a whole number - 8 on; O, l and
+                // the P of this tile so far are rescaled.  In the first tile of a CTA, and rarely after it.
+                const auto move_reference = [&](int c0) {
                     float top = -INFINITY;
 #pragma unroll 1
-                    for (int c = 0; c < 8; ++c) {
+                    for (int c = c0; c < 8; ++c) {
                         uint32_t v[16];
                         tmem_ld16(s_at + 16 * c, v);
-                        tmem_ld_wait();
-                        const float4 k = f[c];
+                        const float kf = unpair2(f[c].x).x, lv = unpair2(f[c].y).x;
+                        tmem_ld_wait16(v);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const float x = fmaf(__uint_as_float(v[i]), k.x, k.y);
-                            if (!masked || 16 * c + i <= last) top = fmaxf(top, x);
+                            const float x = fmaf(__uint_as_float(v[i]), kf, lv);
+                            top = fmaxf(top, 16 * c + i > last ? -INFINITY : x);
                         }
                     }
-                    const float ref = high ? top - kPRefDrop : m;
+                    const float ref = top - m > kPRefMove ? floorf(top) - kPRefDrop : m;
                     const float corr = p_exp2(m - ref);
                     m = ref;
                     l *= corr;
-                    if (j > 0) {  // S being ready says that P V of the tile before is too
+                    if (j > 0) {  // S being ready says that the tiles before are in O
 #pragma unroll 1
-                        for (int c = 0; c < D / 16; ++c) {
-                            uint32_t v[16];
-                            tmem_ld16(o_at + 16 * c, v);
-                            tmem_ld_wait();
+                        for (int i = 0; i < D / 16; ++i) {
+                            uint32_t w[16];
+                            tmem_ld16(o_at + 16 * i, w);
+                            tmem_ld_wait16(w);
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
-                            tmem_st16(o_at + 16 * c, v);
+                            for (int k = 0; k < 16; ++k) w[k] = __float_as_uint(__uint_as_float(w[k]) * corr);
+                            tmem_st16(o_at + 16 * i, w);
                         }
                     }
+                    if (c0 > 0) tmem_st_wait();  // P is read back
+#pragma unroll 1
+                    for (int i = 0; i < c0; ++i) {
+                        uint32_t w[8];
+                        tmem_ld8(s_at + 8 * i, w);
+                        tmem_ld_wait8(w);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {  // in fp32: corr may be below fp16's least number
+                            const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
+                            w[k] = ph_bits(__floats2half2_rn(x.x * corr, x.y * corr));
+                        }
+                        tmem_st8(s_at + 8 * i, w);
+                    }
+                };
+                // Groups c0 .. 7 after the reference moved.
+                const auto rest = [&](int c0) {
+#pragma unroll 1
+                    for (int c = c0; c < 8; ++c) {
+                        uint32_t v[16], p[8];
+                        tmem_ld16(s_at + 16 * c, v);
+                        const float kf = unpair2(f[c].x).x, shift = unpair2(f[c].y).x - m;
+                        tmem_ld_wait16(v);
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            float a0 = p_exp2(fmaf(__uint_as_float(v[2 * i]), kf, shift)), a1 = p_exp2(fmaf(__uint_as_float(v[2 * i + 1]), kf, shift));
+                            a0 = 16 * c + 2 * i > last ? 0.0f : a0;
+                            a1 = 16 * c + 2 * i + 1 > last ? 0.0f : a1;
+                            sum += a0 + a1;
+                            p[i] = ph_bits(__floats2half2_rn(a0, a1));
+                        }
+                        if (16 * c <= last) l = fmaf(sum, fi[c], l);
+                        tmem_st8(s_at + 8 * c, p);
+                    }
+                };
+                if (j == 0) move_reference(0);
+                const int done = masked ? fast(std::true_type{}) : fast(std::false_type{});
+                if (done < 8) {
+                    move_reference(done);
+                    rest(done);
                 }
-                l += lt;
-                tmem_st32(s_at, p);
-                tmem_st32(s_at + 32, p + 32);
                 tmem_st_wait();
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                mbar_arrive(&p_ready[qi]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_ready[qi]);
             }
-            ok = mbar_wait_or(o_done, 0, stop);
-            if (__all_sync(0xffffffffu, ok)) {
+            mbar_wait_or(o_done, 0, stop);
+            if (!*stop) {
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const bool seen = limit >= 0;
                 if (a.splits > 1) {
@@ -285,7 +360,7 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                     for (int c = 0; c < D / 16; ++c) {
                         uint32_t v[16];
                         tmem_ld16(o_at + 16 * c, v);
-                        tmem_ld_wait();
+                        tmem_ld_wait16(v);
                         if (real) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
@@ -301,7 +376,7 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                     for (int c = 0; c < D / 16; ++c) {
                         uint32_t v[16];
                         tmem_ld16(o_at + 16 * c, v);
-                        tmem_ld_wait();
+                        tmem_ld_wait16(v);
                         float x[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) x[i] = seen ? __uint_as_float(v[i]) * inv : 0.0f;
@@ -363,34 +438,41 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                 }
             };
             uint4 kx[kPasses], vx[kPasses];
-            int page = look(key);
+            // pages are looked up two tiles ahead, scales and codes one
+            int page = look(key), ahead = look(key + kPKeys);
             fetch(a.pg.k, key, page, kx);
             fetch(a.pg.v, key, page, vx);
+            __half ks, vs;
+            const auto scales = [&](int64_t k, int pg) {
+                const int64_t so = k < n ? kv8_scale_offset(a.pg, pg, head, k) : 0;
+                ks = a.pg.ks[so];
+                vs = a.pg.vs[so];
+            };
+            scales(key, page);
             for (int j = 0; j < tiles; ++j) {
                 const int st = j & 1;
                 if (lane == 0) {  // the factors of these 16 keys (the ring of 4 outlives their readers)
-                    float4 f = make_float4(0.0f, -24.0f, 0.0f, 0.0f);
-                    if (key < n) {
-                        const int64_t so = kv8_scale_offset(a.pg, page, head, key);
-                        const float vs = __half2float(a.pg.vs[so]);
-                        // a block of scale 0 has values 0: the least scale's exponent moves no reference
-                        f = make_float4(__half2float(a.pg.ks[so]) * a.scale_log2, vs == 0.0f ? -24.0f : log2f(vs),
-                                        vs == 0.0f ? 16777216.0f : 1.0f / vs, 0.0f);
-                    }
-                    meta[(j & 3) * 8 + slice] = f;
+                    // a block of scale 0 has values 0: the least scale's exponent moves no reference
+                    const bool some = key < n;
+                    const float v = some ? __half2float(vs) : 0.0f, kf = some ? __half2float(ks) * a.scale_log2 : 0.0f;
+                    const float lv = v == 0.0f ? -24.0f : log2f(v);
+                    meta[(j & 3) * 8 + slice] = make_ulonglong2(pair2(kf, kf), pair2(lv, lv));
+                    inv_vs[(j & 3) * 8 + slice] = v == 0.0f ? 16777216.0f : 1.0f / v;
                     mbar_arrive(&meta_full[j & 3]);
                 }
                 key += kPKeys;
-                if (j + 1 < tiles) page = look(key);
-                bool ok = j < 2 || mbar_wait_or(&k_free[st], ((j >> 1) - 1) & 1, stop);
-                if (!__all_sync(0xffffffffu, ok)) break;
+                page = ahead;
+                if (j + 1 < tiles) {
+                    scales(key, page);
+                    ahead = look(key + kPKeys);
+                }
+                if (j >= 2) mbar_wait_or(&k_free[st], ((j >> 1) - 1) & 1, stop);
                 expand(base + S::kK + st * S::kTile, kx);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&k_full[st]);
                 if (j + 1 < tiles) fetch(a.pg.k, key, page, kx);
-                ok = j < 2 || mbar_wait_or(&v_free[st], ((j >> 1) - 1) & 1, stop);
-                if (!__all_sync(0xffffffffu, ok)) break;
+                if (j >= 2) mbar_wait_or(&v_free[st], ((j >> 1) - 1) & 1, stop);
                 expand(base + S::kV + st * S::kTile, vx);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -398,52 +480,60 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                 if (j + 1 < tiles) fetch(a.pg.v, key, page, vx);
             }
         } else {
-            fewer_registers<48>();
-            if (warp == 16 && lane == 0) {
-            // ================================================== MMA
-            const uint32_t idesc_s = umma_idesc(128, 128, false), idesc_o = umma_idesc(128, D, true);
-            const auto scores = [&](int qi, int st) {
-                uint32_t q = umma_desc_lo(base + S::kQ + qi * S::kTile), k = umma_desc_lo(base + S::kK + st * S::kTile);
-                asm volatile("" : "+r"(q), "+r"(k));  // the sums below are made here, not kept in registers across tiles
+            fewer_registers<64>();
+            if (warp == 16) {
+                // ============================================== MMA: the warp waits together, one lane issues.  What the
+                // instructions take is made warp-uniform by reductions, so that it lives in uniform registers.
+                const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
+                const int nt = __reduce_max_sync(0xffffffffu, tiles);
+                const uint32_t idesc_s = umma_idesc(128, 128, false), idesc_o = umma_idesc(128, D, true);
+                const auto scores = [&](int qi, int st) {
+                    const uint32_t q = umma_desc_lo(base + S::kQ + qi * S::kTile);
+                    const uint32_t k = umma_desc_lo(base + S::kK + st * S::kTile);
 #pragma unroll
-                for (int s = 0; s < D / 16; ++s) {
-                    const uint32_t off = static_cast<uint32_t>((s >> 2) * 1024 + 2 * (s & 3));  // 16-byte units
-                    umma_ss(tmem + 128 * qi, q + off, k + off, idesc_s, s > 0);
-                }
-                umma_commit(&s_ready[qi]);
-            };
-            const auto values = [&](int qi, int st, bool acc) {
-                uint32_t v = umma_desc_lo(base + S::kV + st * S::kTile, 16384), t = tmem;
-                asm volatile("" : "+r"(v), "+r"(t));
+                    for (int s = 0; s < D / 16; ++s) {
+                        const uint32_t off = static_cast<uint32_t>((s >> 2) * 1024 + 2 * (s & 3));  // 16-byte units
+                        umma_ss(tm + 128 * qi, q + off, k + off, idesc_s, s > 0);
+                    }
+                    umma_commit(&s_ready[qi]);
+                };
+                const auto values = [&](int qi, int st, bool acc) {
+                    const uint32_t v = umma_desc_lo(base + S::kV + st * S::kTile, 16384);
 #pragma unroll
-                for (int s = 0; s < kPKeys / 16; ++s)
-                    umma_ts(t + 256 + D * qi, t + 128 * qi + 8 * s, v + 128 * s, idesc_o, acc || s > 0);
-            };
-            bool ok = mbar_wait_or(q_full, 0, stop) && mbar_wait_or(&k_full[0], 0, stop);
-            if (ok) {
+                    for (int s = 0; s < 8; ++s)
+                        umma_ts(tm + 256 + D * qi, tm + 128 * qi + 8 * s, v + 128 * s, idesc_o, acc || s > 0);
+                };
+                mbar_wait_or(q_full, 0, stop);
+                mbar_wait_or(&k_full[0], 0, stop);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                scores(0, 0);
-                scores(1, 0);
-                umma_commit(&k_free[0]);
-            }
-            for (int j = 0; j < tiles && ok; ++j) {
-                const int st = j & 1, next = st ^ 1;
-                const bool more = j + 1 < tiles;
-                ok = mbar_wait_or(&v_full[st], (j >> 1) & 1, stop) &&
-                     (!more || mbar_wait_or(&k_full[next], ((j + 1) >> 1) & 1, stop));
-#pragma unroll
-                for (int qi = 0; qi < 2; ++qi) {
-                    ok = ok && mbar_wait_or(&p_ready[qi], j & 1, stop);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    values(qi, st, j > 0);
-                    if (qi == 1) umma_commit(&v_free[st]);
-                    if (more) scores(qi, next);
+                if (elect_one()) {
+                    scores(0, 0);
+                    scores(1, 0);
+                    umma_commit(&k_free[0]);
                 }
-                if (ok && more) umma_commit(&k_free[next]);
-            }
-            umma_commit(o_done);
-            mbar_wait_or(o_done, 0, nullptr);  // nothing of this CTA is in flight when it frees its TMEM
+                __syncwarp();
+                for (int j = 0; j < nt; ++j) {
+                    const int st = j & 1, next = st ^ 1;
+                    const bool more = j + 1 < nt;
+                    mbar_wait_or(&v_full[st], (j >> 1) & 1, stop);
+                    if (more) mbar_wait_or(&k_full[next], ((j + 1) >> 1) & 1, stop);
+#pragma unroll
+                    for (int qi = 0; qi < 2; ++qi) {
+                        mbar_wait_or(&p_ready[qi], j & 1, stop);
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (elect_one()) {
+                            values(qi, st, j > 0);
+                            if (qi == 1) umma_commit(&v_free[st]);
+                            if (more) scores(qi, next);
+                            if (more && qi == 1) umma_commit(&k_free[next]);
+                        }
+                        __syncwarp();
+                    }
+                }
+                if (elect_one()) umma_commit(o_done);
+                __syncwarp();
+                *stop_last = 0;
+                mbar_wait_or(o_done, 0, stop_last);  // nothing of this CTA is in flight when it frees its TMEM
             }
         }
     } else if (warp < 8 && a.splits == 1) {
