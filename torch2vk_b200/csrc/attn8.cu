@@ -1,5 +1,4 @@
-// Attention over the paged KV cache in 8 bits: one warp per query row, one
-// lane per key for the scores, lanes across head_dim for the values.
+// Attention of single tokens over the paged KV cache in 8 bits.
 #include <cooperative_groups.h>
 #include <cudaTypedefs.h>
 
@@ -31,56 +30,6 @@ __device__ __forceinline__ int64_t visible(const int32_t *positions, int b, int 
         return max_len;
     }
     return n < 0 ? 0 : n;
-}
-
-__device__ __forceinline__ float dot_row(const int8_t *row, const float *q, int D) {
-    float acc = 0.0f;
-    for (int i = 0; i < D; i += 16) {
-        const uint4 c = *reinterpret_cast<const uint4 *>(row + i);
-        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc = fmaf(static_cast<float>(static_cast<int8_t>(w[j] >> (8 * e))), q[i + 4 * j + e], acc);
-    }
-    return acc;
-}
-
-// One warp per (sequence, KV head, 32 keys): a lane's key against every query that sees it.
-template <int D>
-__global__ void __launch_bounds__(32) attn8_weights_kernel(AttnArgs a, const float *lse, const float *w_in, float *w_out,
-                                                           int64_t w_sb, int64_t w_sh) {
-    __shared__ float qs[D];
-    const int lane = threadIdx.x;
-    const int head = blockIdx.y, b = blockIdx.z;
-    pdl_wait();
-    pdl_trigger();
-    const int64_t first = a.positions[b];
-    const int64_t n = visible(a.positions, b, a.T - 1, a.max_len);
-    const int64_t key = static_cast<int64_t>(blockIdx.x) * 32 + lane;
-    if (key - lane >= n) return;
-    const int64_t at = key < n ? key : n - 1;
-    int page = kv8_page(a.pg, a.table + b * a.t_stride, at);
-    if (page < 0) page = 0;
-    const int8_t *row = a.pg.k + kv8_row_offset(a.pg, page, head, at);
-    const float s = __half2float(a.pg.ks[kv8_scale_offset(a.pg, page, head, at)]) * a.scale_log2;
-    const int group = a.NH / a.pg.n_kv;
-    float sum = 0.0f;
-    for (int t = 0; t < a.T; ++t) {
-        if (first + t < key - lane) continue;
-        for (int g = 0; g < group; ++g) {
-            const int h = head * group + g;
-            __syncwarp();
-            for (int i = lane; i < D; i += 32) qs[i] = __half2float(a.q[b * a.q_sb + t * a.q_st + h * a.q_sh + i]);
-            __syncwarp();
-            const float x = dot_row(row, qs, D) * s;
-            if (key <= first + t)
-                sum += exp2f(x - lse[(static_cast<int64_t>(b) * a.NH + h) * a.T + t] * 1.4426950408889634f);
-        }
-    }
-    if (key >= n) return;
-    const int64_t o = b * w_sb + head * w_sh + key;
-    w_out[o] = sum + (w_in && key < first ? w_in[o] : 0.0f);
 }
 
 // ------------------------------------------------------------------ one token per sequence
@@ -664,13 +613,6 @@ __global__ void __launch_bounds__(kJoinThreads) attn8_join_kernel(const __grid_c
     }
 }
 
-int launch_weights(const AttnArgs &a, const float *lse, const float *weights, float *weights_out, int64_t w_sb,
-                   int64_t w_sh, int64_t D, cudaStream_t s) {
-    const dim3 grid(static_cast<unsigned>((a.max_len + 31) / 32), static_cast<unsigned>(a.pg.n_kv), static_cast<unsigned>(a.B));
-    return kv8_launch("attn_key_weights_q8", D == 128 ? attn8_weights_kernel<128> : attn8_weights_kernel<64>, grid, dim3(32), 0,
-                      1, s, a, lse, weights, weights_out, w_sb, w_sh);
-}
-
 struct DecodePlan {
     int splits, head_chunks, ctas;
     int64_t part_floats, unit_floats, lse_floats, floats;
@@ -766,21 +708,4 @@ extern "C" int t2c_attn_decode_q8(const t2c_q8_pages *pages, const void *q, int6
     return kv8_launch("attn_decode_q8 join", D == 128 ? attn8_join_kernel<128> : attn8_join_kernel<64>,
                       dim3(static_cast<unsigned>(group + chunks), static_cast<unsigned>(a.pg.n_kv), static_cast<unsigned>(B)),
                       dim3(kJoinThreads), static_cast<size_t>(p.ctas * 4), 1, s, p);
-}
-
-extern "C" int t2c_attn_key_weights_q8(const t2c_q8_pages *pages, const void *q, int64_t q_sb, int64_t q_st,
-                                       int64_t q_sh, const float *lse, const int32_t *positions,
-                                       const int32_t *block_table, int64_t bt_stride, int64_t bt_width, int64_t B,
-                                       int64_t T, int64_t NH, float scale, int64_t max_len, const float *weights,
-                                       float *weights_out, int64_t w_sb, int64_t w_sh, void *stream) {
-    AttnArgs a = {};
-    int rc = kv8_attn_check(pages, "attn_key_weights_q8", a.pg, block_table, bt_stride, bt_width, positions, B, T, NH, max_len);
-    if (rc != T2C_OK) return rc;
-    if (!kv8_strides(q, q_sb, q_st, q_sh)) return set_error(T2C_EINVAL, "attn_key_weights_q8: q rows must be 16-byte aligned");
-    if (!lse || !weights_out) return set_error(T2C_EINVAL, "attn_key_weights_q8: NULL pointer");
-    a.q = static_cast<const __half *>(q), a.q_sb = q_sb, a.q_st = q_st, a.q_sh = q_sh;
-    a.positions = positions, a.table = block_table, a.t_stride = bt_stride, a.max_len = max_len;
-    a.B = static_cast<int>(B), a.T = static_cast<int>(T), a.NH = static_cast<int>(NH);
-    a.scale_log2 = scale * 1.4426950408889634f;
-    return launch_weights(a, lse, weights, weights_out, w_sb, w_sh, pages->head_dim, as_stream(stream));
 }

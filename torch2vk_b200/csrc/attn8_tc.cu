@@ -68,34 +68,6 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-__device__ __forceinline__ float p_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Two fp32 values in a register pair, and the packed operations on them.
-__device__ __forceinline__ uint64_t pair2(float x, float y) {
-    uint64_t v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
-    return v;
-}
-__device__ __forceinline__ float2 unpair2(uint64_t v) {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-    return f;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t v;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
-    return v;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t v;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-    return v;
-}
-
 // Registers of the roles, of the 640 x 96 the CTA has: 2 x 136 + 2 x 72 + 64 = 5 x 96.
 template <int R>
 __device__ __forceinline__ void more_registers() {
@@ -239,16 +211,16 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                         }
                         if (r < 4) {
                             tmem_ld_wait32(s);
-                            const uint64_t k0 = pair2(kf[2 * r], kf[2 * r]), k1 = pair2(kf[2 * r + 1], kf[2 * r + 1]);
+                            const uint64_t k0 = f32x2(kf[2 * r], kf[2 * r]), k1 = f32x2(kf[2 * r + 1], kf[2 * r + 1]);
                             const float h0 = lv[2 * r] - m, h1 = lv[2 * r + 1] - m;
-                            const uint64_t shift0 = pair2(h0, h0), shift1 = pair2(h1, h1);
+                            const uint64_t shift0 = f32x2(h0, h0), shift1 = f32x2(h1, h1);
 #pragma unroll
                             for (int i = 0; i < 16; ++i) {
-                                y[r & 1][i] = fma2(pair2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), i < 8 ? k0 : k1,
+                                y[r & 1][i] = f32x2_fma(f32x2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), i < 8 ? k0 : k1,
                                                    i < 8 ? shift0 : shift1);
                                 if (hide) {
-                                    const float2 v = unpair2(y[r & 1][i]);
-                                    y[r & 1][i] = pair2(32 * r + 2 * i > last ? -INFINITY : v.x, 32 * r + 2 * i + 1 > last ? -INFINITY : v.y);
+                                    const float2 v = f32x2_parts(y[r & 1][i]);
+                                    y[r & 1][i] = f32x2(32 * r + 2 * i > last ? -INFINITY : v.x, 32 * r + 2 * i + 1 > last ? -INFINITY : v.y);
                                 }
                             }
                             if (r < 3) tmem_ld32(s_at + 32 * (r + 1), s);
@@ -258,13 +230,13 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                             uint64_t sum[4];
 #pragma unroll
                             for (int i = 0; i < 16; ++i) {
-                                const float2 v = unpair2(y[c][i]);
-                                const float e0 = p_exp2(v.x), e1 = p_exp2(v.y);
+                                const float2 v = f32x2_parts(y[c][i]);
+                                const float e0 = ex2(v.x), e1 = ex2(v.y);
                                 const int k = (i >> 3) * 2 + (i & 1);
-                                sum[k] = (i & 7) < 2 ? pair2(e0, e1) : add2(sum[k], pair2(e0, e1));
+                                sum[k] = (i & 7) < 2 ? f32x2(e0, e1) : f32x2_add(sum[k], f32x2(e0, e1));
                                 p[c][i] = ph_bits(__floats2half2_rn(e0, e1));
                             }
-                            const float2 t0 = unpair2(add2(sum[0], sum[1])), t1 = unpair2(add2(sum[2], sum[3]));
+                            const float2 t0 = f32x2_parts(f32x2_add(sum[0], sum[1])), t1 = f32x2_parts(f32x2_add(sum[2], sum[3]));
                             total[c][0] = t0.x + t0.y;
                             total[c][1] = t1.x + t1.y;
                         }
@@ -279,7 +251,7 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                     for (int c = c0; c < 8; ++c) {
                         uint32_t v[16];
                         tmem_ld16(s_at + 16 * c, v);
-                        const float kf = unpair2(f[c].x).x, lv = unpair2(f[c].y).x;
+                        const float kf = f32x2_parts(f[c].x).x, lv = f32x2_parts(f[c].y).x;
                         tmem_ld_wait16(v);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
@@ -288,7 +260,7 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                         }
                     }
                     const float ref = top - m > kPRefMove ? floorf(top) - kPRefDrop : m;
-                    const float corr = p_exp2(m - ref);
+                    const float corr = ex2(m - ref);
                     m = ref;
                     l *= corr;
                     if (j > 0) {  // S being ready says that the tiles before are in O
@@ -322,12 +294,12 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                     for (int c = c0; c < 8; ++c) {
                         uint32_t v[16], p[8];
                         tmem_ld16(s_at + 16 * c, v);
-                        const float kf = unpair2(f[c].x).x, shift = unpair2(f[c].y).x - m;
+                        const float kf = f32x2_parts(f[c].x).x, shift = f32x2_parts(f[c].y).x - m;
                         tmem_ld_wait16(v);
                         float sum = 0.0f;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            float a0 = p_exp2(fmaf(__uint_as_float(v[2 * i]), kf, shift)), a1 = p_exp2(fmaf(__uint_as_float(v[2 * i + 1]), kf, shift));
+                            float a0 = ex2(fmaf(__uint_as_float(v[2 * i]), kf, shift)), a1 = ex2(fmaf(__uint_as_float(v[2 * i + 1]), kf, shift));
                             a0 = 16 * c + 2 * i > last ? 0.0f : a0;
                             a1 = 16 * c + 2 * i + 1 > last ? 0.0f : a1;
                             sum += a0 + a1;
@@ -349,7 +321,7 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                 if (lane == 0) mbar_arrive(&p_ready[qi]);
             }
             mbar_wait_or(o_done, 0, stop);
-            if (!*stop) {
+            if (!__any_sync(0xffffffffu, *stop != 0)) {
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const bool seen = limit >= 0;
                 if (a.splits > 1) {
@@ -456,7 +428,7 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                     const bool some = key < n;
                     const float v = some ? __half2float(vs) : 0.0f, kf = some ? __half2float(ks) * a.scale_log2 : 0.0f;
                     const float lv = v == 0.0f ? -24.0f : log2f(v);
-                    meta[(j & 3) * 8 + slice] = make_ulonglong2(pair2(kf, kf), pair2(lv, lv));
+                    meta[(j & 3) * 8 + slice] = make_ulonglong2(f32x2(kf, kf), f32x2(lv, lv));
                     inv_vs[(j & 3) * 8 + slice] = v == 0.0f ? 16777216.0f : 1.0f / v;
                     mbar_arrive(&meta_full[j & 3]);
                 }
@@ -580,7 +552,7 @@ __global__ void __launch_bounds__(256) attn8_prefill_join_kernel(const __grid_co
 #pragma unroll 4
     for (int s = 0; s < used; ++s) {
         const float *part = base + static_cast<int64_t>(s) * 256 * (D + 2);
-        const float f = p_exp2(part[256 * D + row] - top);
+        const float f = ex2(part[256 * D + row] - top);
         sum = fmaf(part[256 * (D + 1) + row], f, sum);
         const float *o = part + row * D + kPer * lane;
 #pragma unroll

@@ -17,6 +17,7 @@ cudaError_t status_attn_tc(unsigned int *bits, int clear, cudaStream_t s);
 cudaError_t status_kv8(unsigned int *bits, int clear, cudaStream_t s);
 cudaError_t status_attn8(unsigned int *bits, int clear, cudaStream_t s);
 cudaError_t status_attn8_tc(unsigned int *bits, int clear, cudaStream_t s);
+cudaError_t status_attn8_kw(unsigned int *bits, int clear, cudaStream_t s);
 
 static thread_local char g_last_error[1024] = "";
 
@@ -75,6 +76,7 @@ extern "C" int t2c_device_status(unsigned int *bits, int clear, void *stream) {
     if (err == cudaSuccess) err = t2c::status_kv8(&value, clear, s);
     if (err == cudaSuccess) err = t2c::status_attn8(&value, clear, s);
     if (err == cudaSuccess) err = t2c::status_attn8_tc(&value, clear, s);
+    if (err == cudaSuccess) err = t2c::status_attn8_kw(&value, clear, s);
     if (err != cudaSuccess) return t2c::set_error(T2C_ECUDA, "t2c_device_status: %s", cudaGetErrorString(err));
     *bits = value;
     return T2C_OK;

@@ -64,7 +64,7 @@ int kv8_attn_check(const t2c_q8_pages *pages, const char *what, KvPages &pg, con
     return T2C_OK;
 }
 
-bool kv8_maps(const t2c_q8_pages *p, int rows, CUtensorMap &k_map, CUtensorMap &v_map) {
+PFN_cuTensorMapEncodeTiled kv8_encoder() {
     static PFN_cuTensorMapEncodeTiled encode = [] {
         void *fn = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -73,6 +73,11 @@ bool kv8_maps(const t2c_q8_pages *p, int rows, CUtensorMap &k_map, CUtensorMap &
             fn = nullptr;
         return reinterpret_cast<PFN_cuTensorMapEncodeTiled>(fn);
     }();
+    return encode;
+}
+
+bool kv8_maps(const t2c_q8_pages *p, int rows, CUtensorMap &k_map, CUtensorMap &v_map) {
+    const auto encode = kv8_encoder();
     if (!encode) return false;
     const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p->head_dim), static_cast<cuuint64_t>(p->page_size),
                                 static_cast<cuuint64_t>(p->n_kv), static_cast<cuuint64_t>(p->num_pages)};

@@ -32,6 +32,9 @@ int kv8_table(const t2c_q8_pages *pages, const int32_t *table, int64_t stride, i
 int kv8_attn_check(const t2c_q8_pages *pages, const char *what, KvPages &pg, const int32_t *table, int64_t bt_stride,
                    int64_t bt_width, const int32_t *positions, int64_t B, int64_t T, int64_t NH, int64_t &max_len);
 
+// cuTensorMapEncodeTiled, or null.
+PFN_cuTensorMapEncodeTiled kv8_encoder();
+
 // Tensor maps of the codes as (dim, row of page, KV head, page), boxes of `rows` rows of one head in the swizzle that
 // is as wide as a row (128 or 64 bytes).  False when the driver refuses.
 bool kv8_maps(const t2c_q8_pages *pages, int rows, CUtensorMap &k_map, CUtensorMap &v_map);
