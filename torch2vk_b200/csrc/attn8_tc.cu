@@ -545,18 +545,38 @@ __global__ void __launch_bounds__(256) attn8_prefill_join_kernel(const __grid_co
     const int per = (tiles + a.splits - 1) / a.splits, used = per > 0 ? (tiles + per - 1) / per : 0;
     const float *base = a.parts + ((static_cast<int64_t>(b) * a.pg.n_kv + head) * a.pairs + pair) * a.splits * (256 * (D + 2));
     const bool seen = p0 + t >= 0;
-    constexpr int kPer = D / 32;
-    float acc[kPer] = {}, top = kPRefStart, sum = 0.0f;
-    for (int s = lane; s < used; s += 32) top = fmaxf(top, base[static_cast<int64_t>(s) * 256 * (D + 2) + 256 * D + row]);
-    top = warp_max(top);
-#pragma unroll 4
-    for (int s = 0; s < used; ++s) {
-        const float *part = base + static_cast<int64_t>(s) * 256 * (D + 2);
-        const float f = ex2(part[256 * D + row] - top);
-        sum = fmaf(part[256 * (D + 1) + row], f, sum);
-        const float *o = part + row * D + kPer * lane;
+    constexpr int kPer = D / 32, kAhead = 8;
+    constexpr int64_t kPart = 256 * (D + 2);
+    // lane s (and s + 32): the statistics of split s; the first rows of O come beside them
+    using Vec = typename std::conditional<kPer == 4, float4, float2>::type;
+    const float *rows = base + row * D + kPer * lane;
+    Vec v[kAhead];
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) acc[i] = fmaf(o[i], f, acc[i]);
+    for (int s = 0; s < kAhead; ++s)
+        if (s < used) v[s] = *reinterpret_cast<const Vec *>(rows + s * kPart);
+    float m[2], l[2], top = kPRefStart;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int s = lane + 32 * k;
+        m[k] = s < used ? base[s * kPart + 256 * D + row] : kPRefStart;
+        l[k] = s < used ? base[s * kPart + 256 * (D + 1) + row] : 0.0f;
+        top = fmaxf(top, m[k]);
+    }
+    top = warp_max(top);
+    float f[2] = {ex2(m[0] - top), ex2(m[1] - top)};
+    const float sum = warp_sum(fmaf(l[0], f[0], l[1] * f[1]));
+    float acc[kPer] = {};
+    for (int s0 = 0; s0 < used; s0 += kAhead) {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int s = s0 + k;
+            const float w = __shfl_sync(0xffffffffu, s < 32 ? f[0] : f[1], s & 31);
+            const float *o = reinterpret_cast<const float *>(&v[k]);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if (s < used) acc[i] = fmaf(o[i], w, acc[i]);
+            if (s + kAhead < used) v[k] = *reinterpret_cast<const Vec *>(rows + (s + kAhead) * kPart);
+        }
     }
     const float inv = seen ? 1.0f / sum : 0.0f;
     __half2 *out = reinterpret_cast<__half2 *>(a.out + b * a.o_sb + static_cast<int64_t>(t) * a.o_st + h * a.o_sh) + kPer / 2 * lane;

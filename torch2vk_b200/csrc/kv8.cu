@@ -201,61 +201,58 @@ __global__ void __launch_bounds__(128) kv8_write_kernel(KvPages pg, const __half
 }
 
 // ------------------------------------------------------------------ read
-// A thread turns 16 codes into 16 fp16 values; K and V of one unit by neighbouring grid halves.
+// A thread turns 16 codes into 16 fp16 values; blockIdx.y: sequence, K or V.  (Several units a thread were slower: the
+// table, scale and code loads of a unit depend on one another, and more threads hide that better.)
 template <int D>
 __global__ void __launch_bounds__(256) kv8_read_kernel(KvPages pg, __half *__restrict__ k_out,
                                                        __half *__restrict__ v_out, const int32_t *__restrict__ first,
                                                        const int32_t *__restrict__ lengths,
                                                        const int32_t *__restrict__ table, int64_t t_stride,
-                                                       int64_t capacity, int T, int64_t units) {
-    constexpr int kPerRow = D / 16;
+                                                       int64_t capacity, int T, unsigned units) {
+    constexpr unsigned kPerRow = D / 16;
+    const bool is_v = blockIdx.y & 1;
+    const int b = blockIdx.y >> 1;
+    const unsigned per_token = static_cast<unsigned>(pg.n_kv) * kPerRow, u = blockIdx.x * 256u + threadIdx.x;
     pdl_wait();
     pdl_trigger();
-    const bool is_v = blockIdx.y;
-    const int64_t u = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
     if (u >= units) return;
-    const int part = static_cast<int>(u % kPerRow);
-    const int64_t r = u / kPerRow;  // (b, t, head) row of the output
-    const int head = static_cast<int>(r % pg.n_kv);
-    const int t = static_cast<int>(r / pg.n_kv % T);
-    const int b = static_cast<int>(r / pg.n_kv / T);
-    const int64_t pos = static_cast<int64_t>(first[b]) + t;
+    const int64_t pos = static_cast<int64_t>(first[b]) + u / per_token;
     int64_t n = lengths[b];
     if (n > capacity) {
         report_device_error(T2C_EINVAL);
         n = capacity;
     }
+    const int page = pos >= 0 && pos < n ? kv8_page(pg, table + b * t_stride, pos) : -1;
     uint4 out[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-    if (pos >= 0 && pos < n) {
-        const int page = kv8_page(pg, table + b * t_stride, pos);
-        if (page >= 0) {
-            const uint4 c = *reinterpret_cast<const uint4 *>((is_v ? pg.v : pg.k) + kv8_row_offset(pg, page, head, pos) +
-                                                             16 * part);
-            const __half2 s = __half2half2((is_v ? pg.vs : pg.ks)[kv8_scale_offset(pg, page, head, pos)]);
-            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-            uint32_t *o = reinterpret_cast<uint32_t *>(out);
+    if (page >= 0) {
+        const int head = static_cast<int>(u % per_token / kPerRow);
+        const uint4 c = ldg_nc_v4((is_v ? pg.v : pg.k) + kv8_row_offset(pg, page, head, pos) + 16 * (u % kPerRow));
+        const __half2 s = __half2half2((is_v ? pg.vs : pg.ks)[kv8_scale_offset(pg, page, head, pos)]);
+        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+        uint32_t *o = reinterpret_cast<uint32_t *>(out);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                __half2 even, odd;
-                kv8_unpack(w[j], even, odd);
-                even = __hmul2(even, s);  // exact product, rounded once
-                odd = __hmul2(odd, s);
-                const __half2 a = __lows2half2(even, odd), d = __highs2half2(even, odd);
-                o[2 * j] = *reinterpret_cast<const uint32_t *>(&a);
-                o[2 * j + 1] = *reinterpret_cast<const uint32_t *>(&d);
-            }
+        for (int j = 0; j < 4; ++j) {
+            __half2 even, odd;
+            kv8_unpack(w[j], even, odd);
+            even = __hmul2(even, s);  // exact product, rounded once
+            odd = __hmul2(odd, s);
+            const __half2 x = __lows2half2(even, odd), y = __highs2half2(even, odd);
+            o[2 * j] = *reinterpret_cast<const uint32_t *>(&x);
+            o[2 * j + 1] = *reinterpret_cast<const uint32_t *>(&y);
         }
     }
-    uint4 *dst = reinterpret_cast<uint4 *>((is_v ? v_out : k_out) + r * D + 16 * part);
+    uint4 *dst = reinterpret_cast<uint4 *>((is_v ? v_out : k_out) + static_cast<int64_t>(b) * T * pg.n_kv * D + 16ll * u);
     dst[0] = out[0];
     dst[1] = out[1];
 }
 
 // ------------------------------------------------------------------ eviction
-constexpr int kEvThreads = 512;
+constexpr int kEvThreads = 1024;
 constexpr int kEvWarps = kEvThreads / 32;
-constexpr int kEvCache = 8192;                // weights of a CTA's slice kept in shared memory
-constexpr int kEvRows = kEvWarps / 2 * 16;    // rows a CTA moves per round: a warp 16 rows of K or of V
+constexpr int kEvCache = 32768;             // weights of a CTA's slice kept in shared memory
+// Rows a CTA moves at a time: a warp 16 rows of K or of V.
+constexpr int mv_threads(bool in_place) { return in_place ? 512 : 256; }
+constexpr int mv_rows(bool in_place) { return mv_threads(in_place) / 64 * 16; }
 
 // A weight as an integer that orders as the weights do; NaN above all, -0 as 0.
 __device__ __forceinline__ uint32_t ev_key(float w) {
@@ -266,28 +263,20 @@ __device__ __forceinline__ uint32_t ev_key(float w) {
 
 __device__ __forceinline__ int ev_warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
 
-// One cluster per (sequence, KV head).  Selection: the quota-th largest weight
-// of the unprotected positions by three radix passes (11, 11, 10 bits) whose
-// histograms are summed over the cluster through distributed shared memory;
-// equal weights go to the lowest positions.  Move: rounds of 128 rows per CTA
-// in ascending order; in place, every CTA has read its rows of the round (and
-// all earlier rounds) before any stores, and a row never moves up, so a store
-// of round r can only hit sources of rounds <= r.
-template <int D>
-__global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(
-    KvPages pg, const float *weights, int64_t w_sb, int64_t w_sh, const int32_t *__restrict__ lengths,
-    const int32_t *table, int64_t t_stride, int64_t capacity, const int32_t *out_table, int64_t o_stride, bool in_place,
-    int keep, int sinks, int recent, float *weights_out, int64_t wo_sb, int64_t wo_sh, int32_t *kept,
-    int32_t *new_lengths) {
+// Which positions stay.  One CTA per (sequence, KV head), a cluster where the weights are more than its shared memory
+// holds: the quota-th largest weight of the unprotected positions by three radix passes (11, 11, 10 bits) whose
+// histograms are summed over the cluster through distributed shared memory; equal weights go to the lowest positions.
+__global__ void __launch_bounds__(kEvThreads) kv8_select_kernel(
+    int n_kv, const float *__restrict__ weights, int64_t w_sb, int64_t w_sh, const int32_t *__restrict__ lengths, int64_t capacity,
+    int cache_size, int keep, int sinks, int recent, int32_t *__restrict__ kept, int32_t *__restrict__ new_lengths) {
     extern __shared__ uint32_t cache[];
     __shared__ uint32_t hist[3][2048];
     __shared__ int warp_sure[kEvWarps], warp_eq[kEvWarps], cta_sure, cta_eq, found[2];
-    __shared__ uint32_t slice_top[kEvWarps];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int head = (blockIdx.x / C) % pg.n_kv;
-    const int b = blockIdx.x / C / pg.n_kv;
+    const int head = (blockIdx.x / C) % n_kv;
+    const int b = blockIdx.x / C / n_kv;
     for (int i = tid; i < 3 * 2048; i += kEvThreads) (&hist[0][0])[i] = 0;
     pdl_wait();
     pdl_trigger();
@@ -299,13 +288,13 @@ __global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(
     const int left = min(n, keep);
     if (rank == 0 && head == 0 && tid == 0) new_lengths[b] = left;
     const float *w = weights + b * w_sb + head * w_sh;
-    int32_t *kp = kept + (static_cast<int64_t>(b) * pg.n_kv + head) * keep;
+    int32_t *kp = kept + (static_cast<int64_t>(b) * n_kv + head) * keep;
     // this CTA's positions, and its warps' spans of them (multiples of 32 keep the order of positions)
     const int per_warp = ((n + C * kEvWarps - 1) / (C * kEvWarps) + 31) & ~31;
     const int64_t lo = static_cast<int64_t>(rank) * kEvWarps * per_warp;
     const int s0 = static_cast<int>(min(lo, static_cast<int64_t>(n)));
     const int s1 = static_cast<int>(min(lo + static_cast<int64_t>(kEvWarps) * per_warp, static_cast<int64_t>(n)));
-    const bool cached = s1 - s0 <= kEvCache;
+    const bool cached = s1 - s0 <= cache_size;
     const auto key_at = [&](int pos) { return cached ? cache[pos - s0] : ev_key(w[pos]); };
 
     uint32_t threshold = 0xffffffffu;  // keys above it stay, and the first `ties` equal to it
@@ -314,6 +303,7 @@ __global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(
     const bool choose = n > keep;
     if (choose) {
         if (cached) {
+#pragma unroll 4
             for (int pos = s0 + tid; pos < s1; pos += kEvThreads) cache[pos - s0] = ev_key(w[pos]);
         }
         __syncthreads();
@@ -324,22 +314,21 @@ __global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(
             for (int pass = 0; pass < 3; ++pass) {
                 const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
                 const int bits = pass == 2 ? 10 : 11;
+#pragma unroll 4
                 for (int pos = a + tid; pos < z; pos += kEvThreads) {
                     const uint32_t key = key_at(pos);
                     if (pass == 0 || (key >> (shift + bits)) == prefix)
                         atomicAdd(&hist[pass][(key >> shift) & ((1u << bits) - 1)], 1u);
                 }
                 cluster.sync();
-                // bins 4 * tid .. + 3 over the cluster, then the bin where the count from the top reaches `want`
-                uint32_t c[4] = {0, 0, 0, 0};
+                // bins 2 * tid and 2 * tid + 1 over the cluster, then the bin where the count from the top reaches `want`
+                int c[2] = {0, 0};
                 for (int r = 0; r < C; ++r) {
-                    const uint4 h = *reinterpret_cast<const uint4 *>(cluster.map_shared_rank(&hist[pass][4 * tid], r));
-                    c[0] += h.x;
-                    c[1] += h.y;
-                    c[2] += h.z;
-                    c[3] += h.w;
+                    const uint2 h = *reinterpret_cast<const uint2 *>(cluster.map_shared_rank(&hist[pass][2 * tid], r));
+                    c[0] += static_cast<int>(h.x);
+                    c[1] += static_cast<int>(h.y);
                 }
-                const int mine = static_cast<int>(c[0] + c[1] + c[2] + c[3]);
+                const int mine = c[0] + c[1];
                 int suffix = mine;  // over this and the higher lanes
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -349,16 +338,14 @@ __global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(
                 if (lane == 0) warp_sure[warp] = suffix;
                 __syncthreads();
                 int above = suffix - mine;
-                for (int i = warp + 1; i < kEvWarps; ++i) above += warp_sure[i];
+                {
+                    const int higher = lane > warp && lane < kEvWarps ? warp_sure[lane] : 0;
+                    above += __reduce_add_sync(0xffffffffu, higher);
+                }
                 if (above < want && above + mine >= want) {
-                    for (int e = 3; e >= 0; --e) {
-                        if (above + static_cast<int>(c[e]) >= want) {
-                            found[0] = 4 * tid + e;
-                            found[1] = want - above;
-                            break;
-                        }
-                        above += static_cast<int>(c[e]);
-                    }
+                    const bool upper = above + c[1] >= want;
+                    found[0] = 2 * tid + (upper ? 1 : 0);
+                    found[1] = want - above - (upper ? 0 : c[1]);
                 }
                 __syncthreads();
                 prefix = (prefix << bits) | static_cast<uint32_t>(found[0]);
@@ -396,14 +383,9 @@ __global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(
         warp_eq[warp] = n_eq;
     }
     __syncthreads();
-    if (tid == 0) {
-        int a = 0, e = 0;
-        for (int i = 0; i < kEvWarps; ++i) {
-            a += warp_sure[i];
-            e += warp_eq[i];
-        }
-        cta_sure = a;
-        cta_eq = e;
+    if (warp == 0) {
+        const int a = ev_warp_sum(warp_sure[lane]), e = ev_warp_sum(warp_eq[lane]);
+        if (lane == 0) cta_sure = a, cta_eq = e;
     }
     cluster.sync();
     int run_sure = 0, run_eq = 0;
@@ -411,10 +393,8 @@ __global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(
         run_sure += *cluster.map_shared_rank(&cta_sure, r);
         run_eq += *cluster.map_shared_rank(&cta_eq, r);
     }
-    for (int i = 0; i < warp; ++i) {
-        run_sure += warp_sure[i];
-        run_eq += warp_eq[i];
-    }
+    run_sure += ev_warp_sum(lane < warp ? warp_sure[lane] : 0);
+    run_eq += ev_warp_sum(lane < warp ? warp_eq[lane] : 0);
     for (int base = p0; base < p1; base += 32) {
         bool sure, eq;
         classify(base + lane, sure, eq);
@@ -426,65 +406,104 @@ __global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(
         run_eq += __popc(me);
     }
     for (int i = left + rank * kEvThreads + tid; i < keep; i += C * kEvThreads) kp[i] = -1;
-    cluster.sync();  // the cluster's kept positions are in memory
-    const bool moved = !(in_place && n <= keep);
+    cluster.sync();  // no CTA leaves while another may still read its shared memory
+}
+
+// Moves the kept rows: half of a CTA's warps K, half V, in 16-row slices.  To other pages each CTA moves 64 rows.  In
+// place the CTAs of a head are a cluster that walks its rows in ascending rounds of 128 a CTA, and stores once each has
+// read its rows of the round: a row never moves up, so the stores of a round hit no source of a later one, and the
+// next round's rows are read ahead of the stores.  (Rounds with that read-ahead, two CTAs per SM, took 41 us where one
+// round per CTA takes 30 when the rows go to other pages: 4 sequences of 16k positions, 4096 of 8 heads kept.)
+template <int D, bool IN_PLACE>
+__global__ void __launch_bounds__(mv_threads(IN_PLACE), IN_PLACE ? 2 : 5) kv8_move_kernel(
+    KvPages pg, const float *weights, int64_t w_sb, int64_t w_sh, const int32_t *__restrict__ lengths,
+    const int32_t *__restrict__ table, int64_t t_stride, int64_t capacity, const int32_t *__restrict__ out_table,
+    int64_t o_stride, int keep, int chunks, float *weights_out, int64_t wo_sb, int64_t wo_sh,
+    const int32_t *__restrict__ kept) {
+    constexpr int kWarps = mv_threads(IN_PLACE) / 32, kRowsCta = mv_rows(IN_PLACE);
+    __shared__ uint32_t slice_top[2][kWarps];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int unit = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+    const int head = unit % pg.n_kv, b = unit / pg.n_kv;
+    pdl_wait();
+    pdl_trigger();
+    int left = keep;  // to other pages the -1 of `kept` ends the rows
+    const int step = chunks * kRowsCta;
+    if (IN_PLACE) {
+        const int n = max(min(lengths[b], static_cast<int>(min(capacity, static_cast<int64_t>(INT32_MAX)))), 0);
+        if (n <= keep) return;  // the whole cluster
+    }
+    const float *w = weights + b * w_sb + head * w_sh;
     float *wo = weights_out + b * wo_sb + head * wo_sh;
     const int32_t *bt = table + b * t_stride, *bo = out_table + b * o_stride;
-
-    // ---- move: warps 0..7 K, 8..15 V of eight 16-row slices
-    const bool is_v = warp >= kEvWarps / 2;
-    const int slice_of = warp & (kEvWarps / 2 - 1);
+    const int32_t *kp = kept + (static_cast<int64_t>(b) * pg.n_kv + head) * keep;
+    const bool is_v = warp >= kWarps / 2;
+    const int slice_of = warp & (kWarps / 2 - 1);
     int8_t *codes = is_v ? pg.v : pg.k;
     __half *scales = is_v ? pg.vs : pg.ks;
     constexpr int kUnits = D / 64 * 2;  // 16-byte units of 16 rows per lane
     constexpr int kPerRow = D / 16;
-    for (int r0 = 0; r0 < left && moved; r0 += C * kEvRows) {
-        const int row0 = r0 + rank * kEvRows + 16 * slice_of;  // destination rows row0 .. row0 + 15
-        // lanes 0..15: the source of row row0 + lane
+
+    uint4 x[kUnits];
+    float s_src = 0.0f, w_val = 0.0f;  // of row lane & 15 of the slice
+    int rows = 0;                      // of the slice
+    const auto fetch = [&](int r0) {
+        const int row0 = r0 + chunk * kRowsCta + 16 * slice_of, my_row = row0 + (lane & 15);
         int64_t src = 0;
-        float s_src = 0.0f, w_val = 0.0f;
-        const int my_row = row0 + (lane & 15);
-        if (my_row < left) {
-            const int pos = kp[my_row];
-            int page = kv8_page(pg, bt, pos);
-            if (page < 0) page = 0;
+        s_src = 0.0f;
+        const int pos = my_row < left ? kp[my_row] : -1;
+        rows = __popc(__ballot_sync(0xffffffffu, lane < 16 && pos >= 0));
+        if (pos >= 0) {
+            const int page = max(kv8_page(pg, bt, pos), 0);
             src = kv8_row_offset(pg, page, head, pos);
             s_src = __half2float(scales[kv8_scale_offset(pg, page, head, pos)]);
             if (!is_v) w_val = w[pos];
         }
-        uint4 x[kUnits];
-        float s_row[kUnits];
-        float top = 0.0f;
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
             const int u = i * 32 + lane, row = u / kPerRow;
             const int64_t at = __shfl_sync(0xffffffffu, src, row);
-            s_row[i] = __shfl_sync(0xffffffffu, s_src, row);
             x[i] = make_uint4(0, 0, 0, 0);
-            if (row0 + row < left) x[i] = *reinterpret_cast<const uint4 *>(codes + at + (u % kPerRow) * 16);
-            uint32_t m = kv8_absmax(x[i].x, 0);
-            m = kv8_absmax(x[i].y, m);
-            m = kv8_absmax(x[i].z, m);
-            m = kv8_absmax(x[i].w, m);
+            if (row < rows) x[i] = *reinterpret_cast<const uint4 *>(codes + at + (u % kPerRow) * 16);
+        }
+    };
+    fetch(0);
+    for (int r0 = 0, round = 0; r0 < (IN_PLACE ? left : 1); r0 += step, ++round) {
+        const int row0 = r0 + chunk * kRowsCta + 16 * slice_of, my_row = row0 + (lane & 15);
+        float s_row[kUnits], top = 0.0f;
+        uint4 q[kUnits];
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+            s_row[i] = __shfl_sync(0xffffffffu, s_src, (i * 32 + lane) / kPerRow);
+            q[i] = x[i];
+            uint32_t m = kv8_absmax(q[i].x, 0);
+            m = kv8_absmax(q[i].y, m);
+            m = kv8_absmax(q[i].z, m);
+            m = kv8_absmax(q[i].w, m);
             const float mag = static_cast<float>(max(m >> 16, m & 0xffffu)) * s_row[i];
             top = s_row[i] != s_row[i] ? INFINITY : fmaxf(top, mag);
         }
+        const float w_row = w_val;
+        const int mine = rows;
         const uint32_t top_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-        __syncthreads();  // the round before is done with slice_top
-        if (lane == 0) slice_top[warp] = top_bits;
-        if (in_place)
+        uint32_t *tops = slice_top[round & 1];
+        if (lane == 0) tops[warp] = top_bits;
+        if (IN_PLACE) {
             cluster.sync();
-        else
+            if (r0 + step < left) fetch(r0 + step);
+        } else {
             __syncthreads();
+        }
         const int per_block = 1 << (pg.block_log2 - 4);
         const int w0 = warp & ~(per_block - 1);
         uint32_t best = 0;
-        for (int i = 0; i < per_block; ++i) best = max(best, slice_top[w0 + i]);
+        for (int i = 0; i < per_block; ++i) best = max(best, tops[w0 + i]);
         const __half s_half = kv8_scale_for(__uint_as_float(best));
         const float s = __half2float(s_half);
         const bool ok = s > 0.0f;
         const float inv = ok ? 1.0f / s : 0.0f;
-        if (row0 >= left) continue;
+        if (mine == 0) continue;
         const int page = kv8_page(pg, bo, row0);
         if (page < 0) continue;
         if (lane == 0 && warp == w0) scales[kv8_scale_offset(pg, page, head, row0)] = s_half;
@@ -492,21 +511,20 @@ __global__ void __launch_bounds__(kEvThreads) kv8_evict_kernel(
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
             const int u = i * 32 + lane, row = u / kPerRow;
-            if (row0 + row >= left) continue;
-            uint32_t *q = reinterpret_cast<uint32_t *>(&x[i]);
+            if (row >= mine) continue;
+            uint32_t *c4 = reinterpret_cast<uint32_t *>(&q[i]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint32_t c[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    c[e] = kv8_code(static_cast<float>(static_cast<int8_t>(q[j] >> (8 * e))) * s_row[i], s, inv);
-                q[j] = ok ? kv8_pack4(c[0], c[1], c[2], c[3]) : 0u;
+                    c[e] = kv8_code(static_cast<float>(static_cast<int8_t>(c4[j] >> (8 * e))) * s_row[i], s, inv);
+                c4[j] = ok ? kv8_pack4(c[0], c[1], c[2], c[3]) : 0u;
             }
-            *reinterpret_cast<uint4 *>(dst + row * pg.row_stride + (u % kPerRow) * 16) = x[i];
+            *reinterpret_cast<uint4 *>(dst + row * pg.row_stride + (u % kPerRow) * 16) = q[i];
         }
-        if (!is_v && lane < 16 && my_row < left) wo[my_row] = w_val;
+        if (!is_v && lane < mine) wo[my_row] = w_row;
     }
-    cluster.sync();  // no CTA leaves while another may still read its shared memory
 }
 
 }  // namespace
@@ -551,13 +569,14 @@ extern "C" int t2c_kv_cache_read_q8(const t2c_q8_pages *pages, void *k_out, void
     if (B <= 0 || T <= 0 || T > INT32_MAX) return set_error(T2C_EINVAL, "kv_cache_read_q8: bad shape");
     if (!kv8_aligned(k_out, 16) || !kv8_aligned(v_out, 16))
         return set_error(T2C_EINVAL, "kv_cache_read_q8: outputs must be 16-byte aligned");
-    const int64_t units = B * T * pg.n_kv * (pages->head_dim / 16);
+    const int64_t units = T * pg.n_kv * (pages->head_dim / 16);  // of a sequence
+    if (units > INT32_MAX - 1024 || B > 32767) return set_error(T2C_EINVAL, "kv_cache_read_q8: bad shape");
     const int64_t blocks = (units + 255) / 256;
-    if (blocks > INT32_MAX) return set_error(T2C_EINVAL, "kv_cache_read_q8: bad shape");
     const auto kern = pages->head_dim == 128 ? kv8_read_kernel<128> : kv8_read_kernel<64>;
-    return kv8_launch("kv_cache_read_q8", kern, dim3(static_cast<unsigned>(blocks), 2), dim3(256), 0, 1, as_stream(stream), pg,
+    return kv8_launch("kv_cache_read_q8", kern, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(2 * B)),
+                      dim3(256), 0, 1, as_stream(stream), pg,
                       static_cast<__half *>(k_out), static_cast<__half *>(v_out), first, lengths, block_table, bt_stride,
-                      capacity, static_cast<int>(T), units);
+                      capacity, static_cast<int>(T), static_cast<unsigned>(units));
 }
 
 extern "C" int t2c_kv_cache_evict_q8(const t2c_q8_pages *pages, const float *weights, int64_t w_sb, int64_t w_sh,
@@ -584,22 +603,31 @@ extern "C" int t2c_kv_cache_evict_q8(const t2c_q8_pages *pages, const float *wei
     if (!in_place && weights == weights_out)
         return set_error(T2C_EINVAL, "kv_cache_evict_q8: weights in place need the codes in place");
     const int64_t heads = B * pg.n_kv;
-    // CTAs per (sequence, head): as many as keep all SMs busy, up to 8, and no more than there are rows for
+    // CTAs that select for a head: up to 8 while the SMs have room and each keeps 2048 positions
     unsigned cluster = 1;
-    while (cluster < 8 && heads * cluster < sm_count() && capacity > static_cast<int64_t>(cluster) * 512) cluster *= 2;
-    if (heads * cluster > INT32_MAX) return set_error(T2C_EINVAL, "kv_cache_evict_q8: bad shape");
-    const auto kern = pages->head_dim == 128 ? kv8_evict_kernel<128> : kv8_evict_kernel<64>;
-    static bool configured[2][64] = {};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-    bool &done = configured[pages->head_dim == 128][dev];
-    if (!done) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvCache * 4) != cudaSuccess)
-            return set_error(T2C_ECUDA, "kv_cache_evict_q8: cudaFuncSetAttribute failed");
-        done = true;
+    while (cluster < 8 && capacity > static_cast<int64_t>(cluster) * 4096 &&
+           (heads * cluster * 2 <= sm_count() || capacity > static_cast<int64_t>(cluster) * kEvCache))
+        cluster *= 2;
+    const int64_t slice = (capacity + cluster - 1) / cluster + 32 * kEvWarps;
+    const int cache = static_cast<int>(slice < kEvCache ? slice : kEvCache);
+    int64_t chunks = (keep + mv_rows(in_place) - 1) / mv_rows(in_place);
+    if (in_place) {  // a cluster per head, as large as keeps the SMs busy, up to 8
+        const int64_t full = chunks;
+        chunks = 1;
+        while (chunks < 8 && chunks < full && heads * chunks < 2 * sm_count()) chunks *= 2;
     }
-    return kv8_launch("kv_cache_evict_q8", kern, dim3(static_cast<unsigned>(heads * cluster)), dim3(kEvThreads), kEvCache * 4,
-                      cluster, as_stream(stream), pg, weights, w_sb, w_sh, lengths, block_table, bt_stride, capacity,
-                      out_table, ot_stride, in_place, static_cast<int>(keep), static_cast<int>(sinks),
-                      static_cast<int>(recent), weights_out, wo_sb, wo_sh, kept, new_lengths);
+    if (heads * cluster > INT32_MAX || heads * chunks > INT32_MAX) return set_error(T2C_EINVAL, "kv_cache_evict_q8: bad shape");
+    rc = kv8_configure(kv8_select_kernel, kEvCache * 4, 6, "kv_cache_evict_q8");
+    if (rc == T2C_OK)
+        rc = kv8_launch("kv_cache_evict_q8", kv8_select_kernel, dim3(static_cast<unsigned>(heads * cluster)), dim3(kEvThreads),
+                        static_cast<size_t>(cache) * 4, cluster, as_stream(stream), pg.n_kv, weights, w_sb, w_sh, lengths, capacity, cache,
+                        static_cast<int>(keep), static_cast<int>(sinks), static_cast<int>(recent), kept, new_lengths);
+    if (rc != T2C_OK) return rc;
+    const bool wide = pages->head_dim == 128;
+    const auto kern = in_place ? (wide ? kv8_move_kernel<128, true> : kv8_move_kernel<64, true>)
+                               : (wide ? kv8_move_kernel<128, false> : kv8_move_kernel<64, false>);
+    return kv8_launch("kv_cache_evict_q8 move", kern, dim3(static_cast<unsigned>(heads * chunks)), dim3(mv_threads(in_place)), 0,
+                      in_place ? static_cast<unsigned>(chunks) : 1u, as_stream(stream), pg, weights, w_sb, w_sh, lengths,
+                      block_table, bt_stride, capacity, out_table, ot_stride, static_cast<int>(keep), static_cast<int>(chunks),
+                      weights_out, wo_sb, wo_sh, kept);
 }
