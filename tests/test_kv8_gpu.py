@@ -448,6 +448,31 @@ def test_key_weights_match_definition(NH, NK, dim, T, page, block):
         assert bool(((fresh[b, :, :n].double().cpu() - step).abs() <= step * (2 * eps + 1e-5) + 1e-12).all())
 
 
+@pytest.mark.parametrize("NH,NK,dim,T,p0", [(16, 1, 64, 1100, 0), (24, 2, 128, 900, 70), (8, 2, 128, 3, 5000)])
+def test_key_weights_long(NH, NK, dim, T, p0):
+    """Many query tiles (their keys' sums shared out over a cluster) and many keys under few queries (several key tiles a CTA)."""
+    from torch2vk_b200 import kernels
+
+    page, block = 64, 32
+    width = -(-(p0 + T) // page)
+    cache, table, g, _ = attention_case(1, NH, NK, dim, page, block, width, 85)
+    pages, bt = device_pages(cache, "token_major"), table.cuda()
+    q = torch.randn(1, T, NH, dim, generator=g).half()
+    want = ref.attention(cache, q, [p0], table, dim ** -0.5)
+    before = torch.rand(1, NK, width * page, generator=g)
+    w = torch.zeros(1, NK, width * page, device="cuda")
+    b = before.cuda()
+    qh = q.cuda().transpose(1, 2).contiguous().transpose(1, 2)
+    kernels.attn_key_weights_q8(qh, want["lse"].float().cuda(), pages, i32([p0]), bt, weights=b, weights_out=w)
+    clean()
+    n = p0 + T
+    step = want["probs"][0].view(NK, -1, n).sum(1)
+    old = torch.where(torch.arange(n) < p0, before[0, :, :n].double(), torch.zeros(()).double())
+    eps = float(want["reach"].max()) * 2.0 ** -17
+    assert bool(((w[0, :, :n].double().cpu() - (old + step)).abs() <= step * (2 * eps + 1e-5) + 1e-6 * old + 1e-12).all())
+    assert torch.equal(b.cpu(), before)
+
+
 # ------------------------------------------------------------------ eviction
 @pytest.mark.parametrize("dim,page,block", [(128, 64, 16), (64, 16, 16), (64, 64, 64), (128, 64, 32)])
 @pytest.mark.parametrize("in_place", [False, True])

@@ -8,10 +8,13 @@
 // log-sum-exps are read from shared memory by all lanes alike.  Sums are per 32 columns, per tile, then over tiles, in
 // fp32 and in a fixed order.  What bounds it: the 2^ unit, one per (head, query, key); two CTAs share an SM, so that one's
 // other instructions run under the other's.
+#include <cooperative_groups.h>
 #include <cudaTypedefs.h>
 
 #include "kv8.cuh"
 #include "umma.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace t2c {
 namespace {
@@ -22,7 +25,7 @@ constexpr int kWThreads = 192;  // warps 0-3: keys; 4: query tiles and log-sum-e
 template <int D>
 struct WeightShape {
     static constexpr int kTile = 128 * D * 2;
-    static constexpr int kQ = kTile, kLse = kQ + 2 * kTile, kBars = kLse + 8 * 512, kSmem = kBars + 128;
+    static constexpr int kQ = kTile, kLse = kQ + 2 * kTile, kSums = kLse + 8 * 512, kBars = kSums + 512, kSmem = kBars + 128;
 };
 
 struct WeightArgs {
@@ -47,6 +50,7 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
     const uint32_t base = smem_u32(smem);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kBars);
     uint64_t *q_full = bars, *q_free = bars + 2, *s_ready = bars + 4, *s_free = bars + 6, *k_ready = bars + 8, *all_done = bars + 9;
+    float *sums = reinterpret_cast<float *>(smem + S::kSums);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 10);
     volatile int *stop = reinterpret_cast<volatile int *>(bars + 11), *stop_last = stop + 1;
     if (base & 1023u) {  // the swizzle atoms need it: report, compute nothing
@@ -80,10 +84,12 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
     pdl_wait();
     pdl_trigger();
 
-    // blocks of the first keys, which most queries see, first
-    const int pairs = a.B * a.pg.n_kv;
-    const int head = blockIdx.x % a.pg.n_kv, b = blockIdx.x / a.pg.n_kv % a.B;
-    const int kt0 = static_cast<int>(blockIdx.x / pairs) * a.keys_per;
+    // blocks of the first keys, which most queries see, first; a cluster shares out the query tiles of its keys
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+    const int pairs = a.B * a.pg.n_kv, item = blockIdx.x / C;
+    const int head = item % a.pg.n_kv, b = item / a.pg.n_kv % a.B;
+    const int kt0 = item / pairs * a.keys_per;
     const int64_t p0 = a.positions[b];
     int64_t n = p0 + a.T;
     if (n > a.max_len) {
@@ -92,10 +98,11 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
     }
     const int all_keys = n > 0 ? static_cast<int>((n + 127) / 128) : 0;
     const int kt1 = min(kt0 + a.keys_per, all_keys), nq = (a.T + TT - 1) / TT;
-    // first query tile that sees a key of tile kt
-    const auto first_q = [&](int kt) {
+    // query tiles that see a key of tile kt: this CTA's share of those from the first one on
+    const auto share = [&](int kt, int of) {
         const int64_t t = static_cast<int64_t>(kt) * 128 - p0;
-        return t <= 0 ? 0 : static_cast<int>(t / TT);
+        const int first = t <= 0 ? 0 : static_cast<int>(t / TT);
+        return first + static_cast<int>(static_cast<int64_t>(nq - first) * of / C);
     };
     if (kt0 < kt1) {
         if (warp < 4) {
@@ -154,8 +161,10 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
                 if (kt + 1 < kt1) fetch(kt + 1);
                 const int64_t key = static_cast<int64_t>(kt) * 128 + 32 * warp + lane;
                 const uint64_t kk = f32x2(kf_tile, kf_tile);
+                const int64_t o = b * a.w_sb + head * a.w_sh + key;
+                const float before = C == 1 && a.w_in && key < p0 && key < n ? a.w_in[o] : 0.0f;  // on its way under the products
                 float weight = 0.0f;
-                for (int q = first_q(kt); q < nq; ++q, ++count) {
+                for (int q = share(kt, rank), q_end = share(kt, rank + 1); q < q_end; ++q, ++count) {
                     const int buf = count & 1;
                     mbar_wait_or(&s_ready[buf], (count >> 1) & 1, stop);
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -195,16 +204,17 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
                     }
                     weight += tile;
                 }
-                if (key < n && !*stop) {
-                    const int64_t o = b * a.w_sb + head * a.w_sh + key;
-                    a.w_out[o] = weight + (a.w_in && key < p0 ? a.w_in[o] : 0.0f);
+                if (C > 1) {  // one key tile: the shares are summed below, in their order
+                    sums[tid] = weight;
+                } else if (key < n && !*stop) {
+                    a.w_out[o] = weight + before;
                 }
             }
         } else if (warp == 4) {
             int count = 0;
             const float *lse = a.lse + static_cast<int64_t>(b) * a.NH * a.T + static_cast<int64_t>(head) * group * a.T;
             for (int kt = kt0; kt < kt1; ++kt) {
-                for (int q = first_q(kt); q < nq; ++q, ++count) {
+                for (int q = share(kt, rank), q_end = share(kt, rank + 1); q < q_end; ++q, ++count) {
                     const int slot = count & 1;
                     if (count >= 2) mbar_wait_or(&q_free[slot], ((count >> 1) - 1) & 1, stop);
                     if (lane == 0) {
@@ -235,7 +245,7 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
             int count = 0;
             for (int kt = kt0; kt < kt1; ++kt) {
                 mbar_wait_or(k_ready, (kt - kt0) & 1, stop);
-                for (int q = first_q(kt); q < nq; ++q, ++count) {
+                for (int q = share(kt, rank), q_end = share(kt, rank + 1); q < q_end; ++q, ++count) {
                     const int slot = count & 1;
                     mbar_wait_or(&q_full[slot], (count >> 1) & 1, stop);
                     if (count >= 2) mbar_wait_or(&s_free[slot], ((count >> 1) - 1) & 1, stop);
@@ -258,6 +268,17 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
             *stop_last = 0;
             mbar_wait_or(all_done, 0, stop_last);  // nothing of this CTA is in flight when it frees its TMEM
         }
+    }
+    if (C > 1) {
+        cluster.sync();
+        const int64_t key = static_cast<int64_t>(kt0) * 128 + tid;
+        if (rank == 0 && tid < 128 && kt0 < kt1 && key < n && !*stop) {
+            float weight = 0.0f;
+            for (int r = 0; r < C; ++r) weight += *cluster.map_shared_rank(sums + tid, r);
+            const int64_t o = b * a.w_sb + head * a.w_sh + key;
+            a.w_out[o] = weight + (a.w_in && key < p0 ? a.w_in[o] : 0.0f);
+        }
+        cluster.sync();  // no CTA leaves while another may read its shared memory
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -314,18 +335,24 @@ extern "C" int t2c_attn_key_weights_q8(const t2c_q8_pages *pages, const void *q,
     a.B = static_cast<int>(B), a.T = static_cast<int>(T), a.NH = static_cast<int>(NH);
     a.scale_log2 = scale * 1.4426950408889634f;
     a.w_in = weights, a.w_out = weights_out, a.w_sb = w_sb, a.w_sh = w_sh;
-    // Key tiles of a CTA: one where many query tiles stream past it; where few do, several, so that the next tile's codes
-    // arrive under this one, but two waves of CTAs at least.
-    const int64_t nq = (T + tokens - 1) / tokens, tiles = (max_len + 127) / 128, units = B * a.pg.n_kv;
-    int64_t per = nq >= 8 ? 1 : units * tiles / (4 * sm_count());
-    per = per < 1 ? 1 : (per > 16 ? 16 : per);
+    // Where few query tiles stream past a key tile, a CTA takes several key tiles, as many as make one wave of two CTAs per
+    // SM (the next tile's codes arrive under this one).  Where many do, one, and a cluster of up to 8 CTAs shares out the
+    // query tiles of the first keys, which every query sees, until the longest share is under 3/4 of the mean of an SM's
+    // slot; 32 query tiles a CTA at least, which its beginning costs about 4 of (6000 queries of 16 heads on 8: 165 us
+    // alone, 124 in pairs, 147 in fours; 4096 queries of 16 heads of 64 on 16: 57, 66).
+    const int64_t nq = (T + tokens - 1) / tokens, tiles = (max_len + 127) / 128, units = B * a.pg.n_kv, slots = 2 * sm_count();
+    int64_t per = nq >= 8 ? 1 : (units * tiles + slots - 1) / slots;
+    per = per > 32 ? 32 : per;
+    unsigned cluster = 1;
+    const int64_t seen = units * (max_len > T ? (tiles - T / 128) * nq + nq * (T / 128) / 2 : nq * tiles / 2);
+    while (per == 1 && cluster < 8 && nq >= 64 * cluster && (nq / cluster) * slots > seen * 3 / 4) cluster *= 2;
     a.keys_per = static_cast<int>(per);
-    const int64_t blocks = units * ((tiles + per - 1) / per);
+    const int64_t blocks = units * ((tiles + per - 1) / per) * cluster;
     if (blocks > INT32_MAX) return set_error(T2C_EINVAL, "attn_key_weights_q8: bad shape");
     const auto kern = D == 128 ? attn8_weights_kernel<128> : attn8_weights_kernel<64>;
     const int smem = D == 128 ? WeightShape<128>::kSmem : WeightShape<64>::kSmem;
     rc = kv8_configure(kern, smem, D == 128 ? 4 : 5, "attn_key_weights_q8");
     if (rc != T2C_OK) return rc;
-    return kv8_launch("attn_key_weights_q8", kern, dim3(static_cast<unsigned>(blocks)), dim3(kWThreads), smem, 1, as_stream(stream),
+    return kv8_launch("attn_key_weights_q8", kern, dim3(static_cast<unsigned>(blocks)), dim3(kWThreads), smem, cluster, as_stream(stream),
                       q_map, a);
 }
