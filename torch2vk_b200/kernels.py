@@ -849,7 +849,7 @@ def _q8_index(t: torch.Tensor, batch: int, name: str) -> int:
     return _lib.ptr(t)
 
 
-def _q8_rows(x: torch.Tensor, name: str, heads: int | None, head_dim: int) -> tuple[int, ...]:
+def _head_rows(x: torch.Tensor, name: str, heads: int | None, head_dim: int) -> tuple[int, ...]:
     """Pointer and (batch, token, head) strides of an fp16 [B, T, heads, head_dim] tensor."""
     shape = x.shape
     if x.dtype != torch.float16 or len(shape) != 4 or shape[3] != head_dim or (heads is not None and shape[2] != heads):
@@ -869,7 +869,7 @@ def kv_cache_write_q8(pages: Q8Pages, k: torch.Tensor, v: torch.Tensor, position
     shape = k.shape
     if shape != v.shape:
         raise ValueError("k and v must have one shape")
-    kp, vp = _q8_rows(k, "k", pages.n_kv, pages.head_dim), _q8_rows(v, "v", pages.n_kv, pages.head_dim)
+    kp, vp = _head_rows(k, "k", pages.n_kv, pages.head_dim), _head_rows(v, "v", pages.n_kv, pages.head_dim)
     batch, tokens = shape[0], shape[1]
     _lib.lib().call("t2c_kv_cache_write_q8", pages.ref, *kp, *vp, _q8_index(positions, batch, "positions"),
                     *_q8_table(block_table, batch), batch, tokens, _lib.stream_ptr())
@@ -1005,7 +1005,7 @@ def attn_prefill_q8(q: torch.Tensor, pages: Q8Pages, positions: torch.Tensor, bl
     0..positions[b] + t (none when that is negative: zeros).  With return_lse (or an lse tensor) also the
     log-sum-exp of the scaled scores, fp32 [B, heads, T]."""
     dim, shape = pages.head_dim, q.shape
-    qp = _q8_rows(q, "q", None, dim)
+    qp = _head_rows(q, "q", None, dim)
     batch, tokens, n_heads = shape[0], shape[1], shape[2]
     out = _q8_out(q, out)
     o_strides = out.stride()
@@ -1027,7 +1027,7 @@ def attn_key_weights_q8(q: torch.Tensor, lse: torch.Tensor, pages: Q8Pages, posi
     attn_prefill_q8) give each cached key, summed over queries and the heads of a group and added to weights for
     positions before positions[b]; weights_out fp32 [B, n_kv, positions] is written up to the last query's key."""
     heads, dim, shape = pages.n_kv, pages.head_dim, q.shape
-    qp = _q8_rows(q, "q", None, dim)
+    qp = _head_rows(q, "q", None, dim)
     batch, tokens, n_heads = shape[0], shape[1], shape[2]
     max_len = _q8_max_len(max_len, block_table, pages)
     _q8_lse(lse, False, (batch, n_heads, tokens), q)
