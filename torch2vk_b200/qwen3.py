@@ -28,7 +28,7 @@ from dataclasses import dataclass, field
 import torch
 
 from torch2vk_b200 import kernels
-from torch2vk_b200.paged_kv import PagedKVCache
+from torch2vk_b200.paged_kv import PagedKVCache, PagedKVCacheQ8
 
 Q6_NAMES = ("v_proj", "down_proj")
 
@@ -126,20 +126,38 @@ class Qwen3Runner:
     fused_attention: bool = True
     page_size: int = 0
     kv_pages: int = 0
+    kv_bits: int = 16
+    kv_block: int = 16
+    kv_budget: int = 0
+    kv_sinks: int = 4
+    kv_recent: int = 32
+    kv_window: int = 32
     k_cache: list[torch.Tensor] = field(init=False)
     v_cache: list[torch.Tensor] = field(init=False)
 
     def __post_init__(self) -> None:
         """page_size > 0 keeps the KV cache in a paged pool (PagedKVCache) of kv_pages pages (default: enough
-        for every sequence at max_seq) instead of one contiguous [batch, max_seq] cache per layer."""
+        for every sequence at max_seq) instead of one contiguous [batch, max_seq] cache per layer.
+
+        kv_bits = 8 keeps that pool in 8 bits (PagedKVCacheQ8, one scale per kv_block tokens and KV head).  Prompts
+        then attend over the quantized cache too, and prefill(append=True) continues on what is cached.  kv_budget > 0
+        bounds each sequence's cached positions: the attention weight each key receives is kept (a prompt's from its
+        last kv_window queries, then every decoded token's), and a sequence that has grown to kv_budget plus a page
+        is cut to kv_budget positions per KV head, the first kv_sinks and the last kv_recent always among them."""
         cfg, dev = self.cfg, self.weights.final_norm.device
         self.device = dev
         self.paged: PagedKVCache | None = None
+        if self.kv_bits not in (8, 16) or (self.kv_bits == 8 and self.page_size <= 0):
+            raise ValueError("kv_bits is 16, or 8 with a paged cache (page_size > 0)")
+        if self.kv_budget and (self.kv_bits != 8 or not self.kv_sinks + self.kv_recent <= self.kv_budget < self.max_seq):
+            raise ValueError("kv_budget needs kv_bits=8, room for kv_sinks + kv_recent positions and fewer than max_seq")
         if self.page_size > 0:
             per_seq = -(-self.max_seq // self.page_size)
-            self.paged = PagedKVCache(layers=cfg.layers, num_pages=self.kv_pages or self.batch * per_seq,
-                                      page_size=self.page_size, kv_heads=cfg.kv_heads, head_dim=cfg.head_dim,
-                                      max_seqs=self.batch, max_pages_per_seq=per_seq, device=dev)
+            pool = dict(layers=cfg.layers, num_pages=self.kv_pages or self.batch * per_seq, page_size=self.page_size,
+                        kv_heads=cfg.kv_heads, head_dim=cfg.head_dim, max_seqs=self.batch, max_pages_per_seq=per_seq,
+                        device=dev)
+            self.paged = PagedKVCacheQ8(block=self.kv_block, keep_weights=self.kv_budget > 0, **pool) \
+                if self.kv_bits == 8 else PagedKVCache(**pool)
             self.k_cache, self.v_cache = self.paged.k, self.paged.v
             # the decode step's new K/V rows, written here by the RoPE kernel (position stride 0) and then
             # copied into their pages
@@ -152,6 +170,10 @@ class Qwen3Runner:
             self.v_cache = [torch.zeros(shape, dtype=torch.float16, device=dev) for _ in range(cfg.layers)]
         self.inv_freq = inv_freq(cfg).to(dev)
         self.positions = torch.zeros(self.batch, dtype=torch.int32, device=dev)
+        # the cache row of the next token: its position, until an eviction moves rows up
+        self.slots = torch.zeros(self.batch, dtype=torch.int32, device=dev)
+        # as the host knows them: tokens of each sequence so far, and rows of the cache they have
+        self.length = self.cached = 0
         self.token_index = torch.zeros(1, dtype=torch.int32, device=dev)
         self.next_token = torch.zeros(self.batch, dtype=torch.int64, device=dev)
         self.done = torch.zeros(self.batch, dtype=torch.int32, device=dev)
@@ -177,6 +199,11 @@ class Qwen3Runner:
         self.attn_workspace = torch.empty(max(ws, 1), dtype=torch.float32, device=dev)
         self.fused_workspace = kernels.attn_decode_fused_workspace(self.batch, cfg.heads, cfg.kv_heads, cfg.head_dim,
                                                                    self.decode_splits, dev)
+        if self.kv_bits == 8:
+            need = kernels.attn_decode_q8_workspace(self.paged.layer(0), self.paged.block_table, batch=self.batch,
+                                                    n_heads=cfg.heads, max_len=self._max_cached(),
+                                                    with_weights=self.kv_budget > 0)
+            self.q8_workspace = torch.empty(max(need, 1), dtype=torch.float32, device=dev)
         self.decode = self._alloc(self.batch)
         self._prefill_buffers: tuple[int, _Buffers] | None = None
         self._graph: torch.cuda.CUDAGraph | None = None
@@ -241,6 +268,9 @@ class Qwen3Runner:
         attention.  Prefill (positions start at 0): RoPE into a contiguous prompt cache, causal attention
         over it, then the prompt's rows are copied into their pages."""
         cfg, lw, pool = self.cfg, self.weights.layers[i], self.paged
+        if self.kv_bits == 8:
+            self._attention_q8(i, b, tokens_per_seq, decode)
+            return
         nk, d, bt = cfg.kv_heads, cfg.head_dim, pool.block_table
         if decode:
             ks = self.k_stage.as_strided((self.batch, self.max_seq, nk, d), (nk * d, 0, d, 1))
@@ -263,6 +293,63 @@ class Qwen3Runner:
         else:
             kernels.attn_prefill(b.qr, ks, vs, self.positions, batch=self.batch, tokens=tokens_per_seq,
                                  n_heads=cfg.heads, n_kv=nk, head_dim=d, out=b.attn)
+
+    def _max_cached(self) -> int:
+        """Bound on a sequence's rows in the 8-bit cache during decoding."""
+        return min(self.max_seq, self.kv_budget + self.page_size) if self.kv_budget else self.max_seq
+
+    def _attention_q8(self, i: int, b: _Buffers, tokens_per_seq: int, decode: bool) -> None:
+        """_attention over the 8-bit pool: RoPE (by position) into staging rows, quantized append (by cache row), then
+        attention over the cache; with a budget also the weight each key received."""
+        cfg, lw, pool = self.cfg, self.weights.layers[i], self.paged
+        nh, nk, d, bt, pages = cfg.heads, cfg.kv_heads, cfg.head_dim, pool.block_table, pool.layer(i)
+        weights = pool.weights[i] if pool.weights else None
+        if decode:
+            ks = self.k_stage.as_strided((self.batch, self.max_seq, nk, d), (nk * d, 0, d, 1))
+            vs = self.v_stage.as_strided((self.batch, self.max_seq, nk, d), (nk * d, 0, d, 1))
+            new = [s.view(self.batch, 1, nk, d) for s in (self.k_stage, self.v_stage)]
+        else:
+            done = self.length  # the staging rows are addressed by position
+            ks = torch.empty(self.batch, done + tokens_per_seq, nk, d, dtype=torch.float16, device=self.device)
+            vs = torch.empty_like(ks)
+            new = [s[:, done:] for s in (ks, vs)]
+        kernels.qk_norm_rope_cache(b.q, b.k, b.v, lw.q_norm, lw.k_norm, ks, vs, self.positions, self.inv_freq,
+                                   batch=self.batch, tokens=tokens_per_seq, n_heads=nh, n_kv=nk, head_dim=d, eps=cfg.eps,
+                                   q_out=b.qr)
+        kernels.kv_cache_write_q8(pages, new[0], new[1], self.slots, bt)
+        if decode:
+            kernels.attn_decode_q8(b.qr.view(self.batch, nh, d), pages, self.slots, bt, max_len=self._max_cached(),
+                                   weights=weights, weights_out=weights, workspace=self.q8_workspace,
+                                   out=b.attn.view(self.batch, nh, d))
+            return
+        q = b.qr.view(self.batch, tokens_per_seq, nh, d)
+        out = b.attn.view(self.batch, tokens_per_seq, nh, d)
+        end = self.cached + tokens_per_seq
+        if weights is None:
+            kernels.attn_prefill_q8(q, pages, self.slots, bt, max_len=end, out=out)
+            return
+        _, lse = kernels.attn_prefill_q8(q, pages, self.slots, bt, max_len=end, return_lse=True, out=out)
+        w = min(self.kv_window, tokens_per_seq)
+        last = self.slots + (tokens_per_seq - w)
+        if self.cached:  # keys of an earlier prompt keep what they had; this prompt's start from its own queries
+            weights[:, :, self.cached:end] = 0.0
+        else:
+            weights[:, :, :end] = 0.0
+        kernels.attn_key_weights_q8(q[:, tokens_per_seq - w:], lse[:, :, tokens_per_seq - w:].contiguous(), pages, last, bt,
+                                    max_len=end, weights=weights, weights_out=weights)
+
+    def _evict(self) -> None:
+        """Cuts every sequence to kv_budget rows of the 8-bit cache, in place, and returns the pages that frees."""
+        pool, cfg = self.paged, self.cfg
+        left = torch.empty_like(self.slots)
+        for i in range(cfg.layers):
+            kernels.kv_cache_evict_q8(pool.layer(i), pool.weights[i], self.slots, pool.block_table, keep=self.kv_budget,
+                                      sinks=self.kv_sinks, recent=self.kv_recent, new_lengths=left)
+        self.slots.copy_(left)
+        self.cached = min(self.cached, self.kv_budget)
+        for s in range(self.batch):
+            pool.shrink(s, self._max_cached())
+            pool.reserve(s, self._max_cached())
 
     def _reserve_pages(self, positions: int) -> None:
         """Every sequence gets pages for `positions` positions, handed out round-robin (sequence b's pages
@@ -288,8 +375,11 @@ class Qwen3Runner:
 
     # ------------------------------------------------------------- forward
     def prefill(self, ids: torch.Tensor, *, layer_outputs: list[torch.Tensor] | None = None,
-                inject: tuple[torch.Tensor, torch.Tensor] | None = None) -> None:
+                inject: tuple[torch.Tensor, torch.Tensor] | None = None, append: bool = False) -> None:
         """Runs the prompt ids [batch, T] through all layers and selects the first new token.
+
+        append (8-bit cache): the prompt continues the cached conversation instead of starting a new one.  The token
+        that the last step selected but did not feed back belongs at its front if it is to be part of the history.
 
         inject = (positions int64 [S], rows fp16 [batch, S, hidden]): after the token embedding, the
         rows at those prompt positions are replaced (Qwen3-ASR's audio features at the audio placeholder
@@ -300,9 +390,19 @@ class Qwen3Runner:
         tokens = ids.shape[1]
         if tokens > self.max_seq:
             raise ValueError(f"prompt of {tokens} tokens exceeds max_seq {self.max_seq}")
-        if self.paged is not None:
+        if append and self.kv_bits != 8:
+            raise ValueError("prefill(append=True) needs the 8-bit cache (kv_bits=8)")
+        if not append:
+            self.length = self.cached = 0
+            self.positions.zero_()
+            self.slots.zero_()
+        elif self.cached + tokens > self.max_seq:
+            raise ValueError(f"prompt of {tokens} tokens on {self.cached} cached exceeds max_seq {self.max_seq}")
+        if append:
+            for s in range(self.batch):
+                self.paged.reserve(s, min(self.max_seq, self.cached + tokens + self.max_new_tokens))
+        elif self.paged is not None:
             self._reserve_pages(min(self.max_seq, tokens + self.max_new_tokens))
-        self.positions.zero_()
         self.token_index.zero_()
         self.generated_length.zero_()
         self.stopped.zero_()
@@ -321,11 +421,28 @@ class Qwen3Runner:
                 layer_outputs.append(b.h.clone())
         last = b.h.view(self.batch, tokens, cfg.hidden)[:, -1, :].contiguous()
         self._head(last, b)
-        self.positions.fill_(tokens)
+        self.length += tokens
+        self.cached += tokens
+        self.positions.fill_(self.length)
+        self.slots.fill_(self.cached)
         self.token_index.fill_(1)
+        self._make_room()
 
     def decode_step(self, *, layer_outputs: list[torch.Tensor] | None = None) -> None:
         """One greedy token for every sequence: embeds next_token, appends the new one."""
+        self._make_room()
+        self._decode_step(layer_outputs)
+        self._count_step()
+
+    def _make_room(self) -> None:
+        if self.kv_budget and self.cached >= self._max_cached():
+            self._evict()
+
+    def _count_step(self) -> None:
+        self.length += 1
+        self.cached += 1
+
+    def _decode_step(self, layer_outputs: list[torch.Tensor] | None = None) -> None:
         cfg, b = self.cfg, self.decode
         self._embed(self.next_token, b.h)
         for i in range(cfg.layers):
@@ -334,10 +451,12 @@ class Qwen3Runner:
                 layer_outputs.append(b.h.clone())
         self._head(b.h, b)
         kernels.advance_positions(self.positions, self.token_index)
+        if self.kv_bits == 8:
+            kernels.advance_positions(self.slots)
 
     def _step_state(self) -> list[torch.Tensor]:
-        return [self.positions, self.token_index, self.next_token, self.done, self.generated, self.generated_length,
-                self.stopped]
+        return [self.positions, self.slots, self.token_index, self.next_token, self.done, self.generated,
+                self.generated_length, self.stopped, *(self.paged.weights if self.kv_budget else [])]
 
     def capture(self) -> None:
         """Captures decode_step in a CUDA graph (replayed by step()).
@@ -350,21 +469,23 @@ class Qwen3Runner:
         side = torch.cuda.Stream(device=self.device)
         side.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(side):
-            self.decode_step()  # warm up every launch path outside capture
+            self._decode_step()  # warm up every launch path outside capture
         torch.cuda.current_stream(self.device).wait_stream(side)
         for t, v in zip(self._step_state(), saved):
             t.copy_(v)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=side):
-            self.decode_step()
+            self._decode_step()
         self._graph = graph
         for t, v in zip(self._step_state(), saved):
             t.copy_(v)
 
     def step(self) -> None:
+        self._make_room()
         if self._graph is None:
             self.capture()
         self._graph.replay()
+        self._count_step()
 
     def generate(self, prompt: torch.Tensor, max_new_tokens: int) -> torch.Tensor:
         """Prefill + (max_new_tokens - 1) graph-replayed decode steps; returns [batch, max_new_tokens]."""
