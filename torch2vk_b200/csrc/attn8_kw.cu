@@ -11,6 +11,8 @@
 #include <cooperative_groups.h>
 #include <cudaTypedefs.h>
 
+#include <type_traits>
+
 #include "kv8.cuh"
 #include "umma.cuh"
 
@@ -174,35 +176,39 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
                     const int64_t ahead = (key - p0 - static_cast<int64_t>(q) * TT) * group;
                     const bool masked = __any_sync(0xffffffffu, ahead > 0);
                     const int from = static_cast<int>(ahead < 0 ? 0 : (ahead > 128 ? 128 : ahead));
-                    float tile = 0.0f;
-                    uint32_t s[2][32];
-                    tmem_ld32(at, s[0]);
+                    // (the columns in view and the others apart: a select per column would be half of the instructions)
+                    const auto columns = [&](auto hide) -> float {
+                        float tile = 0.0f;
+                        uint32_t s[2][32];
+                        tmem_ld32(at, s[0]);
 #pragma unroll
-                    for (int c4 = 0; c4 < 4; ++c4) {
-                        tmem_ld_wait32(s[c4 & 1]);
-                        if (c4 < 3) tmem_ld32(at + 32 * (c4 + 1), s[(c4 + 1) & 1]);
-                        if (c4 == 3) {  // the buffer is read
-                            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&s_free[buf]);
-                        }
-                        uint64_t sum[2];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const ulonglong2 two = nl[8 * c4 + (i >> 1)];
-                            const uint32_t *v = s[c4 & 1] + 2 * i;
-                            float2 y = f32x2_parts(f32x2_fma(f32x2(__uint_as_float(v[0]), __uint_as_float(v[1])), kk, i & 1 ? two.y : two.x));
-                            if (masked) {
-                                y.x = 32 * c4 + 2 * i < from ? -INFINITY : y.x;
-                                y.y = 32 * c4 + 2 * i + 1 < from ? -INFINITY : y.y;
+                        for (int c4 = 0; c4 < 4; ++c4) {
+                            tmem_ld_wait32(s[c4 & 1]);
+                            if (c4 < 3) tmem_ld32(at + 32 * (c4 + 1), s[(c4 + 1) & 1]);
+                            if (c4 == 3) {  // the buffer is read
+                                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(&s_free[buf]);
                             }
-                            const uint64_t e = f32x2(ex2(y.x), ex2(y.y));
-                            sum[i & 1] = i < 2 ? e : f32x2_add(sum[i & 1], e);
+                            uint64_t sum[2];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const ulonglong2 two = nl[8 * c4 + (i >> 1)];
+                                const uint32_t *v = s[c4 & 1] + 2 * i;
+                                float2 y = f32x2_parts(f32x2_fma(f32x2(__uint_as_float(v[0]), __uint_as_float(v[1])), kk, i & 1 ? two.y : two.x));
+                                if (hide) {
+                                    y.x = 32 * c4 + 2 * i < from ? -INFINITY : y.x;
+                                    y.y = 32 * c4 + 2 * i + 1 < from ? -INFINITY : y.y;
+                                }
+                                const uint64_t e = f32x2(ex2(y.x), ex2(y.y));
+                                sum[i & 1] = i < 2 ? e : f32x2_add(sum[i & 1], e);
+                            }
+                            const float2 both = f32x2_parts(f32x2_add(sum[0], sum[1]));
+                            tile += both.x + both.y;
                         }
-                        const float2 both = f32x2_parts(f32x2_add(sum[0], sum[1]));
-                        tile += both.x + both.y;
-                    }
-                    weight += tile;
+                        return tile;
+                    };
+                    weight += masked ? columns(std::true_type{}) : columns(std::false_type{});
                 }
                 if (C > 1) {  // one key tile: the shares are summed below, in their order
                     sums[tid] = weight;
