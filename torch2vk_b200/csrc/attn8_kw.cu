@@ -7,7 +7,8 @@
 // Keys are the rows, so a thread owns a key: its sum needs no exchange, its K scale is a register, and the columns'
 // log-sum-exps are read from shared memory by all lanes alike.  Sums are per 32 columns, per tile, then over tiles, in
 // fp32 and in a fixed order.  What bounds it: the 2^ unit, one per (head, query, key); two CTAs share an SM, so that one's
-// other instructions run under the other's.
+// other instructions run under the other's (8192 queries of 32 heads on 8: 361 us, 0.66 of that unit's rate of 16 a clock
+// and SM; with eight warps of half the columns each 369).
 #include <cooperative_groups.h>
 #include <cudaTypedefs.h>
 
@@ -344,8 +345,9 @@ extern "C" int t2c_attn_key_weights_q8(const t2c_q8_pages *pages, const void *q,
     // Where few query tiles stream past a key tile, a CTA takes several key tiles, as many as make one wave of two CTAs per
     // SM (the next tile's codes arrive under this one).  Where many do, one, and a cluster of up to 8 CTAs shares out the
     // query tiles of the first keys, which every query sees, until the longest share is under 3/4 of the mean of an SM's
-    // slot; 32 query tiles a CTA at least, which its beginning costs about 4 of (6000 queries of 16 heads on 8: 165 us
-    // alone, 124 in pairs, 147 in fours; 4096 queries of 16 heads of 64 on 16: 57, 66).
+    // slot; 32 query tiles a CTA at least, which its beginning costs about 4 of (6000 queries of 16 heads on 8: 150 us
+    // alone, 116 in pairs, 139 in fours; 4096 queries of 16 heads of 64 on 16: 53, 62, 84).  32 queries on 2 x 16007
+    // positions: 7 key tiles a CTA 27 us, one 39.
     const int64_t nq = (T + tokens - 1) / tokens, tiles = (max_len + 127) / 128, units = B * a.pg.n_kv, slots = 2 * sm_count();
     int64_t per = nq >= 8 ? 1 : (units * tiles + slots - 1) / slots;
     per = per > 32 ? 32 : per;
