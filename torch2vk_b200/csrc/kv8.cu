@@ -182,6 +182,7 @@ __global__ void __launch_bounds__(128) kv8_write_kernel(KvPages pg, const __half
     if (!earlier || slice >= p0 || s == s_old) return;
     // the rows already there, at the grown scale
     constexpr int kOldUnits = (16 * D / 16 + 31) / 32;
+    const float2 ratio = kv8_ratio(s_old, s, inv);
 #pragma unroll 1
     for (int i = 0; i < kOldUnits; ++i) {
         const int u = i * 32 + lane;
@@ -191,13 +192,7 @@ __global__ void __launch_bounds__(128) kv8_write_kernel(KvPages pg, const __half
         uint4 codes = *at;
         uint32_t *w = reinterpret_cast<uint32_t *>(&codes);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t c[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                c[e] = kv8_code(static_cast<float>(static_cast<int8_t>(w[j] >> (8 * e))) * s_old, s, inv);
-            w[j] = ok ? kv8_pack4(c[0], c[1], c[2], c[3]) : 0u;
-        }
+        for (int j = 0; j < 4; ++j) w[j] = ok ? kv8_recode(w[j], ratio) : 0u;
         *at = codes;
     }
 }
@@ -423,14 +418,13 @@ template <int D, bool IN_PLACE>
 __global__ void __launch_bounds__(mv_threads(IN_PLACE), IN_PLACE ? 2 : 5) kv8_move_kernel(
     KvPages pg, const float *weights, int64_t w_sb, int64_t w_sh, const int32_t *__restrict__ lengths,
     const int32_t *__restrict__ table, int64_t t_stride, int64_t capacity, const int32_t *__restrict__ out_table,
-    int64_t o_stride, int keep, int chunks, float *weights_out, int64_t wo_sb, int64_t wo_sh,
+    int64_t o_stride, int keep, float *weights_out, int64_t wo_sb, int64_t wo_sh,
     const int32_t *__restrict__ kept) {
     constexpr int kWarps = mv_threads(IN_PLACE) / 32, kRowsCta = mv_rows(IN_PLACE);
     __shared__ uint32_t slice_top[2][kWarps];
     cg::cluster_group cluster = cg::this_cluster();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int unit = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
-    const int head = unit % pg.n_kv, b = unit / pg.n_kv;
+    const int chunks = gridDim.x, chunk = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
     pdl_wait();
     pdl_trigger();
     int left = keep;  // to other pages the -1 of `kept` ends the rows
@@ -476,20 +470,20 @@ __global__ void __launch_bounds__(mv_threads(IN_PLACE), IN_PLACE ? 2 : 5) kv8_mo
     fetch(0);
     for (int r0 = 0, round = 0; r0 < (IN_PLACE ? left : 1); r0 += step, ++round) {
         const int row0 = r0 + chunk * kRowsCta + 16 * slice_of, my_row = row0 + (lane & 15);
-        float s_row[kUnits], top = 0.0f;
+        float top = 0.0f;
         uint4 q[kUnits];
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
-            s_row[i] = __shfl_sync(0xffffffffu, s_src, (i * 32 + lane) / kPerRow);
+            const float s_row = __shfl_sync(0xffffffffu, s_src, (i * 32 + lane) / kPerRow);
             q[i] = x[i];
-            uint32_t m = kv8_absmax(q[i].x, 0);
-            m = kv8_absmax(q[i].y, m);
-            m = kv8_absmax(q[i].z, m);
-            m = kv8_absmax(q[i].w, m);
-            const float mag = static_cast<float>(max(m >> 16, m & 0xffffu)) * s_row[i];
-            top = s_row[i] != s_row[i] ? INFINITY : fmaxf(top, mag);
+            uint32_t most = 0, least = 0;
+            kv8_extremes(q[i].x, most, least);
+            kv8_extremes(q[i].y, most, least);
+            kv8_extremes(q[i].z, most, least);
+            kv8_extremes(q[i].w, most, least);
+            top = s_row != s_row ? INFINITY : fmaxf(top, static_cast<float>(kv8_largest(most, least)) * s_row);
         }
-        const float w_row = w_val;
+        const float w_row = w_val, s_mine = s_src;
         const int mine = rows;
         const uint32_t top_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
         uint32_t *tops = slice_top[round & 1];
@@ -512,21 +506,15 @@ __global__ void __launch_bounds__(mv_threads(IN_PLACE), IN_PLACE ? 2 : 5) kv8_mo
         const int page = kv8_page(pg, bo, row0);
         if (page < 0) continue;
         if (lane == 0 && warp == w0) scales[kv8_scale_offset(pg, page, head, row0)] = s_half;
-        int8_t *dst = codes + kv8_row_offset(pg, page, head, row0);
+        int8_t *dst = codes + kv8_row_offset(pg, page, head, row0) + lane / kPerRow * pg.row_stride + lane % kPerRow * 16;
+        const float2 own = kv8_ratio(s_mine, s, inv);
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
-            const int u = i * 32 + lane, row = u / kPerRow;
-            if (row >= mine) continue;
-            uint32_t *c4 = reinterpret_cast<uint32_t *>(&q[i]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t c[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    c[e] = kv8_code(static_cast<float>(static_cast<int8_t>(c4[j] >> (8 * e))) * s_row[i], s, inv);
-                c4[j] = ok ? kv8_pack4(c[0], c[1], c[2], c[3]) : 0u;
-            }
-            *reinterpret_cast<uint4 *>(dst + row * pg.row_stride + (u % kPerRow) * 16) = q[i];
+            const int row = (i * 32 + lane) / kPerRow;
+            const float2 ratio = make_float2(__shfl_sync(0xffffffffu, own.x, row), __shfl_sync(0xffffffffu, own.y, row));
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (ok) v = make_uint4(kv8_recode(q[i].x, ratio), kv8_recode(q[i].y, ratio), kv8_recode(q[i].z, ratio), kv8_recode(q[i].w, ratio));
+            if (row < mine) *reinterpret_cast<uint4 *>(dst + i * (32 / kPerRow) * pg.row_stride) = v;
         }
         if (!is_v && lane < mine) wo[my_row] = w_row;
     }
@@ -624,7 +612,7 @@ extern "C" int t2c_kv_cache_evict_q8(const t2c_q8_pages *pages, const float *wei
         chunks = 1;
         while (chunks < 8 && chunks < full && heads * chunks < 2 * sm_count()) chunks *= 2;
     }
-    if (heads * cluster > INT32_MAX || heads * chunks > INT32_MAX) return set_error(T2C_EINVAL, "kv_cache_evict_q8: bad shape");
+    if (heads * cluster > INT32_MAX || B > 65535) return set_error(T2C_EINVAL, "kv_cache_evict_q8: bad shape");
     rc = kv8_configure(kv8_select_kernel, kEvCache * 4, 6, "kv_cache_evict_q8");
     if (rc == T2C_OK)
         rc = kv8_launch("kv_cache_evict_q8", kv8_select_kernel, dim3(static_cast<unsigned>(heads * cluster)), dim3(kEvThreads),
@@ -634,8 +622,9 @@ extern "C" int t2c_kv_cache_evict_q8(const t2c_q8_pages *pages, const float *wei
     const bool wide = pages->head_dim == 128;
     const auto kern = in_place ? (wide ? kv8_move_kernel<128, true> : kv8_move_kernel<64, true>)
                                : (wide ? kv8_move_kernel<128, false> : kv8_move_kernel<64, false>);
-    return kv8_launch("kv_cache_evict_q8 move", kern, dim3(static_cast<unsigned>(heads * chunks)), dim3(mv_threads(in_place)), 0,
+    return kv8_launch("kv_cache_evict_q8 move", kern,
+                      dim3(static_cast<unsigned>(chunks), static_cast<unsigned>(pg.n_kv), static_cast<unsigned>(B)), dim3(mv_threads(in_place)), 0,
                       in_place ? static_cast<unsigned>(chunks) : 1u, as_stream(stream), pg, weights, w_sb, w_sh, lengths,
-                      block_table, bt_stride, capacity, out_table, ot_stride, static_cast<int>(keep), static_cast<int>(chunks),
+                      block_table, bt_stride, capacity, out_table, ot_stride, static_cast<int>(keep),
                       weights_out, wo_sb, wo_sh, kept);
 }

@@ -11,6 +11,7 @@
 #include <math.h>
 
 #include "common.cuh"
+#include "umma.cuh"
 
 namespace t2c {
 
@@ -98,11 +99,44 @@ __device__ __forceinline__ uint32_t kv8_pack4(uint32_t a, uint32_t b, uint32_t c
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// Largest |code| of a word's four codes, folded into a running u16x2 maximum.
-__device__ __forceinline__ uint32_t kv8_absmax(uint32_t w, uint32_t best) {
-    const uint32_t sign = (w >> 7) & 0x01010101u;
-    const uint32_t mag = (w ^ (sign * 0xffu)) + sign;  // codes are >= -127: no byte overflows
-    return __vmaxu2(best, __vmaxu2(mag & 0x00ff00ffu, (mag >> 8) & 0x00ff00ffu));
+// Largest and least code of a word's four, folded into running s16x2 extremes.
+__device__ __forceinline__ void kv8_extremes(uint32_t w, uint32_t &most, uint32_t &least) {
+    uint32_t even, odd;  // bytes 0, 2 and 1, 3, sign-extended
+    asm("prmt.b32 %0, %1, 0, 0xa280;" : "=r"(even) : "r"(w));
+    asm("prmt.b32 %0, %1, 0, 0xb391;" : "=r"(odd) : "r"(w));
+    most = __vimax3_s16x2(even, odd, most);
+    least = __vimin3_s16x2(even, odd, least);
+}
+
+__device__ __forceinline__ int kv8_largest(uint32_t most, uint32_t least) {
+    const auto half = [](uint32_t v, int h) { return static_cast<int>(static_cast<int16_t>(v >> (16 * h))); };
+    return max(max(half(most, 0), half(most, 1)), -min(half(least, 0), half(least, 1)));
+}
+
+// s_old / s_new in two floats, high + low to 2^-46 of it.  rint(code * (high + low)), the small product first, is then
+// the correctly rounded code * s_old / s_new: that is within 2^-23 of the quotient, whose distance from a tie is zero or
+// at least 2^-19 of it (both scales have 11 bits, the code 7), and exact where it is a tie.
+__device__ __forceinline__ float2 kv8_ratio(float s_old, float s_new, float inv_new) {
+    const float high = __fdiv_rn(s_old, s_new);
+    return make_float2(high, fmaf(-high, s_new, s_old) * inv_new);
+}
+
+// A word's four codes at another scale.  (Code + 128 in the mantissa of 2^23 becomes a float without a conversion
+// instruction, two values an instruction from there on: 5 instructions a code in all, where conversion, product, quotient
+// and its correction took 9 and the move's time was theirs: 26 us, now see there.)
+__device__ __forceinline__ uint32_t kv8_recode(uint32_t w, float2 ratio) {
+    const uint32_t u = w ^ 0x80808080u;
+    const uint64_t bias = f32x2(-8388736.0f, -8388736.0f), round = f32x2(12582912.0f, 12582912.0f);
+    const uint64_t high = f32x2(ratio.x, ratio.x), low = f32x2(ratio.y, ratio.y);
+    uint64_t c[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint64_t v = f32x2_add(f32x2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + 2 * i)),
+                                           __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441 + 2 * i))), bias);
+        c[i] = f32x2_add(f32x2_fma(v, high, f32x2_mul(v, low)), round);
+    }
+    const float2 a = f32x2_parts(c[0]), b = f32x2_parts(c[1]);
+    return kv8_pack4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
 }
 
 template <typename Kernel, typename... Args>
