@@ -524,14 +524,15 @@ __global__ void __launch_bounds__(kJoinThreads) attn8_join_kernel(const __grid_c
     const int head = blockIdx.y, b = blockIdx.z, group = a.NH / a.pg.n_kv;
     const bool is_out = static_cast<int>(blockIdx.x) < group;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    pdl_wait();
-    pdl_trigger();
     const int2 *ctas = p.unit_ctas + (static_cast<int64_t>(b) * a.pg.n_kv + head) * p.head_chunks;
     const int first = is_out ? blockIdx.x : 0, last = is_out ? first + 1 : group;
-    const int2 own = ctas[first >> 3];
     const int64_t n = min(static_cast<int64_t>(a.positions[b]) + 1, a.max_len);
     const int64_t w0 = (static_cast<int64_t>(blockIdx.x) - group) * kJoinKeys;
-    if (is_out ? own.x == own.y : w0 >= n) return;  // a unit of one CTA is written
+    if (!is_out && w0 >= n) return;
+    pdl_wait();  // positions were there before the kernel whose parts are joined
+    pdl_trigger();
+    const int2 own = ctas[first >> 3];
+    if (is_out && own.x == own.y) return;  // a unit of one CTA is written
     // part i of a unit whose tiles begin in CTA c0: that CTA's last one, then the others' first
     const auto part_of = [&](int c0, int i) { return p.parts + (2 * static_cast<int64_t>(c0 + i) + (i == 0 ? 1 : 0)) * kPart; };
 

@@ -533,11 +533,9 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
 template <int D>
 __global__ void __launch_bounds__(256) attn8_prefill_join_kernel(const __grid_constant__ PrefillArgs a) {
     const int lane = threadIdx.x & 31;
-    const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    pdl_wait();
-    pdl_trigger();
-    if (w >= static_cast<int64_t>(a.B) * a.T * a.NH) return;
-    const int h = static_cast<int>(w % a.NH), t = static_cast<int>(w / a.NH % a.T), b = static_cast<int>(w / a.NH / a.T);
+    const unsigned w = blockIdx.x * 8u + (threadIdx.x >> 5), tokens = w / static_cast<unsigned>(a.NH);
+    if (tokens >= static_cast<unsigned>(a.B) * a.T) return;
+    const int h = static_cast<int>(w % a.NH), t = static_cast<int>(tokens % a.T), b = static_cast<int>(tokens / a.T);
     const int group = a.NH / a.pg.n_kv, TT = kPRows / group, head = h / group;
     const int pair = t / (2 * TT), in_pair = t % (2 * TT);
     const int row = in_pair / TT * 128 + in_pair % TT * group + h % group;
@@ -547,6 +545,9 @@ __global__ void __launch_bounds__(256) attn8_prefill_join_kernel(const __grid_co
     const int per = (tiles + a.splits - 1) / a.splits, used = per > 0 ? (tiles + per - 1) / per : 0;
     const float *base = a.parts + ((static_cast<int64_t>(b) * a.pg.n_kv + head) * a.pairs + pair) * a.splits * (256 * (D + 2));
     const bool seen = p0 + t >= 0;
+    // positions were there before the kernel whose parts are joined: all of the above runs under that one's end
+    pdl_wait();
+    pdl_trigger();
     constexpr int kPer = D / 32, kAhead = 8;
     constexpr int64_t kPart = 256 * (D + 2);
     // lane s (and s + 32): the statistics of split s; the first rows of O come beside them
@@ -661,7 +662,7 @@ extern "C" int t2c_attn_prefill_q8(const t2c_q8_pages *pages, const void *q, int
     a.scale_log2 = scale * 1.4426950408889634f;
     a.parts = workspace;
     const int64_t ctas = B * a.pg.n_kv * plan.pairs * plan.splits, rows = B * T * NH;
-    if (ctas > INT32_MAX) return set_error(T2C_EINVAL, "attn_prefill_q8: bad shape");
+    if (ctas > INT32_MAX || rows > UINT32_MAX - 8) return set_error(T2C_EINVAL, "attn_prefill_q8: bad shape");
     const cudaStream_t s = as_stream(stream);
     const auto kern = D == 128 ? attn8_prefill_kernel<128> : attn8_prefill_kernel<64>;
     const int smem = D == 128 ? PrefillShape<128>::kSmem : PrefillShape<64>::kSmem;
