@@ -2,6 +2,8 @@
 #include <cooperative_groups.h>
 #include <cudaTypedefs.h>
 
+#include <type_traits>
+
 #include "kv8.cuh"
 
 namespace cg = cooperative_groups;
@@ -508,26 +510,28 @@ __global__ void __launch_bounds__(kDThreads, 4) attn8_decode_kernel(const __grid
     if (C > 1) cluster.sync();  // no CTA leaves while another may read its shared memory
 }
 
-// Joins the runs.  Blocks 0 .. group - 1 of a (sequence, KV head): one head's output, the parts dealt to the block's
-// quarters; the others: the weights of 4096 keys each.  What does not depend on the softmax statistics is loaded
+// Joins the runs.  The first blocks of a (sequence, KV head): the output of one head, its parts dealt to the block's
+// quarters, or of a head for each quarter; the others: the weights of 4096 keys each.  What does not depend on the softmax statistics is loaded
 // beside them: a block is three dependent trips to memory long (32801 positions of one sequence: 7 us; 32 sequences of up to
 // 6007 with the weights: 14 us, 8 MB).
 constexpr int kJoinThreads = 512;
 constexpr int kJoinKeys = 4096;
 
-template <int D>
+template <int D, bool ALONE>
 __global__ void __launch_bounds__(kJoinThreads) attn8_join_kernel(const __grid_constant__ DecodeArgs p) {
-    extern __shared__ float factor[];  // [parts] of the block's head
-    __shared__ float ref[128], sum, quarter[kJoinThreads];
+    constexpr int kShare = kJoinThreads / D, kHeads = ALONE ? 1 : kShare, kAhead = 4;
+    extern __shared__ float factor[];  // [parts] of the block's heads
+    __shared__ float ref[128], sum[kShare], quarter[kJoinThreads];
     constexpr int kPart = DecodeShape<D>::kPart;
     const AttnArgs &a = p.a;
     const int head = blockIdx.y, b = blockIdx.z, group = a.NH / a.pg.n_kv;
-    const bool is_out = static_cast<int>(blockIdx.x) < group;
+    const int out_blocks = (group + kHeads - 1) / kHeads;
+    const bool is_out = static_cast<int>(blockIdx.x) < out_blocks;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int2 *ctas = p.unit_ctas + (static_cast<int64_t>(b) * a.pg.n_kv + head) * p.head_chunks;
-    const int first = is_out ? blockIdx.x : 0, last = is_out ? first + 1 : group;
+    const int first = is_out ? blockIdx.x * kHeads : 0, last = is_out ? min(first + kHeads, group) : group;
     const int64_t n = min(static_cast<int64_t>(a.positions[b]) + 1, a.max_len);
-    const int64_t w0 = (static_cast<int64_t>(blockIdx.x) - group) * kJoinKeys;
+    const int64_t w0 = (static_cast<int64_t>(blockIdx.x) - out_blocks) * kJoinKeys;
     if (!is_out && w0 >= n) return;
     pdl_wait();  // positions were there before the kernel whose parts are joined
     pdl_trigger();
@@ -536,13 +540,15 @@ __global__ void __launch_bounds__(kJoinThreads) attn8_join_kernel(const __grid_c
     // part i of a unit whose tiles begin in CTA c0: that CTA's last one, then the others' first
     const auto part_of = [&](int c0, int i) { return p.parts + (2 * static_cast<int64_t>(c0 + i) + (i == 0 ? 1 : 0)) * kPart; };
 
-    constexpr int kShare = kJoinThreads / D, kAhead = 4;
+    // a quarter: every kShare-th part of the block's head, or all parts of its own head
     const int d = threadIdx.x % D, q = threadIdx.x / D, count = own.y - own.x + 1;
+    const int mine = ALONE ? first : min(first + q, group - 1), part0 = ALONE ? q : 0;
+    constexpr int step = ALONE ? kShare : 1;
     float ahead[kAhead];
     if (is_out) {
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
-            ahead[k] = q + kShare * k < count ? part_of(own.x, q + kShare * k)[(first & 7) * D + d] : 0.0f;
+            ahead[k] = part0 + step * k < count ? part_of(own.x, part0 + step * k)[(mine & 7) * D + d] : 0.0f;
     }
     for (int h = first + warp; h < last; h += kJoinThreads / 32) {
         const int2 c = ctas[h >> 3];
@@ -562,40 +568,48 @@ __global__ void __launch_bounds__(kJoinThreads) attn8_join_kernel(const __grid_c
         for (int i = lane; i < parts; i += 32) {
             const float *st = part_of(c.x, i) + 8 * D + (h & 7);
             const float f = exp2_approx((i == lane ? m0 : st[0]) - top);
-            if (is_out) factor[i] = f;
+            if (is_out) factor[(h - first) * count + i] = f;
             s = fmaf(i == lane ? l0 : st[8], f, s);
         }
         s = warp_sum(s);
         if (lane == 0) {
             ref[h] = top + log2f(s);
-            if (is_out) sum = s;
+            if (is_out) sum[h - first] = s;
         }
     }
     if (!is_out) {
         const float *xs = p.scores + ((static_cast<int64_t>(b) * a.pg.n_kv + head) * p.s_len + w0) * group;
         const int64_t at = b * p.w_sb + head * p.w_sh + w0;
         const int end = static_cast<int>(n - w0 < kJoinKeys ? n - w0 : kJoinKeys), old = static_cast<int>(n - 1 - w0);
-        if (group == 4) {  // scores of eight keys a thread, all in flight before the statistics are known
-            constexpr int kKeys = kJoinKeys / kJoinThreads;
-            float4 x[kKeys];
+        // scores of eight keys a thread, all in flight before the statistics are known
+        const auto ahead_of = [&](auto heads) {
+            constexpr int G = decltype(heads)::value, kKeys = kJoinKeys / kJoinThreads;
+            using Vec = typename std::conditional<G == 4, float4, typename std::conditional<G == 2, float2, float>::type>::type;
+            Vec x[kKeys];
             float w[kKeys];
 #pragma unroll
             for (int k = 0; k < kKeys; ++k) {
                 const int key = threadIdx.x + kJoinThreads * k;
-                if (key < end) x[k] = *reinterpret_cast<const float4 *>(xs + 4 * key);
+                if (key < end) x[k] = *reinterpret_cast<const Vec *>(xs + G * key);
                 w[k] = p.w_in && key < end && key < old ? p.w_in[at + key] : 0.0f;
             }
             __syncthreads();
-            const float4 r = make_float4(ref[0], ref[1], ref[2], ref[3]);
+            float r[G];
+#pragma unroll
+            for (int g = 0; g < G; ++g) r[g] = ref[g];
 #pragma unroll
             for (int k = 0; k < kKeys; ++k) {
                 const int key = threadIdx.x + kJoinThreads * k;
-                if (key < end)
-                    p.w_out[at + key] = w[k] + exp2_approx(x[k].x - r.x) + exp2_approx(x[k].y - r.y) +
-                                        exp2_approx(x[k].z - r.z) + exp2_approx(x[k].w - r.w);
+                const float *v = reinterpret_cast<const float *>(&x[k]);
+                float total = 0.0f;
+#pragma unroll
+                for (int g = 0; g < G; ++g) total += exp2_approx(v[g] - r[g]);
+                if (key < end) p.w_out[at + key] = w[k] + total;
             }
-            return;
-        }
+        };
+        if (group == 4) return ahead_of(std::integral_constant<int, 4>{});
+        if (group == 2) return ahead_of(std::integral_constant<int, 2>{});
+        if (group == 1) return ahead_of(std::integral_constant<int, 1>{});
         __syncthreads();
         for (int key = threadIdx.x; key < end; key += kJoinThreads) {
             const float w = key_weight(xs + static_cast<int64_t>(key) * group, ref, group);
@@ -605,18 +619,22 @@ __global__ void __launch_bounds__(kJoinThreads) attn8_join_kernel(const __grid_c
     }
     __syncthreads();
     float acc = 0.0f;
+    const float *f = factor + (ALONE ? 0 : (mine - first) * count);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-        if (q + kShare * k < count) acc = fmaf(ahead[k], factor[q + kShare * k], acc);
+        if (part0 + step * k < count) acc = fmaf(ahead[k], f[part0 + step * k], acc);
 #pragma unroll 8
-    for (int i = q + kShare * kAhead; i < count; i += kShare) acc = fmaf(part_of(own.x, i)[(first & 7) * D + d], factor[i], acc);
-    quarter[threadIdx.x] = acc;
-    __syncthreads();
-    if (threadIdx.x < D) {
+    for (int i = part0 + step * kAhead; i < count; i += step) acc = fmaf(part_of(own.x, i)[(mine & 7) * D + d], f[i], acc);
+    if (ALONE) {
+        quarter[threadIdx.x] = acc;
+        __syncthreads();
+        if (threadIdx.x >= D) return;
         for (int i = 1; i < kShare; ++i) acc += quarter[i * D + d];
-        a.out[b * a.o_sb + (head * group + first) * a.o_sh + d] = __float2half(acc / sum);
-        if (a.lse && d == 0) a.lse[static_cast<int64_t>(b) * a.NH + head * group + first] = ref[first] * 0.6931471805599453f;
+    } else if (first + q >= last) {
+        return;
     }
+    a.out[b * a.o_sb + (head * group + mine) * a.o_sh + d] = __float2half(acc / sum[mine - first]);
+    if (a.lse && d == 0) a.lse[static_cast<int64_t>(b) * a.NH + head * group + mine] = ref[mine] * 0.6931471805599453f;
 }
 
 struct DecodePlan {
@@ -711,8 +729,15 @@ extern "C" int t2c_attn_decode_q8(const t2c_q8_pages *pages, const void *q, int6
     rc = kv8_launch("attn_decode_q8", kern, grid, dim3(kDThreads), smem, clusters ? static_cast<unsigned>(p.splits) : 1u, s, k_map,
                     v_map, p);
     if (rc != T2C_OK || clusters) return rc;
-    const int64_t chunks = weights_out ? (max_len + kJoinKeys - 1) / kJoinKeys : 0;
-    return kv8_launch("attn_decode_q8 join", D == 128 ? attn8_join_kernel<128> : attn8_join_kernel<64>,
-                      dim3(static_cast<unsigned>(group + chunks), static_cast<unsigned>(a.pg.n_kv), static_cast<unsigned>(B)),
-                      dim3(kJoinThreads), static_cast<size_t>(p.ctas * 4), 1, s, p);
+    // A block per head while those fit the SMs at once, then a block for as many as it has quarters (32 sequences of up to 6007,
+    // 32 heads on 8: 49 us, with a block per head 54; 32801 positions of one 24, else 26).
+    const int64_t chunks = weights_out ? (max_len + kJoinKeys - 1) / kJoinKeys : 0, tiles = (max_len + kDTile - 1) / kDTile;
+    const int64_t parts = p.ctas < tiles ? p.ctas : tiles, quarters = kJoinThreads / D;
+    const bool alone = B * NH <= 4 * sm_count() || quarters * parts * 4 > 32768;
+    const int64_t heads = alone ? 1 : quarters;
+    const auto join = D == 128 ? (alone ? attn8_join_kernel<128, true> : attn8_join_kernel<128, false>)
+                               : (alone ? attn8_join_kernel<64, true> : attn8_join_kernel<64, false>);
+    return kv8_launch("attn_decode_q8 join", join,
+                      dim3(static_cast<unsigned>((group + heads - 1) / heads + chunks), static_cast<unsigned>(a.pg.n_kv), static_cast<unsigned>(B)),
+                      dim3(kJoinThreads), static_cast<size_t>(heads * parts * 4), 1, s, p);
 }
