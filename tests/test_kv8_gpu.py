@@ -252,6 +252,27 @@ def test_decode_matches_definition(NH, NK, dim, page, block, splits):
     check_attention(again.unsqueeze(1), None, want)
 
 
+@pytest.mark.parametrize("B,NH,NK,dim", [(22, 32, 8, 128), (110, 6, 2, 128), (28, 24, 2, 128), (12, 64, 4, 64), (40, 16, 16, 64)])
+def test_decode_many_sequences(B, NH, NK, dim):
+    """More heads than the SMs hold joining blocks: a block joins several heads; one sequence much longer than the others."""
+    from torch2vk_b200 import kernels
+
+    g = torch.Generator().manual_seed(B)
+    positions = torch.randint(-1, 700, (B,), generator=g).tolist()
+    positions[B // 2], positions[1], positions[2] = 2999, 0, -1
+    cache, table, g, _ = attention_case(B, NH, NK, dim, 64, 16, 47, B + 1)
+    pages, bt = device_pages(cache), table.cuda()
+    q = torch.randn(B, NH, dim, generator=g).half()
+    want = ref.attention(cache, q.unsqueeze(1), positions, table, dim ** -0.5)
+    before = torch.rand(B, NK, 47 * 64, generator=g)
+    lse = torch.empty(B, NH, device="cuda")
+    weights = before.cuda()
+    out = kernels.attn_decode_q8(q.cuda(), pages, i32(positions), bt, lse=lse, weights=weights, weights_out=weights)
+    clean()
+    check_attention(out.unsqueeze(1), lse.unsqueeze(-1), want)
+    check_weights(weights, before, want, positions, 1, NK)
+
+
 @pytest.mark.parametrize("length", [1000, 5003, 20011])
 def test_decode_long(length):
     """Long caches, large scores (one key draws nearly all of the weight) and a token-major pool."""
