@@ -49,9 +49,9 @@ __device__ __forceinline__ int64_t visible(const int32_t *positions, int b, int 
 // running reference per head, moved (and O, l rescaled) only when some exponent passes 14: P stays in fp16's range,
 // and its one rounding to fp16, which the tensor core asks for, is the only one before the output's.
 // What bounds it: the cache's bytes where there are many (32 sequences of up to 6007 positions, 32 heads of 128 on 8:
-// 251 MB in 55 us, 4.6 TB/s; with the weights 259 MB in 62 us), the chain of a CTA's beginning, its few tiles and the
+// 251 MB in 49 us, 5.1 TB/s; with the weights 259 MB in 58 us), the chain of a CTA's beginning, its few tiles and the
 // join where there are few (32801 positions of one sequence: 67 MB in 24 us, 7 of them the join).  Two steps of ring, four
-// CTAs an SM: with three or four steps, or eight warps, fewer CTAs fit and the 62 us became 65 to 66.
+// CTAs an SM: with three or four steps, or eight warps, fewer CTAs fit and the time with the weights was 5 % longer.
 constexpr int kDWarps = 4;
 constexpr int kDStages = 2;
 constexpr int kDThreads = 32 * kDWarps;
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(kDThreads, 4) attn8_decode_kernel(const __grid
 // Joins the runs.  The first blocks of a (sequence, KV head): the output of one head, its parts dealt to the block's
 // quarters, or of a head for each quarter; the others: the weights of 4096 keys each.  What does not depend on the softmax statistics is loaded
 // beside them: a block is three dependent trips to memory long (32801 positions of one sequence: 7 us; 32 sequences of up to
-// 6007 with the weights: 14 us, 8 MB).
+// 6007 with the weights: 10 us, 8 MB).
 constexpr int kJoinThreads = 512;
 constexpr int kJoinKeys = 4096;
 
@@ -645,7 +645,7 @@ struct DecodePlan {
 // A cluster of one 64-key tile per CTA where the longest sequence has at most 8 tiles and one wave of CTAs holds
 // them all (a group of more than 8 heads whose weights are wanted is in no one CTA's hands, so it takes the runs);
 // else runs of tiles, four CTAs per SM.  (333 positions, 16 heads on 8: 6.7 us, as runs 7.1; 8 sequences of 512, 32 heads
-// on 8: 8.1, 9.5; but 32 of them 31.7 as clusters, 20.7 as runs.)
+// on 8: 8.1, 9.5; but 32 of them 31.7 as clusters, 15.3 as runs.)
 DecodePlan decode_plan(int64_t B, int64_t NH, int64_t NK, int64_t D, int64_t max_len, int64_t splits, bool weights) {
     DecodePlan r = {};
     const int64_t group = NH / NK;

@@ -606,7 +606,7 @@ struct PrefillPlan {
 };
 
 // One CTA per SM: the keys of a pair of query tiles are split while CTAs would be missing, at least two tiles each.
-// (45 queries on 9111 keys, 32 heads on 8: 18 splits 29 us; one 170, 9 36, 36 41.  512 on 8192: two splits 105 us, one 158,
+// (45 queries on 9111 keys, 32 heads on 8: 18 splits 27 us; one 170, 9 35, 36 40.  512 on 8192: two splits 105 us, one 158,
 // four 117.  4 x 512 on up to 3500, 16 heads of 64 on 16: one split 72, two 99.)
 PrefillPlan prefill_plan(int64_t B, int64_t T, int64_t NH, int64_t NK, int64_t D, int64_t max_len, int64_t splits) {
     PrefillPlan r = {};

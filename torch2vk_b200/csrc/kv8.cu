@@ -104,7 +104,7 @@ namespace {
 // Rows before positions[b] in a block that gets new rows are rescaled when the
 // block's scale grows; the largest new magnitude of the block crosses warps
 // through shared memory.  Bound by memory for prompts (8191 tokens, 8 heads of
-// 128: 50 MB in 14 us), by its chain of position, table, scale and codes for
+// 128: 50 MB in 13 us), by its chain of position, table, scale and codes for
 // single tokens (48 sequences: 5 us).
 template <int D>
 __global__ void __launch_bounds__(128) kv8_write_kernel(KvPages pg, const __half *__restrict__ k,
@@ -160,6 +160,7 @@ __global__ void __launch_bounds__(128) kv8_write_kernel(KvPages pg, const __half
     const float s = (s_new_rows != s_new_rows || s_old != s_old) ? __int_as_float(0x7fffffff) : fmaxf(s_old, s_new_rows);
     const bool ok = s > 0.0f;  // false for NaN and for an all-zero block: codes 0
     const float inv = ok ? 1.0f / s : 0.0f;
+    const float2 one_over = kv8_ratio(1.0f, s, inv);
     if (lane == 0 && warp == w0) *sp = __float2half_rn(s);
     int8_t *dst = (is_v ? pg.v : pg.k) + kv8_row_offset(pg, page, head, slice);
 #pragma unroll
@@ -167,15 +168,14 @@ __global__ void __launch_bounds__(128) kv8_write_kernel(KvPages pg, const __half
         const int u = i * 32 + lane;
         const int64_t row = slice + u / kPerRow;
         if (row < p0 || row >= p1) continue;
-        uint32_t c[8];
+        uint64_t c[4];
         const uint32_t words[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&words[j]));
-            c[2 * j] = kv8_code(f.x, s, inv);
-            c[2 * j + 1] = kv8_code(f.y, s, inv);
+            c[j] = kv8_codes(f32x2(f.x, f.y), one_over);
         }
-        uint2 out = make_uint2(kv8_pack4(c[0], c[1], c[2], c[3]), kv8_pack4(c[4], c[5], c[6], c[7]));
+        uint2 out = make_uint2(kv8_pack(c[0], c[1]), kv8_pack(c[2], c[3]));
         if (!ok) out = make_uint2(0, 0);
         *reinterpret_cast<uint2 *>(dst + (row - slice) * pg.row_stride + (u % kPerRow) * 8) = out;
     }
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(kEvThreads) kv8_select_kernel(
 // place the CTAs of a head are a cluster that walks its rows in ascending rounds of 128 a CTA, and stores once each has
 // read its rows of the round: a row never moves up, so the stores of a round hit no source of a later one, and the
 // next round's rows are read ahead of the stores.  (Rounds with that read-ahead, two CTAs per SM, took 41 us where CTAs of
-// 64 rows take 25 when the rows go to other pages: 4 sequences of 16k positions, 4096 of 8 heads kept, 67 MB in rows of
+// 64 rows take 24 when the rows go to other pages: 4 sequences of 16k positions, 4096 of 8 heads kept, 67 MB in rows of
 // 128 bytes.)
 template <int D, bool IN_PLACE>
 __global__ void __launch_bounds__(mv_threads(IN_PLACE), IN_PLACE ? 2 : 5) kv8_move_kernel(
@@ -597,7 +597,7 @@ extern "C" int t2c_kv_cache_evict_q8(const t2c_q8_pages *pages, const float *wei
         return set_error(T2C_EINVAL, "kv_cache_evict_q8: weights in place need the codes in place");
     const int64_t heads = B * pg.n_kv;
     // CTAs that select for a head: up to 8 while the SMs have room and each keeps 2048 positions (select, move and read back,
-    // 8 heads: 16007 positions of 4 sequences 59 us, one CTA a head 73, eight 72; 60000 of one 73, one CTA 162; 1003 of one
+    // 8 heads: 16007 positions of 4 sequences 57 us, one CTA a head 72, eight 70; 60000 of one 71, one CTA 160; 1003 of one
     // 16, eight 28)
     unsigned cluster = 1;
     while (cluster < 8 && capacity > static_cast<int64_t>(cluster) * 4096 &&
@@ -607,7 +607,7 @@ extern "C" int t2c_kv_cache_evict_q8(const t2c_q8_pages *pages, const float *wei
     const int cache = static_cast<int>(slice < kEvCache ? slice : kEvCache);
     int64_t chunks = (keep + mv_rows(in_place) - 1) / mv_rows(in_place);
     if (in_place) {  // a cluster per head, as large as keeps the SMs busy, up to 8 (4096 of 16384 positions, 4 sequences of 8
-                     // heads: 55 us, one CTA a head 217; 1024 of 2048, 32 sequences: 67, eight 72)
+                     // heads: 47 us, one CTA a head 175; 1024 of 2048, 32 sequences: 57, eight 61)
         const int64_t full = chunks;
         chunks = 1;
         while (chunks < 8 && chunks < full && heads * chunks < 2 * sm_count()) chunks *= 2;

@@ -85,16 +85,6 @@ __device__ __forceinline__ __half kv8_scale_for(float top) {
     return __float2half_ru(fminf(__fdiv_rn(top, 127.0f), 515.5f));
 }
 
-// round-to-nearest-even of x / s as the low byte of the result.  inv = 1 / s.  y = x * inv is within a few
-// ulp; adding the exactly computed residual x - y * s once makes every representable quotient (the ties
-// k + 1/2 among them) exact, and no other x / s of an up-to-18-bit x and an 11-bit s lies within 2^-20 of a
-// tie.  1.5 * 2^23 then leaves the integer in the low mantissa bits.  |x / s| <= 127.
-__device__ __forceinline__ uint32_t kv8_code(float x, float s, float inv) {
-    float y = x * inv;
-    y = fmaf(fmaf(-y, s, x), inv, y);
-    return __float_as_uint(y + 12582912.0f);
-}
-
 __device__ __forceinline__ uint32_t kv8_pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
@@ -113,30 +103,38 @@ __device__ __forceinline__ int kv8_largest(uint32_t most, uint32_t least) {
     return max(max(half(most, 0), half(most, 1)), -min(half(least, 0), half(least, 1)));
 }
 
-// s_old / s_new in two floats, high + low to 2^-46 of it.  rint(code * (high + low)), the small product first, is then
-// the correctly rounded code * s_old / s_new: that is within 2^-23 of the quotient, whose distance from a tie is zero or
-// at least 2^-19 of it (both scales have 11 bits, the code 7), and exact where it is a tie.
-__device__ __forceinline__ float2 kv8_ratio(float s_old, float s_new, float inv_new) {
-    const float high = __fdiv_rn(s_old, s_new);
-    return make_float2(high, fmaf(-high, s_new, s_old) * inv_new);
+// x / s in two floats, high + low to 2^-46 of it (inv = 1 / s).
+__device__ __forceinline__ float2 kv8_ratio(float x, float s, float inv) {
+    const float high = __fdiv_rn(x, s);
+    return make_float2(high, fmaf(-high, s, x) * inv);
+}
+
+// rint of two values times a ratio, |result| <= 127, as the low bytes of two words.  With a code of 7 bits and ratios of two
+// scales of 11, or a value of 11 bits and one over a scale, this is the correctly rounded quotient: the small product first,
+// what is rounded is within 2^-23 of the quotient, whose distance from a tie is zero or at least 2^-19 of it, and it is the
+// quotient itself where that is a tie.  1.5 * 2^23 then leaves the integer in the low mantissa bits.
+__device__ __forceinline__ uint64_t kv8_codes(uint64_t x, float2 ratio) {
+    const uint64_t y = f32x2_fma(x, f32x2(ratio.x, ratio.x), f32x2_mul(x, f32x2(ratio.y, ratio.y)));
+    return f32x2_add(y, f32x2(12582912.0f, 12582912.0f));
+}
+
+__device__ __forceinline__ uint32_t kv8_pack(uint64_t a, uint64_t b) {
+    const float2 x = f32x2_parts(a), y = f32x2_parts(b);
+    return kv8_pack4(__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(y.x), __float_as_uint(y.y));
 }
 
 // A word's four codes at another scale.  (Code + 128 in the mantissa of 2^23 becomes a float without a conversion
-// instruction, two values an instruction from there on: 5 instructions a code in all, where conversion, product, quotient
-// and its correction took 9 and the move's time was theirs: 26 us, now see there.)
+// instruction, two values an instruction from there on: with conversions, a product, the quotient and its correction a code
+// 17 M instructions were 13 M here, the in-place move of 4 x 4096 rows of 8 heads 55 us, now 47.)
 __device__ __forceinline__ uint32_t kv8_recode(uint32_t w, float2 ratio) {
     const uint32_t u = w ^ 0x80808080u;
-    const uint64_t bias = f32x2(-8388736.0f, -8388736.0f), round = f32x2(12582912.0f, 12582912.0f);
-    const uint64_t high = f32x2(ratio.x, ratio.x), low = f32x2(ratio.y, ratio.y);
+    const uint64_t bias = f32x2(-8388736.0f, -8388736.0f);
     uint64_t c[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const uint64_t v = f32x2_add(f32x2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + 2 * i)),
-                                           __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441 + 2 * i))), bias);
-        c[i] = f32x2_add(f32x2_fma(v, high, f32x2_mul(v, low)), round);
-    }
-    const float2 a = f32x2_parts(c[0]), b = f32x2_parts(c[1]);
-    return kv8_pack4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+    for (int i = 0; i < 2; ++i)
+        c[i] = kv8_codes(f32x2_add(f32x2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + 2 * i)),
+                                         __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441 + 2 * i))), bias), ratio);
+    return kv8_pack(c[0], c[1]);
 }
 
 template <typename Kernel, typename... Args>
