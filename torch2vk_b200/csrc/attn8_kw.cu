@@ -45,7 +45,8 @@ struct WeightArgs {
 
 __device__ __forceinline__ uint32_t w_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 
-template <int D>
+// MANY: several key tiles a CTA; without, nothing of a next tile takes registers (8192 queries of 32 heads: 361 us, else 372).
+template <int D, bool MANY>
 __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __grid_constant__ CUtensorMap q_map,
                                                                      const __grid_constant__ WeightArgs a) {
     using S = WeightShape<D>;
@@ -92,7 +93,7 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
     const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
     const int pairs = a.B * a.pg.n_kv, item = blockIdx.x / C;
     const int head = item % a.pg.n_kv, b = item / a.pg.n_kv % a.B;
-    const int kt0 = item / pairs * a.keys_per;
+    const int kt0 = item / pairs * (MANY ? a.keys_per : 1);
     const int64_t p0 = a.positions[b];
     int64_t n = p0 + a.T;
     if (n > a.max_len) {
@@ -100,7 +101,7 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
         n = a.max_len;
     }
     const int all_keys = n > 0 ? static_cast<int>((n + 127) / 128) : 0;
-    const int kt1 = min(kt0 + a.keys_per, all_keys), nq = (a.T + TT - 1) / TT;
+    const int kt1 = min(kt0 + (MANY ? a.keys_per : 1), all_keys), nq = (a.T + TT - 1) / TT;
     // query tiles that see a key of tile kt: this CTA's share of those from the first one on
     const auto share = [&](int kt, int of) {
         const int64_t t = static_cast<int64_t>(kt) * 128 - p0;
@@ -116,12 +117,20 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
             const int page_mask = (1 << a.pg.page_log2) - 1;
             const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * warp) << 16);
             uint4 x[kPasses];
-            float kf = 0.0f;
-            const auto fetch = [&](int kt) {  // codes of the warp's 32 keys, the factor of the lane's own
+            __half ks;
+            // the lane's table entry is read two tiles ahead, codes and scale one, and nothing waits for either here
+            const auto entry = [&](int kt) {
+                const int64_t mine = static_cast<int64_t>(kt) * 128 + 32 * warp + lane;
+                return mine < n ? bt[mine >> a.pg.page_log2] : 0;
+            };
+            const auto fetch = [&](int kt, int page) {  // codes of the warp's 32 keys, the scale of the lane's own
                 const int64_t k = static_cast<int64_t>(kt) * 128 + 32 * warp, mine = k + lane;
-                const int page = mine < n ? max(kv8_page(a.pg, bt, mine), 0) : 0;
-                kf = 0.0f;
-                if (mine < n) kf = __half2float(a.pg.ks[kv8_scale_offset(a.pg, page, head, mine)]) * a.scale_log2;
+                if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pg.num_pages)) {
+                    report_device_error(T2C_EINVAL);
+                    page = 0;
+                }
+                ks = __ushort_as_half(0);
+                if (mine < n) ks = a.pg.ks[kv8_scale_offset(a.pg, page, head, mine)];
 #pragma unroll
                 for (int i = 0; i < kPasses; ++i) {
                     const int r = i * kRowsPass + r0;
@@ -132,10 +141,7 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
                                          (static_cast<int>(k + r) & page_mask) * a.pg.row_stride + 16 * c);
                 }
             };
-            fetch(kt0);
-            int count = 0;  // query tiles so far
-            for (int kt = kt0; kt < kt1; ++kt) {
-                // every S of the tile before has been read, so every MMA on this buffer is done
+            const auto expand = [&]() {  // what fetch brought, as the A operand; the factor of the lane's key
 #pragma unroll
                 for (int i = 0; i < kPasses; ++i) {
                     const int r = 32 * warp + i * kRowsPass + r0;
@@ -160,8 +166,16 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(k_ready);
-                const float kf_tile = kf;
-                if (kt + 1 < kt1) fetch(kt + 1);
+                return __half2float(ks) * a.scale_log2;
+            };
+            fetch(kt0, entry(kt0));
+            int page = MANY ? entry(kt0 + 1) : 0;
+            const float kf_only = MANY ? 0.0f : expand();
+            int count = 0;  // query tiles so far
+            for (int kt = kt0; kt < kt1; ++kt) {
+                // every S of the tile before has been read, so every MMA on this buffer is done
+                const float kf_tile = MANY ? expand() : kf_only;
+                if (MANY && kt + 1 < kt1) fetch(kt + 1, page), page = entry(kt + 2);
                 const int64_t key = static_cast<int64_t>(kt) * 128 + 32 * warp + lane;
                 const uint64_t kk = f32x2(kf_tile, kf_tile);
                 const int64_t o = b * a.w_sb + head * a.w_sh + key;
@@ -347,7 +361,7 @@ extern "C" int t2c_attn_key_weights_q8(const t2c_q8_pages *pages, const void *q,
     // query tiles of the first keys, which every query sees, until the longest share is under 3/4 of the mean of an SM's
     // slot; 32 query tiles a CTA at least, which its beginning costs about 4 of (6000 queries of 16 heads on 8: 150 us
     // alone, 116 in pairs, 139 in fours; 4096 queries of 16 heads of 64 on 16: 53, 62, 84).  32 queries on 2 x 16007
-    // positions: 7 key tiles a CTA 27 us, one 39.
+    // positions: 7 key tiles a CTA 26 us, one 39.
     const int64_t nq = (T + tokens - 1) / tokens, tiles = (max_len + 127) / 128, units = B * a.pg.n_kv, slots = 2 * sm_count();
     int64_t per = nq >= 8 ? 1 : (units * tiles + slots - 1) / slots;
     per = per > 32 ? 32 : per;
@@ -357,9 +371,10 @@ extern "C" int t2c_attn_key_weights_q8(const t2c_q8_pages *pages, const void *q,
     a.keys_per = static_cast<int>(per);
     const int64_t blocks = units * ((tiles + per - 1) / per) * cluster;
     if (blocks > INT32_MAX) return set_error(T2C_EINVAL, "attn_key_weights_q8: bad shape");
-    const auto kern = D == 128 ? attn8_weights_kernel<128> : attn8_weights_kernel<64>;
+    const auto kern = per > 1 ? (D == 128 ? attn8_weights_kernel<128, true> : attn8_weights_kernel<64, true>)
+                              : (D == 128 ? attn8_weights_kernel<128, false> : attn8_weights_kernel<64, false>);
     const int smem = D == 128 ? WeightShape<128>::kSmem : WeightShape<64>::kSmem;
-    rc = kv8_configure(kern, smem, D == 128 ? 4 : 5, "attn_key_weights_q8");
+    rc = kv8_configure(kern, smem, (D == 128 ? 4 : 5) + (per > 1 ? 3 : 0), "attn_key_weights_q8");
     if (rc != T2C_OK) return rc;
     return kv8_launch("attn_key_weights_q8", kern, dim3(static_cast<unsigned>(blocks)), dim3(kWThreads), smem, cluster, as_stream(stream),
                       q_map, a);
