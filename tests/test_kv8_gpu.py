@@ -340,6 +340,31 @@ def test_prefill_long(T, length):
         check_attention(out, lse, want)
 
 
+@pytest.mark.parametrize("NH,NK,dim", [(4, 2, 64), (8, 2, 128), (3, 1, 64)])
+@pytest.mark.parametrize("splits", [0, 1, 2])
+def test_prefill_rising_scores(NH, NK, dim, splits):
+    """Scores that rise by 45 to 70 (in log2 units) from each page of 128 keys to the next: the running reference moves in
+    every tile, after sums of earlier tiles were taken."""
+    from torch2vk_b200 import kernels
+
+    length, T, page, block = 2500, 150, 128, 64
+    width = -(-length // page)
+    cache, table, g, _ = attention_case(1, NH, NK, dim, page, block, width, 61)
+    u = torch.randn(dim, generator=g).sign()
+    k = cache["k"]
+    k.copy_((u * 100 + torch.randint(-20, 21, k.shape, generator=g)).to(torch.int8))
+    for i, p in enumerate(table[0].tolist()):
+        cache["ks"][p] = (i + 1) * 0.44 / dim ** 0.5
+    pages, bt = device_pages(cache), table.cuda()
+    q = (u * 8 / dim ** 0.5 + torch.randn(1, T, NH, dim, generator=g) * 0.1).half()
+    want = ref.attention(cache, q, [length - T], table, dim ** -0.5)
+    out, lse = kernels.attn_prefill_q8(q.cuda(), pages, i32([length - T]), bt, splits=splits, return_lse=True)
+    clean()
+    check_attention(out, lse, want)
+    scores = want["lse"]
+    assert float(scores.min()) > 200 and float(scores.max()) < 5000
+
+
 def test_attention_scales_apart():
     """Blocks whose scales differ by many powers of two, zero blocks, and the largest values: no overflow, no loss."""
     from torch2vk_b200 import kernels

@@ -10,7 +10,9 @@
 // to fp16 operand tiles (loads a tile ahead in registers), warp 16 issues the MMAs.
 //
 // The tensor core's work for one query tile runs under the other tile's softmax.  What bounds it: the chain S, softmax, P V
-// of a query tile, whose P takes the place of its S (TMEM holds two S and two O of 128 columns, no third S).  8192 queries
+// of a query tile, whose P takes the place of its S (TMEM holds two S and two O of 128 columns, no third S).  With D = 64 a
+// third S fits: the three go round, S of the next key tile is made while this one's softmax runs, and the chain is the
+// softmax alone (4 x 512 queries on up to 3500, 16 heads of 64 on 16: 65 us, with two 73).  8192 queries
 // on themselves, 32 heads of 128 on 8: 583 us, 943 TFLOP/s; a key tile takes 3800 clocks, of them the softmax 2150 (the 2^
 // unit 1024), the products 1010, two hand-overs through mbarriers 550, where the products alone would take 2020 and the 2^
 // of both query tiles 2050.  Measured and not kept: four softmax warpgroups, half a row a thread (643 us), S in halves of
@@ -46,6 +48,8 @@ struct PrefillShape {
     static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + 2 * kTile, kMeta = kV + 2 * kTile;
     static constexpr int kBars = kMeta + 4 * 8 * 20;   // meta: ring of 4 tiles x 8 groups of 16 keys
     static constexpr int kSmem = kBars + 256;
+    static constexpr int kS = D == 64 ? 3 : 2;         // S buffers of 128 TMEM columns that lie beside the two O
+    static constexpr int kO = 128 * kS;
 };
 
 struct PrefillArgs {
@@ -92,10 +96,10 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
     ulonglong2 *meta = reinterpret_cast<ulonglong2 *>(smem + S::kMeta);
     float *inv_vs = reinterpret_cast<float *>(smem + S::kMeta + 4 * 8 * 16);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kBars);
-    uint64_t *k_full = bars, *v_full = bars + 2, *k_free = bars + 4, *v_free = bars + 6, *s_ready = bars + 8,
-             *o_done = bars + 10, *p_ready = bars + 11, *q_full = bars + 13, *meta_full = bars + 14;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 18);
-    volatile int *stop = reinterpret_cast<volatile int *>(bars + 19), *stop_last = stop + 1;
+    uint64_t *k_full = bars, *v_full = bars + 2, *k_free = bars + 4, *v_free = bars + 6, *o_added = bars + 8, *o_done = bars + 10,
+             *s_ready = bars + 11, *p_ready = bars + 14, *q_full = bars + 17, *meta_full = bars + 18;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 22);
+    volatile int *stop = reinterpret_cast<volatile int *>(bars + 23), *stop_last = stop + 1;
     if (base & 1023u) {  // the swizzle atoms need it: report, compute nothing
         if (threadIdx.x == 0) report_device_error(T2C_EUNSUPPORTED);
         return;
@@ -103,8 +107,8 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < 4; ++i) mbar_init(k_full + i, 8);  // k_full, v_full: the expanding warps
-        for (int i = 4; i < 11; ++i) mbar_init(bars + i, 1);   // commits
-        for (int i = 0; i < 2; ++i) mbar_init(p_ready + i, 4);
+        for (int i = 4; i < 14; ++i) mbar_init(bars + i, 1);   // commits
+        for (int i = 0; i < 3; ++i) mbar_init(p_ready + i, 4);
         mbar_init(q_full, 256);
         for (int i = 0; i < 4; ++i) mbar_init(meta_full + i, 8);
         *stop = 0;
@@ -172,9 +176,13 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
             const int64_t limit = min(p0 + min(t, a.T - 1), n - 1);
             const int64_t least = min(p0 + min(t_first + qi * TT, a.T - 1), n - 1);
             const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
-            const uint32_t s_at = lanes + 128 * qi, o_at = lanes + 256 + D * qi;
+            const uint32_t o_at = lanes + S::kO + D * qi;
             float m = kPRefStart, l = 0.0f;
-            for (int j = 0; j < tiles; ++j) {
+            // S of (key tile j, query tile qi) is number 2 j + qi, in buffer number % kS
+            int buf = qi, turn = 0;
+            for (int j = 0; j < tiles; ++j, buf += 2 - S::kS, turn ^= 1) {
+                if (buf < 0) buf += S::kS, turn ^= 1;  // (two numbers on wrap round or not)
+                const uint32_t s_at = lanes + 128 * buf;
                 mbar_wait_or(&meta_full[j & 3], (j >> 2) & 1, stop);
                 const ulonglong2 *f = meta + (j & 3) * 8;
                 const float *fi = inv_vs + (j & 3) * 8;
@@ -185,7 +193,7 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                     const float4 x = reinterpret_cast<const float4 *>(f)[c];
                     kf[c] = x.x, lv[c] = x.z, iv[c] = fi[c];
                 }
-                mbar_wait_or(&s_ready[qi], j & 1, stop);
+                mbar_wait_or(&s_ready[buf], turn, stop);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const int64_t k0 = static_cast<int64_t>(tile0 + j) * kPKeys;
                 const bool masked = k0 + kPKeys - 1 > least;
@@ -265,7 +273,11 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                     const float corr = ex2(m - ref);
                     m = ref;
                     l *= corr;
-                    if (j > 0) {  // S being ready says that the tiles before are in O
+                    if (j > 0) {
+                        if (S::kS > 2) {  // (with two buffers S being ready says that the tiles before are in O)
+                            mbar_wait_or(&o_added[qi], (j - 1) & 1, stop);
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        }
 #pragma unroll 1
                         for (int i = 0; i < D / 16; ++i) {
                             uint32_t w[16];
@@ -320,7 +332,7 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                 tmem_st_wait();
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_ready[qi]);
+                if (lane == 0) mbar_arrive(&p_ready[buf]);
             }
             mbar_wait_or(o_done, 0, stop);
             if (!__any_sync(0xffffffffu, *stop != 0)) {
@@ -461,47 +473,57 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                 const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
                 const int nt = __reduce_max_sync(0xffffffffu, tiles);
                 const uint32_t idesc_s = umma_idesc(128, 128, false), idesc_o = umma_idesc(128, D, true);
-                const auto scores = [&](int qi, int st) {
+                const auto scores = [&](int buf, int qi, int st) {
                     const uint32_t q = umma_desc_lo(base + S::kQ + qi * S::kTile);
                     const uint32_t k = umma_desc_lo(base + S::kK + st * S::kTile);
 #pragma unroll
                     for (int s = 0; s < D / 16; ++s) {
                         const uint32_t off = static_cast<uint32_t>((s >> 2) * 1024 + 2 * (s & 3));  // 16-byte units
-                        umma_ss(tm + 128 * qi, q + off, k + off, idesc_s, s > 0);
+                        umma_ss(tm + 128 * buf, q + off, k + off, idesc_s, s > 0);
                     }
-                    umma_commit(&s_ready[qi]);
+                    umma_commit(&s_ready[buf]);
+                    if (qi == 1) umma_commit(&k_free[st]);
                 };
-                const auto values = [&](int qi, int st, bool acc) {
+                const auto values = [&](int buf, int qi, int st, bool acc) {
                     const uint32_t v = umma_desc_lo(base + S::kV + st * S::kTile, 16384);
 #pragma unroll
                     for (int s = 0; s < 8; ++s)
-                        umma_ts(tm + 256 + D * qi, tm + 128 * qi + 8 * s, v + 128 * s, idesc_o, acc || s > 0);
+                        umma_ts(tm + S::kO + D * qi, tm + 128 * buf + 8 * s, v + 128 * s, idesc_o, acc || s > 0);
                 };
                 mbar_wait_or(q_full, 0, stop);
-                mbar_wait_or(&k_full[0], 0, stop);
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (elect_one()) {
-                    scores(0, 0);
-                    scores(1, 0);
-                    umma_commit(&k_free[0]);
+#pragma unroll
+                for (int i = 0; i < S::kS; ++i) {  // the first S of every buffer
+                    if (i >> 1 >= nt) break;
+                    if ((i & 1) == 0) mbar_wait_or(&k_full[i >> 1], 0, stop);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (elect_one()) scores(i, i & 1, i >> 1);
+                    __syncwarp();
                 }
-                __syncwarp();
+                // P V of number 2 j + qi, then the S that is kS numbers on over it
+                int buf = 0, turn = 0;
                 for (int j = 0; j < nt; ++j) {
-                    const int st = j & 1, next = st ^ 1;
-                    const bool more = j + 1 < nt;
+                    const int st = j & 1;
                     mbar_wait_or(&v_full[st], (j >> 1) & 1, stop);
-                    if (more) mbar_wait_or(&k_full[next], ((j + 1) >> 1) & 1, stop);
+                    if (S::kS == 2 && j + 1 < nt) mbar_wait_or(&k_full[st ^ 1], ((j + 1) >> 1) & 1, stop);
 #pragma unroll
                     for (int qi = 0; qi < 2; ++qi) {
-                        mbar_wait_or(&p_ready[qi], j & 1, stop);
+                        const int at = S::kS == 2 ? qi : buf, on = S::kS == 2 ? qi : qi ^ 1, ahead = j + (qi + S::kS) / 2;
+                        mbar_wait_or(&p_ready[at], S::kS == 2 ? j & 1 : turn, stop);
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         if (elect_one()) {
-                            values(qi, st, j > 0);
+                            values(at, qi, st, j > 0);
                             if (qi == 1) umma_commit(&v_free[st]);
-                            if (more) scores(qi, next);
-                            if (more && qi == 1) umma_commit(&k_free[next]);
+                            if (S::kS > 2) umma_commit(&o_added[qi]);
+                            if (S::kS == 2 && ahead < nt) scores(at, on, ahead & 1);
                         }
                         __syncwarp();
+                        if (S::kS > 2 && ahead < nt) {
+                            if (on == 0) mbar_wait_or(&k_full[ahead & 1], (ahead >> 1) & 1, stop);
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                            if (elect_one()) scores(at, on, ahead & 1);
+                            __syncwarp();
+                        }
+                        if (++buf == S::kS) buf = 0, turn ^= 1;
                     }
                 }
                 if (elect_one()) umma_commit(o_done);
@@ -606,8 +628,8 @@ struct PrefillPlan {
 };
 
 // One CTA per SM: the keys of a pair of query tiles are split while CTAs would be missing, at least two tiles each.
-// (45 queries on 9111 keys, 32 heads on 8: 18 splits 27 us; one 170, 9 35, 36 40.  512 on 8192: two splits 105 us, one 158,
-// four 117.  4 x 512 on up to 3500, 16 heads of 64 on 16: one split 72, two 99.)
+// (45 queries on 9111 keys, 32 heads on 8: 18 splits 27 us; one 170, 9 35, 36 40.  512 on 8192: two splits 104 us, one
+// 160, four 116.  4 x 512 on up to 3500, 16 heads of 64 on 16: one split 65, two 91.)
 PrefillPlan prefill_plan(int64_t B, int64_t T, int64_t NH, int64_t NK, int64_t D, int64_t max_len, int64_t splits) {
     PrefillPlan r = {};
     const int64_t tokens = 2 * (kPRows / (NH / NK));
