@@ -13,7 +13,7 @@
 // of a query tile, whose P takes the place of its S (TMEM holds two S and two O of 128 columns, no third S).  With D = 64 a
 // third S fits: the three go round, S of the next key tile is made while this one's softmax runs, and the chain is the
 // softmax alone (4 x 512 queries on up to 3500, 16 heads of 64 on 16: 65 us, with two 73).  8192 queries
-// on themselves, 32 heads of 128 on 8: 583 us, 943 TFLOP/s; a key tile takes 3800 clocks, of them the softmax 2150 (the 2^
+// on themselves, 32 heads of 128 on 8: 582 us, 945 TFLOP/s; a key tile takes 3800 clocks, of them the softmax 2150 (the 2^
 // unit 1024), the products 1010, two hand-overs through mbarriers 550, where the products alone would take 2020 and the 2^
 // of both query tiles 2050.  Measured and not kept: four softmax warpgroups, half a row a thread (643 us), S in halves of
 // 64 keys (607), P handed over in halves (660), 16 keys a stage (690), one lane polling the barriers (875).
@@ -131,8 +131,31 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
     item /= a.pg.n_kv;
     const int b = item % a.B;
     const int pair = a.pairs - 1 - item / a.B;
-    const int64_t p0 = a.positions[b];
     const int t_first = pair * 2 * TT, t_last = min(t_first + 2 * TT, a.T) - 1;
+    if (warp < 8) {  // a warp 32 rows of a query tile, neighbouring lanes neighbouring units of a row, all loads in flight (sixteen
+        // of D = 128: the row tiles are there 0.7 us earlier than in two turns of eight), before positions are known
+        const int qi = warp >> 2;
+        constexpr int kUnits = D / 8, kRowsPer = 32 / kUnits, kLoads = 32 / kRowsPer;
+        const uint32_t at = base + S::kQ + qi * S::kTile;
+        const int u = lane % kUnits, r0 = 32 * (warp & 3) + lane / kUnits;
+        const uint32_t per = 65536u / group + 1;  // r / group = r * per >> 16 for r, group <= 128
+        const __half *src = a.q + b * a.q_sb + static_cast<int64_t>(head * group) * a.q_sh + 8 * u;
+        uint4 v[kLoads];
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int r = r0 + i * kRowsPer, tr = r * per >> 16, tq = t_first + qi * TT + tr;
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (tr < TT && tq < a.T)
+                v[i] = *reinterpret_cast<const uint4 *>(src + static_cast<int64_t>(tq) * a.q_st + (r - tr * group) * a.q_sh);
+        }
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+            sts128(at + unit_at(r0 + i * kRowsPer, u), __byte_perm(v[i].x, v[i].y, 0x5410), __byte_perm(v[i].x, v[i].y, 0x7632),
+                   __byte_perm(v[i].z, v[i].w, 0x5410), __byte_perm(v[i].z, v[i].w, 0x7632));
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(q_full);
+    }
+    const int64_t p0 = a.positions[b];
     int64_t n = p0 + t_last + 1;  // keys the last query sees
     if (n > a.max_len) {
         if (tid == 0) report_device_error(T2C_EINVAL);
@@ -150,28 +173,6 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
             const int qi = warp >> 2, row = tid & 127;
             const int t = t_first + qi * TT + row / group, h = head * group + row % group;
             const bool real = row < TT * group && t < a.T;
-            {   // a warp its 32 rows, neighbouring lanes neighbouring units of a row, all loads in flight (sixteen of D = 128:
-                // the row tiles are there 0.7 us earlier than in two turns of eight)
-                constexpr int kUnits = D / 8, kRowsPer = 32 / kUnits, kLoads = 32 / kRowsPer;
-                const uint32_t at = base + S::kQ + qi * S::kTile;
-                const int u = lane % kUnits, r0 = 32 * (warp & 3) + lane / kUnits;
-                const uint32_t per = 65536u / group + 1;  // r / group = r * per >> 16 for r, group <= 128
-                const __half *src = a.q + b * a.q_sb + static_cast<int64_t>(head * group) * a.q_sh + 8 * u;
-                uint4 v[kLoads];
-#pragma unroll
-                for (int i = 0; i < kLoads; ++i) {
-                    const int r = r0 + i * kRowsPer, tr = r * per >> 16, tq = t_first + qi * TT + tr;
-                    v[i] = make_uint4(0, 0, 0, 0);
-                    if (tr < TT && tq < a.T)
-                        v[i] = *reinterpret_cast<const uint4 *>(src + static_cast<int64_t>(tq) * a.q_st + (r - tr * group) * a.q_sh);
-                }
-#pragma unroll
-                for (int i = 0; i < kLoads; ++i)
-                    sts128(at + unit_at(r0 + i * kRowsPer, u), __byte_perm(v[i].x, v[i].y, 0x5410), __byte_perm(v[i].x, v[i].y, 0x7632),
-                           __byte_perm(v[i].z, v[i].w, 0x5410), __byte_perm(v[i].z, v[i].w, 0x7632));
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(q_full);
-            }
             // last key of this row, and of the tile's first token: rows past the end follow the last real token
             const int64_t limit = min(p0 + min(t, a.T - 1), n - 1);
             const int64_t least = min(p0 + min(t_first + qi * TT, a.T - 1), n - 1);
@@ -343,14 +344,14 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                                                 (256 * (D + 2));
                     float *dst = part + (qi * 128 + row) * D;
 #pragma unroll 1
-                    for (int c = 0; c < D / 16; ++c) {
-                        uint32_t v[16];
-                        tmem_ld16(o_at + 16 * c, v);
-                        tmem_ld_wait16(v);
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t v[32];
+                        tmem_ld32(o_at + 32 * c, v);
+                        tmem_ld_wait32(v);
                         if (real) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                reinterpret_cast<uint4 *>(dst)[4 * c + i] = make_uint4(v[4 * i], v[4 * i + 2], v[4 * i + 1], v[4 * i + 3]);
+                            for (int i = 0; i < 8; ++i)
+                                reinterpret_cast<uint4 *>(dst)[8 * c + i] = make_uint4(v[4 * i], v[4 * i + 2], v[4 * i + 1], v[4 * i + 3]);
                         }
                     }
                     part[256 * D + qi * 128 + row] = m;
@@ -359,17 +360,17 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                     const float inv = seen ? 1.0f / l : 0.0f;
                     __half *o = a.out + b * a.o_sb + static_cast<int64_t>(t) * a.o_st + h * a.o_sh;
 #pragma unroll 1
-                    for (int c = 0; c < D / 16; ++c) {
-                        uint32_t v[16];
-                        tmem_ld16(o_at + 16 * c, v);
-                        tmem_ld_wait16(v);
-                        float x[16];
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t v[32];
+                        tmem_ld32(o_at + 32 * c, v);
+                        tmem_ld_wait32(v);
+                        float x[32];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) x[i] = seen ? __uint_as_float(v[i]) * inv : 0.0f;
+                        for (int i = 0; i < 32; ++i) x[i] = seen ? __uint_as_float(v[i]) * inv : 0.0f;
                         if (real) {
 #pragma unroll
-                            for (int i = 0; i < 2; ++i)
-                                reinterpret_cast<uint4 *>(o)[2 * c + i] =
+                            for (int i = 0; i < 4; ++i)
+                                reinterpret_cast<uint4 *>(o)[4 * c + i] =
                                     make_uint4(ph_bits(__floats2half2_rn(x[8 * i], x[8 * i + 2])),
                                                ph_bits(__floats2half2_rn(x[8 * i + 1], x[8 * i + 3])),
                                                ph_bits(__floats2half2_rn(x[8 * i + 4], x[8 * i + 6])),
