@@ -637,7 +637,7 @@ int t2c_attn_key_weights_q8(const t2c_q8_pages *pages, const void *q, int64_t q_
                             int64_t bt_width, int64_t B, int64_t T, int64_t NH, float scale, int64_t max_len,
                             const float *weights, float *weights_out, int64_t w_sb, int64_t w_sh, void *stream);
 /*
- * Cuts every sequence to at most `keep` positions, for each KV head by itself: a sequence of n = lengths[b] <= keep
+ * Cuts every sequence (65535 at most) to at most `keep` positions, for each KV head by itself: a sequence of n = lengths[b] <= keep
  * positions keeps all; otherwise the first `sinks`, the last `recent` and, of the others, those with the largest
  * weights[b, head, j] stay (equal weights: the lowest positions; NaN counts as the largest).  The kept rows move, in
  * order, to positions 0 .. of out_table's pages; each block's new scale is the least fp16 number >= its

@@ -322,10 +322,16 @@ __global__ void __launch_bounds__(kEvThreads) kv8_select_kernel(
                 cluster.sync();
                 // bins 2 * tid and 2 * tid + 1 over the cluster, then the bin where the count from the top reaches `want`
                 int c[2] = {0, 0};
-                for (int r = 0; r < C; ++r) {
-                    const uint2 h = *reinterpret_cast<const uint2 *>(cluster.map_shared_rank(&hist[pass][2 * tid], r));
-                    c[0] += static_cast<int>(h.x);
-                    c[1] += static_cast<int>(h.y);
+                uint2 h[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {  // all in flight
+                    h[r] = make_uint2(0, 0);
+                    if (r < C) h[r] = *reinterpret_cast<const uint2 *>(cluster.map_shared_rank(&hist[pass][2 * tid], r));
+                }
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    c[0] += static_cast<int>(h[r].x);
+                    c[1] += static_cast<int>(h[r].y);
                 }
                 const int mine = c[0] + c[1];
                 int suffix = mine;  // over this and the higher lanes
@@ -387,13 +393,9 @@ __global__ void __launch_bounds__(kEvThreads) kv8_select_kernel(
         if (lane == 0) cta_sure = a, cta_eq = e;
     }
     cluster.sync();
-    int run_sure = 0, run_eq = 0;
-    for (int r = 0; r < rank; ++r) {
-        run_sure += *cluster.map_shared_rank(&cta_sure, r);
-        run_eq += *cluster.map_shared_rank(&cta_eq, r);
-    }
-    run_sure += ev_warp_sum(lane < warp ? warp_sure[lane] : 0);
-    run_eq += ev_warp_sum(lane < warp ? warp_eq[lane] : 0);
+    // what comes before this warp: a lane for each lower rank and each lower warp
+    int run_sure = ev_warp_sum((lane < rank ? *cluster.map_shared_rank(&cta_sure, lane) : 0) + (lane < warp ? warp_sure[lane] : 0));
+    int run_eq = ev_warp_sum((lane < rank ? *cluster.map_shared_rank(&cta_eq, lane) : 0) + (lane < warp ? warp_eq[lane] : 0));
     for (int base = p0; base < p1; base += 32) {
         bool sure, eq;
         classify(base + lane, sure, eq);
