@@ -265,7 +265,7 @@ __device__ __forceinline__ int ev_warp_sum(int v) { return __reduce_add_sync(0xf
 // holds: the quota-th largest weight of the unprotected positions by three radix passes (11, 11, 10 bits) whose
 // histograms are summed over the cluster through distributed shared memory; equal weights go to the lowest positions.
 // Bound by the passes' chain of barriers: 8 us for 1003 positions, 17 us for 4 x 8 heads of 16007.
-__global__ void __launch_bounds__(kEvThreads) kv8_select_kernel(
+__global__ void __launch_bounds__(kEvThreads, 2) kv8_select_kernel(
     int n_kv, const float *__restrict__ weights, int64_t w_sb, int64_t w_sh, const int32_t *__restrict__ lengths, int64_t capacity,
     int cache_size, int keep, int sinks, int recent, int32_t *__restrict__ kept, int32_t *__restrict__ new_lengths) {
     extern __shared__ uint32_t cache[];
@@ -322,16 +322,19 @@ __global__ void __launch_bounds__(kEvThreads) kv8_select_kernel(
                 cluster.sync();
                 // bins 2 * tid and 2 * tid + 1 over the cluster, then the bin where the count from the top reaches `want`
                 int c[2] = {0, 0};
-                uint2 h[8];
+#pragma unroll 1
+                for (int r0 = 0; r0 < C; r0 += 4) {  // four in flight
+                    uint2 h[4];
 #pragma unroll
-                for (int r = 0; r < 8; ++r) {  // all in flight
-                    h[r] = make_uint2(0, 0);
-                    if (r < C) h[r] = *reinterpret_cast<const uint2 *>(cluster.map_shared_rank(&hist[pass][2 * tid], r));
-                }
+                    for (int r = 0; r < 4; ++r) {
+                        h[r] = make_uint2(0, 0);
+                        if (r0 + r < C) h[r] = *reinterpret_cast<const uint2 *>(cluster.map_shared_rank(&hist[pass][2 * tid], r0 + r));
+                    }
 #pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    c[0] += static_cast<int>(h[r].x);
-                    c[1] += static_cast<int>(h[r].y);
+                    for (int r = 0; r < 4; ++r) {
+                        c[0] += static_cast<int>(h[r].x);
+                        c[1] += static_cast<int>(h[r].y);
+                    }
                 }
                 const int mine = c[0] + c[1];
                 int suffix = mine;  // over this and the higher lanes
@@ -616,8 +619,10 @@ extern "C" int t2c_kv_cache_evict_q8(const t2c_q8_pages *pages, const float *wei
     }
     if (heads * cluster > INT32_MAX || B > 65535) return set_error(T2C_EINVAL, "kv_cache_evict_q8: bad shape");
     rc = kv8_configure(kv8_select_kernel, kEvCache * 4, 6, "kv_cache_evict_q8");
+    // not resident early: CTAs of 1024 threads in wait slowed the kernel before them (4096 of 16384 positions of 4 sequences in
+    // place, call after call: 38 us, with early residence 48)
     if (rc == T2C_OK)
-        rc = kv8_launch("kv_cache_evict_q8", kv8_select_kernel, dim3(static_cast<unsigned>(heads * cluster)), dim3(kEvThreads),
+        rc = kv8_launch_as(false, "kv_cache_evict_q8", kv8_select_kernel, dim3(static_cast<unsigned>(heads * cluster)), dim3(kEvThreads),
                         static_cast<size_t>(cache) * 4, cluster, as_stream(stream), pg.n_kv, weights, w_sb, w_sh, lengths, capacity, cache,
                         static_cast<int>(keep), static_cast<int>(sinks), static_cast<int>(recent), kept, new_lengths);
     if (rc != T2C_OK) return rc;

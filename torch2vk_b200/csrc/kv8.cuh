@@ -137,9 +137,10 @@ __device__ __forceinline__ uint32_t kv8_recode(uint32_t w, float2 ratio) {
     return kv8_pack(c[0], c[1]);
 }
 
+// overlap: the kernel may be resident before the one ahead of it in the stream has ended (it waits in pdl_wait).
 template <typename Kernel, typename... Args>
-int kv8_launch(const char *what, Kernel kernel, dim3 grid, dim3 block, size_t smem, unsigned cluster,
-               cudaStream_t stream, Args... args) {
+int kv8_launch_as(bool overlap, const char *what, Kernel kernel, dim3 grid, dim3 block, size_t smem, unsigned cluster,
+                  cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -147,7 +148,7 @@ int kv8_launch(const char *what, Kernel kernel, dim3 grid, dim3 block, size_t sm
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[0].val.programmaticStreamSerializationAllowed = overlap ? 1 : 0;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = cluster;
     attr[1].val.clusterDim.y = 1;
@@ -157,6 +158,12 @@ int kv8_launch(const char *what, Kernel kernel, dim3 grid, dim3 block, size_t sm
     const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (err != cudaSuccess) return set_error(T2C_ECUDA, "%s launch: %s", what, cudaGetErrorString(err));
     return T2C_OK;
+}
+
+template <typename Kernel, typename... Args>
+int kv8_launch(const char *what, Kernel kernel, dim3 grid, dim3 block, size_t smem, unsigned cluster, cudaStream_t stream,
+               Args... args) {
+    return kv8_launch_as(true, what, kernel, grid, block, smem, cluster, stream, args...);
 }
 
 // Raises a kernel's shared-memory limit once per device; `slot` numbers the kernel.
