@@ -264,7 +264,7 @@ __device__ __forceinline__ int ev_warp_sum(int v) { return __reduce_add_sync(0xf
 // Which positions stay.  One CTA per (sequence, KV head), a cluster where the weights are more than its shared memory
 // holds: the quota-th largest weight of the unprotected positions by three radix passes (11, 11, 10 bits) whose
 // histograms are summed over the cluster through distributed shared memory; equal weights go to the lowest positions.
-// Bound by the passes' chain of barriers: 8 us for 1003 positions, 17 us for 4 x 8 heads of 16007.
+// Bound by the passes' chain of barriers: 8 us for 1003 positions, 16 us for 4 x 8 heads of 16007.
 __global__ void __launch_bounds__(kEvThreads, 2) kv8_select_kernel(
     int n_kv, const float *__restrict__ weights, int64_t w_sb, int64_t w_sh, const int32_t *__restrict__ lengths, int64_t capacity,
     int cache_size, int keep, int sinks, int recent, int32_t *__restrict__ kept, int32_t *__restrict__ new_lengths) {
@@ -602,8 +602,8 @@ extern "C" int t2c_kv_cache_evict_q8(const t2c_q8_pages *pages, const float *wei
         return set_error(T2C_EINVAL, "kv_cache_evict_q8: weights in place need the codes in place");
     const int64_t heads = B * pg.n_kv;
     // CTAs that select for a head: up to 8 while the SMs have room and each keeps 2048 positions (select, move and read back,
-    // 8 heads: 16007 positions of 4 sequences 57 us, one CTA a head 72, eight 70; 60000 of one 71, one CTA 160; 1003 of one
-    // 16, eight 28)
+    // 8 heads: 16007 positions of 4 sequences 55 us, one CTA a head 62, eight 70; 60000 of one 70, one CTA 160; 1003 of one
+    // 13, eight 20)
     unsigned cluster = 1;
     while (cluster < 8 && capacity > static_cast<int64_t>(cluster) * 4096 &&
            (heads * cluster * 2 <= sm_count() || capacity > static_cast<int64_t>(cluster) * kEvCache))
@@ -611,11 +611,11 @@ extern "C" int t2c_kv_cache_evict_q8(const t2c_q8_pages *pages, const float *wei
     const int64_t slice = (capacity + cluster - 1) / cluster + 32 * kEvWarps;
     const int cache = static_cast<int>(slice < kEvCache ? slice : kEvCache);
     int64_t chunks = (keep + mv_rows(in_place) - 1) / mv_rows(in_place);
-    if (in_place) {  // a cluster per head, as large as keeps the SMs busy, up to 8 (4096 of 16384 positions, 4 sequences of 8
-                     // heads: 47 us, one CTA a head 175; 1024 of 2048, 32 sequences: 57, eight 61)
+    if (in_place) {  // a cluster per head, as large as gives every SM a CTA, up to 8 (4096 of 16384 positions, 4 sequences of 8
+                     // heads: 38 us, one CTA a head 175; 1024 of 2048, 32 sequences: one 57, two 60, eight 63)
         const int64_t full = chunks;
         chunks = 1;
-        while (chunks < 8 && chunks < full && heads * chunks < 2 * sm_count()) chunks *= 2;
+        while (chunks < 8 && chunks < full && heads * chunks < sm_count()) chunks *= 2;
     }
     if (heads * cluster > INT32_MAX || B > 65535) return set_error(T2C_EINVAL, "kv_cache_evict_q8: bad shape");
     rc = kv8_configure(kv8_select_kernel, kEvCache * 4, 6, "kv_cache_evict_q8");
