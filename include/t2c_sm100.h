@@ -642,9 +642,10 @@ int t2c_attn_key_weights_q8(const t2c_q8_pages *pages, const void *q, int64_t q_
  * weights[b, head, j] stay (equal weights: the lowest positions; NaN counts as the largest).  The kept rows move, in
  * order, to positions 0 .. of out_table's pages; each block's new scale is the least fp16 number >= its
  * max|code * scale| / 127, code' = round-half-even(code * scale / new scale).  out_table = block_table (one pointer)
- * compacts in place (a sequence that keeps all is then left as it is); otherwise the tables' pages must be disjoint.
- * kept int32 [B, n_kv, keep] gets the kept positions (ascending, then -1), new_lengths[b] = min(n, keep),
- * weights_out[b, head, i] = the weight of kept position i (may be weights itself when in place).
+ * compacts in place (the rows of a sequence that keeps all are then left as they are); otherwise the tables' pages must be
+ * disjoint.  kept int32 [B, n_kv, keep] gets the kept positions (ascending, then -1), new_lengths[b] = min(n, keep),
+ * weights_out[b, head, i] = the weight of kept position i, for every sequence.  When in place weights_out may be weights
+ * itself (with its strides); otherwise the two must not overlap.
  */
 int t2c_kv_cache_evict_q8(const t2c_q8_pages *pages, const float *weights, int64_t w_sb, int64_t w_sh,
                           const int32_t *lengths, const int32_t *block_table, int64_t bt_stride, int64_t bt_width,

@@ -1,0 +1,69 @@
+"""Edges of the paged KV cache in 8 bits.
+
+Codes, scales, kept positions and moved weights are compared bit for bit with the 64-bit statement (tests/kv8_ref.py);
+attention within the bounds that tests/test_kv8_gpu.py derives."""
+
+from __future__ import annotations
+
+import kv8_ref as ref
+import pytest
+import torch
+from test_kv8_gpu import clean, device_pages, i32, same_cache
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _status():
+    from torch2vk_b200 import kernels
+
+    kernels.device_status(clear=True)
+
+
+def _weights(B, heads, positions, seed):
+    """Weights with many ties and zeros."""
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randint(0, 6, (B, heads, positions), generator=g).float() / 4
+    return torch.where(torch.rand(w.shape, generator=g) < 0.5, w, torch.rand(w.shape, generator=g))
+
+
+def _check_kept(kept, moved, chosen, w, keep):
+    for b, heads in enumerate(chosen):
+        for h, want in enumerate(heads):
+            assert kept[b, h].cpu().tolist() == want + [-1] * (keep - len(want)), (b, h)
+            assert torch.equal(moved[b, h, : len(want)].cpu(), w[b, h, want]), (b, h)
+
+
+# ------------------------------------------------------------------ eviction
+@pytest.mark.parametrize("lengths,keep", [([300, 100, 129, 0, 1, 128], 128), ([640, 500, 501, 3, 499, 640], 500), ([5, 60, 64, 0, 1, 2], 64)])
+@pytest.mark.parametrize("dim,page,block", [(128, 64, 16), (64, 16, 16)])
+def test_evict_in_place_own_weights_out(lengths, keep, dim, page, block):
+    """Rows in place, their weights to another tensor: also those of the sequences that keep everything."""
+    from torch2vk_b200 import kernels
+
+    B, NK, width = len(lengths), 3, 640 // page
+    cache = ref.pool(B * width + 1, NK, page, dim, block, seed=201)
+    table = ref.tables(B, width, 1, seed=202)
+    w = _weights(B, NK, width * page, 203)
+    pages, bt, wd = device_pages(cache), table.cuda(), w.cuda()
+    big = torch.full((B, NK + 1, keep + 3), -9.0, device="cuda")
+    wo = big[:, 1:, :keep]  # strides of its own
+    kept, left = kernels.kv_cache_evict_q8(pages, wd, i32(lengths), bt, keep=keep, sinks=4, recent=32, weights_out=wo)
+    clean()
+    chosen, want_left = ref.evict(cache, w, lengths, table, table, keep=keep, sinks=4, recent=32)
+    assert left.cpu().tolist() == want_left
+    _check_kept(kept, wo, chosen, w, keep)
+    for b, n in enumerate(want_left):
+        assert bool((wo[b, :, n:] == -9.0).all())
+    assert torch.equal(wd.cpu(), w) and bool((big[:, 0] == -9.0).all()) and bool((big[:, :, keep:] == -9.0).all())
+    same_cache(pages, cache)
+
+
+def test_evict_refuses_one_tensor_with_two_strides():
+    from torch2vk_b200 import kernels
+
+    cache, table = ref.pool(9, 2, 16, 64, 16, seed=205), ref.tables(2, 4, 1, seed=206)
+    buf = torch.zeros(2 * 2 * 64, device="cuda")
+    with pytest.raises(RuntimeError, match="strides"):
+        kernels.kv_cache_evict_q8(device_pages(cache), buf.view(2, 2, 64), i32([60, 60]), table.cuda(), keep=32,
+                                  weights_out=buf[:128].view(2, 2, 32))

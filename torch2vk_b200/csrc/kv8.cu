@@ -432,14 +432,18 @@ __global__ void __launch_bounds__(mv_threads(IN_PLACE), IN_PLACE ? 2 : 5) kv8_mo
     const int chunks = gridDim.x, chunk = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
     pdl_wait();
     pdl_trigger();
+    const float *w = weights + b * w_sb + head * w_sh;
+    float *wo = weights_out + b * wo_sb + head * wo_sh;
     int left = keep;  // to other pages the -1 of `kept` ends the rows
     const int step = chunks * kRowsCta;
     if (IN_PLACE) {
         const int n = max(min(lengths[b], static_cast<int>(min(capacity, static_cast<int64_t>(INT32_MAX)))), 0);
-        if (n <= keep) return;  // the whole cluster
+        if (n <= keep) {  // the whole cluster: the rows stay where they are, and so do the weights unless they have a place of their own
+            if (wo != w)
+                for (int i = chunk * blockDim.x + threadIdx.x; i < n; i += chunks * blockDim.x) wo[i] = w[i];
+            return;
+        }
     }
-    const float *w = weights + b * w_sb + head * w_sh;
-    float *wo = weights_out + b * wo_sb + head * wo_sh;
     const int32_t *bt = table + b * t_stride, *bo = out_table + b * o_stride;
     const int32_t *kp = kept + (static_cast<int64_t>(b) * pg.n_kv + head) * keep;
     const bool is_v = warp >= kWarps / 2;
@@ -600,6 +604,8 @@ extern "C" int t2c_kv_cache_evict_q8(const t2c_q8_pages *pages, const float *wei
     if (in_place && ot_stride != bt_stride) return set_error(T2C_EINVAL, "kv_cache_evict_q8: one table with two strides");
     if (!in_place && weights == weights_out)
         return set_error(T2C_EINVAL, "kv_cache_evict_q8: weights in place need the codes in place");
+    if (weights == weights_out && ((B > 1 && w_sb != wo_sb) || (pg.n_kv > 1 && w_sh != wo_sh)))
+        return set_error(T2C_EINVAL, "kv_cache_evict_q8: one tensor of weights with two strides");
     const int64_t heads = B * pg.n_kv;
     // CTAs that select for a head: up to 8 while the SMs have room and each keeps 2048 positions (select, move and read back,
     // 8 heads: 16007 positions of 4 sequences 55 us, one CTA a head 62, eight 70; 60000 of one 70, one CTA 160; 1003 of one
