@@ -67,3 +67,30 @@ def test_evict_refuses_one_tensor_with_two_strides():
     with pytest.raises(RuntimeError, match="strides"):
         kernels.kv_cache_evict_q8(device_pages(cache), buf.view(2, 2, 64), i32([60, 60]), table.cuda(), keep=32,
                                   weights_out=buf[:128].view(2, 2, 32))
+
+
+def test_evict_in_place_through_a_view_of_the_table():
+    """A view that begins where the block table does names the same pages: the move is in place, the weights too."""
+    from torch2vk_b200 import kernels
+
+    B, NK, page, dim, block, width, keep = 3, 2, 32, 64, 16, 6, 40
+    lengths = [190, 40, 41]
+    cache, table = ref.pool(B * width, NK, page, dim, block, seed=211), ref.tables(B, width, 0, seed=212)
+    w = _weights(B, NK, width * page, 213)
+    pages, bt, wd = device_pages(cache), table.cuda(), w.cuda()
+    kept, left = kernels.kv_cache_evict_q8(pages, wd, i32(lengths), bt, keep=keep, sinks=2, recent=8, out_table=bt[:, :2])
+    clean()
+    chosen, want_left = ref.evict(cache, w, lengths, table, table, keep=keep, sinks=2, recent=8)
+    assert left.cpu().tolist() == want_left
+    _check_kept(kept, wd, chosen, w, keep)
+    same_cache(pages, cache)
+
+
+def test_evict_to_other_pages_needs_a_place_for_the_weights():
+    from torch2vk_b200 import kernels
+
+    cache, both = ref.pool(16, 2, 16, 64, 16, seed=215), ref.tables(2, 8, 0, seed=216).cuda()
+    w = torch.zeros(2, 2, 64, device="cuda")
+    with pytest.raises(ValueError, match="weights_out"):
+        kernels.kv_cache_evict_q8(device_pages(cache), w, i32([60, 60]), both[:, :4].contiguous(), keep=32,
+                                  out_table=both[:, 4:].contiguous())

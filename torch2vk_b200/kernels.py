@@ -1044,8 +1044,9 @@ def kv_cache_evict_q8(pages: Q8Pages, weights: torch.Tensor, lengths: torch.Tens
                       new_lengths: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Cuts each sequence to at most `keep` positions per KV head: the first `sinks`, the last `recent` and of the
     others those with the largest weights [B, n_kv, positions] (ties: the lowest positions).  The rows move to
-    positions 0.. of out_table's pages (default: block_table's own, in place; another table's pages must be
-    disjoint from them), their weights to weights_out (default in place: weights itself).
+    positions 0.. of out_table's pages, their weights to weights_out.  Without out_table, or with one that begins where
+    block_table does, that is in place, and weights_out is weights itself unless given; another table's pages must be
+    disjoint from block_table's, and weights_out must be given.
     Returns (kept positions int32 [B, n_kv, keep], ascending then -1; new lengths int32 [B])."""
     heads = pages.n_kv
     batch = lengths.numel()
@@ -1056,7 +1057,9 @@ def kv_cache_evict_q8(pages: Q8Pages, weights: torch.Tensor, lengths: torch.Tens
     if out_table is None:
         out_table = block_table
     if weights_out is None:
-        weights_out = weights if out_table is block_table else weights.new_empty((batch, heads, keep))
+        if out_table.data_ptr() != block_table.data_ptr():
+            raise ValueError("an out_table of other pages needs a weights_out")
+        weights_out = weights
     if weights_out.dtype != torch.float32 or weights_out.dim() != 3 or weights_out.stride(2) != 1 \
             or weights_out.shape[0] < batch or weights_out.shape[1] != heads or weights_out.shape[2] < keep:
         raise ValueError(f"weights_out must be float32 [batch, {heads}, at least {keep}] with unit last stride")
