@@ -5,6 +5,7 @@
 #include <type_traits>
 
 #include "kv8.cuh"
+#include "kv8_parts.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -121,6 +122,7 @@ struct DecodeArgs {
     int splits;       // CTAs per unit in a cluster; 0: tile runs, joined by the second kernel
     int head_chunks;  // chunks of 8 heads of a group
     int ctas;         // of the tile runs
+    int most_parts;   // of a unit
     float *parts;     // [2 * ctas][kPart]
     int2 *unit_ctas;  // [B * n_kv * head_chunks] first and last CTA of a unit's tiles
     float *unit_lse;  // [B][NH] in log2 units, of units one CTA finished; where the weights are wanted
@@ -536,12 +538,13 @@ __global__ void __launch_bounds__(kJoinThreads) attn8_join_kernel(const __grid_c
     pdl_wait();  // positions were there before the kernel whose parts are joined
     pdl_trigger();
     const int2 own = ctas[first >> 3];
-    if (is_out && own.x == own.y) return;  // a unit of one CTA is written
+    const int count = kv8_part_count(own.x, own.y, p.ctas, p.most_parts);
+    if (is_out && count <= 1) return;  // a unit of one CTA is written, one whose CTA gave up has no result
     // part i of a unit whose tiles begin in CTA c0: that CTA's last one, then the others' first
     const auto part_of = [&](int c0, int i) { return p.parts + (2 * static_cast<int64_t>(c0 + i) + (i == 0 ? 1 : 0)) * kPart; };
 
     // a quarter: every kShare-th part of the block's head, or all parts of its own head
-    const int d = threadIdx.x % D, q = threadIdx.x / D, count = own.y - own.x + 1;
+    const int d = threadIdx.x % D, q = threadIdx.x / D;
     const int mine = ALONE ? first : min(first + q, group - 1), part0 = ALONE ? q : 0;
     constexpr int step = ALONE ? kShare : 1;
     float ahead[kAhead];
@@ -552,9 +555,9 @@ __global__ void __launch_bounds__(kJoinThreads) attn8_join_kernel(const __grid_c
     }
     for (int h = first + warp; h < last; h += kJoinThreads / 32) {
         const int2 c = ctas[h >> 3];
-        const int parts = c.y - c.x + 1;
-        if (parts == 1) {
-            if (lane == 0) ref[h] = p.unit_lse[static_cast<int64_t>(b) * a.NH + head * group + h];
+        const int parts = kv8_part_count(c.x, c.y, p.ctas, p.most_parts);
+        if (parts <= 1) {  // without a result: no probability
+            if (lane == 0) ref[h] = parts == 1 ? p.unit_lse[static_cast<int64_t>(b) * a.NH + head * group + h] : INFINITY;
             continue;
         }
         float top = kRefStart, s = 0.0f, m0 = kRefStart, l0 = 0.0f;
@@ -707,7 +710,9 @@ extern "C" int t2c_attn_decode_q8(const t2c_q8_pages *pages, const void *q, int6
     a.positions = positions, a.table = block_table, a.t_stride = bt_stride, a.max_len = max_len;
     a.B = static_cast<int>(B), a.T = 1, a.NH = static_cast<int>(NH);
     a.scale_log2 = scale * 1.4426950408889634f;
+    const int64_t tiles = (max_len + kDTile - 1) / kDTile;
     p.splits = plan.splits, p.head_chunks = plan.head_chunks, p.ctas = plan.ctas;
+    p.most_parts = static_cast<int>(p.ctas < tiles ? p.ctas : tiles);
     p.parts = workspace;
     p.unit_ctas = reinterpret_cast<int2 *>(workspace + plan.part_floats);
     p.unit_lse = workspace + plan.part_floats + plan.unit_floats;
@@ -731,8 +736,8 @@ extern "C" int t2c_attn_decode_q8(const t2c_q8_pages *pages, const void *q, int6
     if (rc != T2C_OK || clusters) return rc;
     // A block per head while those fit the SMs at once, then a block for as many as it has quarters (32 sequences of up to 6007,
     // 32 heads on 8: 49 us, with a block per head 54; 32801 positions of one 24, else 26).
-    const int64_t chunks = weights_out ? (max_len + kJoinKeys - 1) / kJoinKeys : 0, tiles = (max_len + kDTile - 1) / kDTile;
-    const int64_t parts = p.ctas < tiles ? p.ctas : tiles, quarters = kJoinThreads / D;
+    const int64_t chunks = weights_out ? (max_len + kJoinKeys - 1) / kJoinKeys : 0;
+    const int64_t parts = p.most_parts, quarters = kJoinThreads / D;
     const bool alone = B * NH <= 4 * sm_count() || quarters * parts * 4 > 32768;
     const int64_t heads = alone ? 1 : quarters;
     const auto join = D == 128 ? (alone ? attn8_join_kernel<128, true> : attn8_join_kernel<128, false>)
