@@ -305,6 +305,9 @@ __global__ void __launch_bounds__(kDThreads, 4) attn8_decode_kernel(const __grid
                 }
                 const bool arrived = mbar_wait(&full[warp][st], (phases >> st) & 1u);
                 if (!__all_sync(0xffffffffu, arrived)) {
+                    // the copies of this step and of those loaded ahead end (or are given up) before the CTA may
+                    for (int k = 0; k < kDStages && i + k < mine; ++k)
+                        mbar_wait(&full[warp][(st + k) % kDStages], (phases >> ((st + k) % kDStages)) & 1u);
                     failed = true;
                     break;
                 }

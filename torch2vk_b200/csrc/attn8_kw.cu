@@ -108,6 +108,7 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
         const int first = t <= 0 ? 0 : static_cast<int>(t / TT);
         return first + static_cast<int>(static_cast<int64_t>(nq - first) * of / C);
     };
+    int loads = 0;  // query tiles that warp 4 has fetched
     if (kt0 < kt1) {
         if (warp < 4) {
             constexpr int kPerRow = D / 16, kRowsPass = 32 / kPerRow, kPasses = 32 / kRowsPass;
@@ -232,12 +233,14 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
                 }
             }
         } else if (warp == 4) {
-            int count = 0;
             const float *lse = a.lse + static_cast<int64_t>(b) * a.NH * a.T + static_cast<int64_t>(head) * group * a.T;
-            for (int kt = kt0; kt < kt1; ++kt) {
-                for (int q = share(kt, rank), q_end = share(kt, rank + 1); q < q_end; ++q, ++count) {
-                    const int slot = count & 1;
-                    if (count >= 2) mbar_wait_or(&q_free[slot], ((count >> 1) - 1) & 1, stop);
+            bool on = true;
+            for (int kt = kt0; kt < kt1 && on; ++kt) {
+                for (int q = share(kt, rank), q_end = share(kt, rank + 1); q < q_end; ++q, ++loads) {
+                    const int slot = loads & 1;
+                    if (loads >= 2) on = mbar_wait_or(&q_free[slot], ((loads >> 1) - 1) & 1, stop);
+                    on = __all_sync(0xffffffffu, on);
+                    if (!on) break;  // no copy over one that may still be in flight
                     if (lane == 0) {
                         mbar_arrive_expect_tx(&q_full[slot], static_cast<uint32_t>(TT * group * D * 2));
 #pragma unroll
@@ -245,7 +248,7 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
                             tma_load_4d(base + S::kQ + slot * S::kTile + i * 16384, &q_map, 64 * i, head * group, q * TT, b, &q_full[slot]);
                     }
                     // (the ring of 8 outlives its readers) minus the log-sum-exp in log2 units; -inf (weight 0) for rows past the end and rows that see nothing
-                    float *dst = reinterpret_cast<float *>(smem + S::kLse + (count & 7) * 512);
+                    float *dst = reinterpret_cast<float *>(smem + S::kLse + (loads & 7) * 512);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int r = 32 * i + lane, t = q * TT + r / group;
@@ -303,7 +306,11 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (tid == 0 && *stop) report_device_error(T2C_ETIMEOUT);
+    if (*stop) {
+        if (tid == 0) report_device_error(T2C_ETIMEOUT);
+        if (warp == 4)  // the last copies end (or are given up) before the CTA may
+            for (int i = max(loads - 2, 0); i < loads; ++i) mbar_wait(&q_full[i & 1], (i >> 1) & 1);
+    }
     if (warp == 5) {
         __syncwarp();
         tmem_free(tmem, 256);

@@ -171,12 +171,15 @@ __device__ __forceinline__ bool mbar_tries(uint64_t *bar, uint32_t parity) {
 }
 // Waits for a phase of `bar`: gives up after two seconds, or when another wait of the CTA did, with *stop set.  The
 // caller goes on either way (every later wait then returns at once) and looks at *stop before it writes results, so
-// that no branch hangs on a wait.
-__device__ __forceinline__ void mbar_wait_or(uint64_t *bar, uint32_t parity, volatile int *stop) {
-    if (mbar_tries(bar, parity)) return;
+// that no branch hangs on a wait; or it goes by what is returned, false for a wait that gave up.
+__device__ __forceinline__ bool mbar_wait_or(uint64_t *bar, uint32_t parity, volatile int *stop) {
+    if (mbar_tries(bar, parity)) return true;
     const uint64_t start = global_timer_ns();
-    while (!*stop && !mbar_tries(bar, parity))
+    while (!*stop) {
+        if (mbar_tries(bar, parity)) return true;
         if (global_timer_ns() - start > 2000000000ull) *stop = 1;
+    }
+    return false;
 }
 
 }  // namespace t2c
