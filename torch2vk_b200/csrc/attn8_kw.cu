@@ -293,6 +293,19 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
             mbar_wait_or(all_done, 0, stop_last);  // nothing of this CTA is in flight when it frees its TMEM
         }
     }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (*stop) {
+        if (tid == 0) report_device_error(T2C_ETIMEOUT);
+        if (warp == 4)  // the last copies end (or are given up) before the CTA may
+            for (int i = max(loads - 2, 0); i < loads; ++i) mbar_wait(&q_full[i & 1], (i >> 1) & 1);
+        __syncwarp();
+    }
+    if (warp == 5) {
+        __syncwarp();
+        tmem_free(tmem, 256);
+    }
+    // (TMEM is free before the wait for the cluster: its CTAs may be waiting for TMEM that other clusters' CTAs hold)
     if (C > 1) {
         cluster.sync();
         const int64_t key = static_cast<int64_t>(kt0) * 128 + tid;
@@ -303,17 +316,6 @@ __global__ void __launch_bounds__(kWThreads, 2) attn8_weights_kernel(const __gri
             a.w_out[o] = weight + (a.w_in && key < p0 ? a.w_in[o] : 0.0f);
         }
         cluster.sync();  // no CTA leaves while another may read its shared memory
-    }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    if (*stop) {
-        if (tid == 0) report_device_error(T2C_ETIMEOUT);
-        if (warp == 4)  // the last copies end (or are given up) before the CTA may
-            for (int i = max(loads - 2, 0); i < loads; ++i) mbar_wait(&q_full[i & 1], (i >> 1) & 1);
-    }
-    if (warp == 5) {
-        __syncwarp();
-        tmem_free(tmem, 256);
     }
 }
 
