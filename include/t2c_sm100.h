@@ -602,7 +602,8 @@ int t2c_kv_cache_read_q8(const t2c_q8_pages *pages, void *k_out, void *v_out, co
  * Attention of T queries per sequence over the cache: query t of sequence b sees positions 0 .. positions[b] + t
  * (its own row is already cached); grouped heads (NH % n_kv == 0, query head h reads KV head h / (NH / n_kv)).
  *   out = softmax(scale * q k^T) v, lse = log sum exp of the scaled scores (natural log; NULL: not stored).
- * A query that sees nothing (negative position) gives out 0 and lse -inf.
+ * A query that sees nothing (negative position) gives out 0 and lse -inf.  A V block that reads as NaN makes out NaN where
+ * it is seen, and neither lse nor the weights below; a K block of NaN makes all three NaN for its head.
  * q, out fp16 with element strides (multiples of 8, unit along head_dim); lse fp32 [B, NH, T].
  * max_len > 0: no sequence has more than max_len positions (longer ones are cut to it and reported).
  * splits: CTAs that share one sequence's keys, 0 = chosen by the library; workspace: at least

@@ -5,10 +5,12 @@ attention within the bounds that tests/test_kv8_gpu.py derives."""
 
 from __future__ import annotations
 
+import math
+
 import kv8_ref as ref
 import pytest
 import torch
-from test_kv8_gpu import clean, device_pages, i32, same_cache
+from test_kv8_gpu import attention_case, check_attention, check_weights, clean, device_pages, i32, same_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +96,72 @@ def test_evict_to_other_pages_needs_a_place_for_the_weights():
     with pytest.raises(ValueError, match="weights_out"):
         kernels.kv_cache_evict_q8(device_pages(cache), w, i32([60, 60]), both[:, :4].contiguous(), keep=32,
                                   out_table=both[:, 4:].contiguous())
+
+
+# ------------------------------------------------------------------ blocks that read as NaN
+def _seen_nan(out, lse, want, poisoned):
+    """out is NaN where `poisoned` [B, T, NH] and nowhere else; the rest, and every log-sum-exp, as without the NaN."""
+    mask = poisoned.unsqueeze(-1).expand(out.shape)
+    assert torch.equal(torch.isnan(out).cpu(), mask)
+    check_attention(torch.where(mask, want["out"].half(), out.cpu()), lse, want)
+
+
+@pytest.mark.parametrize("NH,NK,dim", [(16, 8, 128), (6, 2, 64), (24, 2, 128)])
+@pytest.mark.parametrize("splits", [0, 1, 3])
+def test_nan_values_leave_scores_alone(NH, NK, dim, splits):
+    """A V block of NaN makes the outputs that see it NaN and nothing else: log-sum-exps, the weights a decode step adds
+    and the key weights come from the scores, so they stay what they are."""
+    from torch2vk_b200 import kernels
+
+    page, block, T, width = 64, 16, 37, 6
+    positions = [20, 300, -3]
+    cache, table, g, _ = attention_case(3, NH, NK, dim, page, block, width, 221)
+    q = torch.randn(3, T, NH, dim, generator=g).half()
+    want = ref.attention(cache, q, positions, table, dim ** -0.5)
+    cache["vs"][table[0, 0], 0, 1] = math.nan  # keys 16 .. 31 of KV head 0: seen by all queries
+    cache["vs"][table[1, 5], 1, 0] = math.nan  # keys 320 .. 335 of KV head 1: seen from query 20 on
+    cache["v"][table[1, 5], 1, :16] = 0
+    group = NH // NK
+    poisoned = torch.zeros(3, T, NH, dtype=torch.bool)
+    poisoned[0, :, :group] = True
+    poisoned[1, 20:, group: 2 * group] = True
+    pages, bt = device_pages(cache), table.cuda()
+    out, lse = kernels.attn_prefill_q8(q.cuda(), pages, i32(positions), bt, splits=splits, return_lse=True)
+    clean()
+    _seen_nan(out, lse, want, poisoned)
+    before = torch.rand(3, NK, width * page, generator=g)
+    w = before.cuda()
+    kernels.attn_key_weights_q8(q.cuda(), lse, pages, i32(positions), bt, weights=w, weights_out=w)
+    clean()
+    check_weights(w, before, want, positions, T, NK)
+
+    last = [p + T - 1 for p in positions]
+    w, lse1 = before.cuda(), torch.empty(3, NH, device="cuda")
+    out1 = kernels.attn_decode_q8(q[:, -1].cuda(), pages, i32(last), bt, splits=splits, lse=lse1, weights=w, weights_out=w)
+    clean()
+    one = {n: (x[:, -1:] if n in ("out", "spread") else x[:, :, -1:]) for n, x in want.items() if n != "probs"}
+    one["probs"] = [p[:, -1:] for p in want["probs"]]
+    _seen_nan(out1.unsqueeze(1), lse1.unsqueeze(-1), one, poisoned[:, -1:])
+    check_weights(w, before, one, last, 1, NK)
+
+
+def test_nan_values_in_a_short_cache():
+    """The same where one launch joins a cluster: 200 keys, the NaN block in one CTA's tile."""
+    from torch2vk_b200 import kernels
+
+    NH, NK, dim, page, block = 8, 2, 128, 32, 32
+    cache, table, g, _ = attention_case(2, NH, NK, dim, page, block, 7, 225)
+    q = torch.randn(2, NH, dim, generator=g).half()
+    positions = [199, 120]
+    want = ref.attention(cache, q.unsqueeze(1), positions, table, dim ** -0.5)
+    cache["vs"][table[0, 4], 1, 0] = math.nan  # keys 128 .. 159 of KV head 1
+    cache["vs"][table[1, 4], :, 0] = math.nan  # past the keys of sequence 1
+    poisoned = torch.zeros(2, 1, NH, dtype=torch.bool)
+    poisoned[0, :, 4:] = True
+    pages, bt = device_pages(cache), table.cuda()
+    before = torch.rand(2, NK, 7 * page, generator=g)
+    w, lse = before.cuda(), torch.empty(2, NH, device="cuda")
+    out = kernels.attn_decode_q8(q.cuda(), pages, i32(positions), bt, lse=lse, weights=w, weights_out=w)
+    clean()
+    _seen_nan(out.unsqueeze(1), lse.unsqueeze(-1), want, poisoned)
+    check_weights(w, before, want, positions, 1, NK)

@@ -250,12 +250,17 @@ __global__ void __launch_bounds__(kDThreads, 4) attn8_decode_kernel(const __grid
             next_ks = a.pg.ks[so];
             next_vs = a.pg.vs[so];
         };
+        bool nan_values = false;  // a V block of this lane's steps reads as NaN
         const auto store_meta = [&](int window) {
             const float vs = __half2float(next_vs);
-            // a block of scale 0 has values 0: any exponent adds nothing to O, the least scale's moves no reference
+            // a block of scale 0 has values 0: any exponent adds nothing to O, the least scale's moves no reference.  One of
+            // NaN is taken alike, so that the softmax's statistics, which are the scores' alone, stay theirs; O becomes NaN
+            // at the end.
+            const bool flat = vs == 0.0f || vs != vs;
+            nan_values |= vs != vs && window * 32 + lane < mine;
             meta[(window & 1) * 32 + lane] =
-                make_float4(__half2float(next_ks) * a.scale_log2, vs == 0.0f ? -24.0f : log2f(vs),
-                            vs == 0.0f ? 16777216.0f : 1.0f / vs, __int_as_float(next_page));
+                make_float4(__half2float(next_ks) * a.scale_log2, flat ? -24.0f : log2f(vs),
+                            flat ? 16777216.0f : 1.0f / vs, __int_as_float(next_page));
             __syncwarp();
         };
         const auto load = [&](int i, int stage, int page) {  // by one lane
@@ -385,6 +390,10 @@ __global__ void __launch_bounds__(kDThreads, 4) attn8_decode_kernel(const __grid
                 if (lane == 0 && i + kDStages < mine)
                     load(i + kDStages, st, __float_as_int(meta[(i + kDStages) & 63].w));
             }
+        }
+        if (__any_sync(0xffffffffu, nan_values)) {
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) o[w][0] = o[w][1] = o[w][2] = o[w][3] = __int_as_float(0x7fffffff);
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {

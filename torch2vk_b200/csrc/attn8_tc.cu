@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
              *s_ready = bars + 11, *p_ready = bars + 14, *q_full = bars + 17, *meta_full = bars + 18;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 22);
     volatile int *stop = reinterpret_cast<volatile int *>(bars + 23), *stop_last = stop + 1;
+    int *nan_from = reinterpret_cast<int *>(bars + 24);  // first key of this CTA's tiles whose V reads as NaN
     if (base & 1023u) {  // the swizzle atoms need it: report, compute nothing
         if (threadIdx.x == 0) report_device_error(T2C_EUNSUPPORTED);
         return;
@@ -112,6 +113,7 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
         mbar_init(q_full, 256);
         for (int i = 0; i < 4; ++i) mbar_init(meta_full + i, 8);
         *stop = 0;
+        *nan_from = INT32_MAX;
         fence_mbar_init();
     }
     if (warp == 16) tmem_alloc(tmem_slot, 512);
@@ -216,8 +218,8 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                                 tmem_ld_wait();  // the load ahead
                                 return 2 * c;
                             }
-                            if (!hide || 32 * c <= last) l = fmaf(total[c & 1][0], iv[2 * c], l);  // an unseen block may have any scale
-                            if (!hide || 32 * c + 16 <= last) l = fmaf(total[c & 1][1], iv[2 * c + 1], l);
+                            l = fmaf(total[c & 1][0], iv[2 * c], l);
+                            l = fmaf(total[c & 1][1], iv[2 * c + 1], l);
                             tmem_st16(s_at + 16 * c, p[c & 1]);
                         }
                         if (r < 4) {
@@ -320,7 +322,7 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                             sum += a0 + a1;
                             p[i] = ph_bits(__floats2half2_rn(a0, a1));
                         }
-                        if (16 * c <= last) l = fmaf(sum, fi[c], l);
+                        l = fmaf(sum, fi[c], l);
                         tmem_st8(s_at + 8 * c, p);
                     }
                 };
@@ -338,7 +340,7 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
             mbar_wait_or(o_done, 0, stop);
             if (!__any_sync(0xffffffffu, *stop != 0)) {
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const bool seen = limit >= 0;
+                const bool seen = limit >= 0, poisoned = limit >= *nan_from;  // (written before the factors of those keys)
                 if (a.splits > 1) {
                     float *part = a.parts + (((static_cast<int64_t>(b) * a.pg.n_kv + head) * a.pairs + pair) * a.splits + split) *
                                                 (256 * (D + 2));
@@ -348,6 +350,10 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                         uint32_t v[32];
                         tmem_ld32(o_at + 32 * c, v);
                         tmem_ld_wait32(v);
+                        if (poisoned) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = 0x7fffffffu;
+                        }
                         if (real) {
 #pragma unroll
                             for (int i = 0; i < 8; ++i)
@@ -357,7 +363,7 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
                     part[256 * D + qi * 128 + row] = m;
                     part[256 * (D + 1) + qi * 128 + row] = l;
                 } else {
-                    const float inv = seen ? 1.0f / l : 0.0f;
+                    const float inv = poisoned ? __int_as_float(0x7fffffff) : (seen ? 1.0f / l : 0.0f);
                     __half *o = a.out + b * a.o_sb + static_cast<int64_t>(t) * a.o_st + h * a.o_sh;
 #pragma unroll 1
                     for (int c = 0; c < D / 32; ++c) {
@@ -439,9 +445,16 @@ __global__ void __launch_bounds__(kPThreads, 1) attn8_prefill_kernel(const __gri
             for (int j = 0; j < tiles; ++j) {
                 const int st = j & 1;
                 if (lane == 0) {  // the factors of these 16 keys (the ring of 4 outlives their readers)
-                    // a block of scale 0 has values 0: the least scale's exponent moves no reference
+                    // a block of scale 0 has values 0: the least scale's exponent moves no reference.  One of NaN is taken
+                    // alike, so that the softmax's statistics, which are the scores' alone, stay theirs; rows that see it
+                    // get NaN at the end.
                     const bool some = key < n;
-                    const float v = some ? __half2float(vs) : 0.0f, kf = some ? __half2float(ks) * a.scale_log2 : 0.0f;
+                    float v = some ? __half2float(vs) : 0.0f;
+                    const float kf = some ? __half2float(ks) * a.scale_log2 : 0.0f;
+                    if (v != v) {
+                        atomicMin(nan_from, static_cast<int>(key));
+                        v = 0.0f;
+                    }
                     const float lv = v == 0.0f ? -24.0f : log2f(v);
                     meta[(j & 3) * 8 + slice] = make_ulonglong2(f32x2(kf, kf), f32x2(lv, lv));
                     inv_vs[(j & 3) * 8 + slice] = v == 0.0f ? 16777216.0f : 1.0f / v;
