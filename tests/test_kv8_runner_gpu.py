@@ -170,3 +170,29 @@ def test_runner_refusals():
         _runner(kv_bits=8, kv_budget=256)
     with pytest.raises(ValueError, match="8-bit"):
         r.prefill(_ids(cfg, 2, 8, 6), append=True)
+
+
+def test_appended_prompts_stage_their_own_rows():
+    """The memory that a continued prompt takes goes by its tokens, not by how long the conversation has become."""
+    cfg, r = _runner(kv_bits=8, kv_budget=64, kv_recent=16)
+    ids = _ids(cfg, 2, 20, 7)
+    r.prefill(ids)
+
+    def peak():
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        r.prefill(ids, append=True)
+        torch.cuda.synchronize()
+        return torch.cuda.max_memory_allocated() - before
+
+    peak()  # buffers that stay
+    first = peak()
+    for _ in range(110):
+        r.step()
+    for _ in range(8):
+        last = peak()
+    assert r.length > 300 and r.cached <= 80
+    # what is not bound to the tokens: lists of kept rows where an eviction follows, 4 bytes a row and KV head
+    assert last <= first + 2 * cfg.kv_heads * 64 * 4 * cfg.layers + 4096
+    _clean()

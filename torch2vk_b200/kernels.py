@@ -175,17 +175,21 @@ def cache_strides(cache: torch.Tensor, layout: str) -> tuple[int, int, int]:
 def qk_norm_rope_cache(q_in: torch.Tensor, k_in: torch.Tensor, v_in: torch.Tensor, q_w: torch.Tensor,
                        k_w: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, positions: torch.Tensor,
                        inv_freq: torch.Tensor, *, batch: int, tokens: int, n_heads: int, n_kv: int, head_dim: int,
-                       layout: str = "token_major", eps: float = 1e-6,
+                       layout: str = "token_major", eps: float = 1e-6, first_row: int = 0,
                        q_out: torch.Tensor | None = None) -> torch.Tensor:
-    """q/k RMSNorm + RoPE; rotated k and raw v written into the caches at positions[b] + t."""
+    """q/k RMSNorm + RoPE; rotated k and raw v written into the caches at positions[b] + t.
+
+    first_row: the position that row 0 of the caches stands for, so that rows for late positions need no rows before
+    them; no position may lie before it."""
     for t, n in ((q_in, "q_in"), (k_in, "k_in"), (v_in, "v_in")):
         _check(t, torch.float16, n)
     _check(positions, torch.int32, "positions")
     _check(inv_freq, torch.float32, "inv_freq")
     q_out = torch.empty_like(q_in) if q_out is None else q_out
     cb, cs, ch = cache_strides(k_cache, layout)
+    before = first_row * cs * k_cache.element_size()  # bytes from where row 0 would be to first_row
     _lib.lib().call("t2c_qk_norm_rope_cache", _lib.ptr(q_in), _lib.ptr(k_in), _lib.ptr(v_in), _lib.ptr(q_w),
-                    _lib.ptr(k_w), _lib.ptr(q_out), _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(positions),
+                    _lib.ptr(k_w), _lib.ptr(q_out), _lib.ptr(k_cache) - before, _lib.ptr(v_cache) - before, _lib.ptr(positions),
                     batch, tokens, n_heads, n_kv, head_dim, cb, cs, ch, _lib.ptr(inv_freq), float(eps),
                     _lib.stream_ptr())
     return q_out

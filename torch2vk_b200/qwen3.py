@@ -309,13 +309,13 @@ class Qwen3Runner:
             vs = self.v_stage.as_strided((self.batch, self.max_seq, nk, d), (nk * d, 0, d, 1))
             new = [s.view(self.batch, 1, nk, d) for s in (self.k_stage, self.v_stage)]
         else:
-            done = self.length  # the staging rows are addressed by position
-            ks = torch.empty(self.batch, done + tokens_per_seq, nk, d, dtype=torch.float16, device=self.device)
+            ks = torch.empty(self.batch, tokens_per_seq, nk, d, dtype=torch.float16, device=self.device)
             vs = torch.empty_like(ks)
-            new = [s[:, done:] for s in (ks, vs)]
+            new = [ks, vs]
+        # staging rows are addressed by position: the prompt's first row is its first position, the step's only row any
         kernels.qk_norm_rope_cache(b.q, b.k, b.v, lw.q_norm, lw.k_norm, ks, vs, self.positions, self.inv_freq,
                                    batch=self.batch, tokens=tokens_per_seq, n_heads=nh, n_kv=nk, head_dim=d, eps=cfg.eps,
-                                   q_out=b.qr)
+                                   first_row=0 if decode else self.length, q_out=b.qr)
         kernels.kv_cache_write_q8(pages, new[0], new[1], self.slots, bt)
         if decode:
             kernels.attn_decode_q8(b.qr.view(self.batch, nh, d), pages, self.slots, bt, max_len=self._max_cached(),
