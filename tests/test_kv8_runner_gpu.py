@@ -196,3 +196,16 @@ def test_appended_prompts_stage_their_own_rows():
     # what is not bound to the tokens: lists of kept rows where an eviction follows, 4 bytes a row and KV head
     assert last <= first + 2 * cfg.kv_heads * 64 * 4 * cfg.layers + 4096
     _clean()
+
+
+def test_pool_sized_for_the_budget():
+    """With a budget a sequence takes the pages of its bound (or of a longer prompt), however many tokens may follow."""
+    cfg, r = _runner(kv_bits=8, kv_budget=64, kv_recent=16, kv_pages=10)  # 80 rows for each of two sequences
+    _, wide = _runner(kv_bits=8, kv_budget=64, kv_recent=16)
+    ids = _ids(cfg, 2, 50, 8)
+    tokens = r.generate(ids, 100)
+    assert torch.equal(tokens, wide.generate(ids, 100))
+    assert r.paged.free_pages == 0 and r.cached <= 80
+    r.prefill(ids[:, :10].contiguous(), append=True)
+    r.step()
+    _clean()

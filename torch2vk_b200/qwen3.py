@@ -349,7 +349,6 @@ class Qwen3Runner:
         self.cached = min(self.cached, self.kv_budget)
         for s in range(self.batch):
             pool.shrink(s, self._max_cached())
-            pool.reserve(s, self._max_cached())
 
     def _reserve_pages(self, positions: int) -> None:
         """Every sequence gets pages for `positions` positions, handed out round-robin (sequence b's pages
@@ -398,11 +397,14 @@ class Qwen3Runner:
             self.slots.zero_()
         elif self.cached + tokens > self.max_seq:
             raise ValueError(f"prompt of {tokens} tokens on {self.cached} cached exceeds max_seq {self.max_seq}")
+        # pages for the prompt and what may follow it: max_new_tokens rows, or with a budget up to its bound
+        rows = self.cached + tokens
+        rows = max(rows, self._max_cached()) if self.kv_budget else min(self.max_seq, rows + self.max_new_tokens)
         if append:
             for s in range(self.batch):
-                self.paged.reserve(s, min(self.max_seq, self.cached + tokens + self.max_new_tokens))
+                self.paged.reserve(s, rows)
         elif self.paged is not None:
-            self._reserve_pages(min(self.max_seq, tokens + self.max_new_tokens))
+            self._reserve_pages(rows)
         self.token_index.zero_()
         self.generated_length.zero_()
         self.stopped.zero_()
