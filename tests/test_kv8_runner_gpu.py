@@ -209,3 +209,17 @@ def test_pool_sized_for_the_budget():
     r.prefill(ids[:, :10].contiguous(), append=True)
     r.step()
     _clean()
+
+
+def test_generation_past_max_seq_with_a_budget():
+    """max_seq bounds the cached rows; with a budget a generation may be longer."""
+    cfg, r = _runner(max_seq=96, kv_bits=8, kv_budget=64, kv_recent=16)
+    _, wide = _runner(max_seq=256, kv_bits=8, kv_budget=64, kv_recent=16)
+    ids = _ids(cfg, 2, 60, 9)
+    tokens = r.generate(ids, 110).clone()
+    assert r.length == 169 and int(r.positions[0]) == 169 and r.cached <= 80
+    assert torch.equal(tokens, wide.generate(ids, 110))
+    _, free = _runner(max_seq=96, kv_bits=8)
+    with pytest.raises(ValueError, match="max_seq"):
+        free.generate(ids, 110)
+    _clean()

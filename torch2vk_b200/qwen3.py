@@ -143,7 +143,8 @@ class Qwen3Runner:
         then attend over the quantized cache too, and prefill(append=True) continues on what is cached.  kv_budget > 0
         bounds each sequence's cached positions: the attention weight each key receives is kept (a prompt's from its
         last kv_window queries, then every decoded token's), and a sequence that has grown to kv_budget plus a page
-        is cut to kv_budget positions per KV head, the first kv_sinks and the last kv_recent always among them."""
+        is cut to kv_budget positions per KV head, the first kv_sinks and the last kv_recent always among them.  max_seq
+        then bounds a prompt with what is cached before it, not the tokens of a conversation."""
         cfg, dev = self.cfg, self.weights.final_norm.device
         self.device = dev
         self.paged: PagedKVCache | None = None
@@ -490,10 +491,12 @@ class Qwen3Runner:
         self._count_step()
 
     def generate(self, prompt: torch.Tensor, max_new_tokens: int) -> torch.Tensor:
-        """Prefill + (max_new_tokens - 1) graph-replayed decode steps; returns [batch, max_new_tokens]."""
+        """Prefill + (max_new_tokens - 1) graph-replayed decode steps; returns [batch, max_new_tokens].
+
+        Prompt and new tokens fit max_seq together, or with kv_budget the prompt alone: the cut cache holds the rest."""
         if max_new_tokens > self.max_new_tokens:
             raise ValueError(f"max_new_tokens {max_new_tokens} > capacity {self.max_new_tokens}")
-        if prompt.shape[1] + max_new_tokens > self.max_seq:
+        if not self.kv_budget and prompt.shape[1] + max_new_tokens > self.max_seq:
             raise ValueError("prompt + new tokens exceed max_seq")
         self.prefill(prompt)
         for _ in range(max_new_tokens - 1):
