@@ -223,3 +223,9 @@ def test_generation_past_max_seq_with_a_budget():
     with pytest.raises(ValueError, match="max_seq"):
         free.generate(ids, 110)
     _clean()
+
+
+@pytest.mark.parametrize("bad", [dict(kv_window=0), dict(kv_window=-1), dict(kv_sinks=-1), dict(kv_recent=-2)])
+def test_runner_refuses_bad_windows(bad):
+    with pytest.raises(ValueError, match="kv_window|kv_sinks"):
+        _runner(kv_bits=8, kv_budget=64, **bad)

@@ -152,6 +152,8 @@ class Qwen3Runner:
             raise ValueError("kv_bits is 16, or 8 with a paged cache (page_size > 0)")
         if self.kv_budget and (self.kv_bits != 8 or not self.kv_sinks + self.kv_recent <= self.kv_budget < self.max_seq):
             raise ValueError("kv_budget needs kv_bits=8, room for kv_sinks + kv_recent positions and fewer than max_seq")
+        if self.kv_budget and (min(self.kv_sinks, self.kv_recent) < 0 or self.kv_window < 1):
+            raise ValueError("kv_sinks and kv_recent are 0 or more, kv_window (the queries a prompt's keys are weighed by) 1 or more")
         if self.page_size > 0:
             per_seq = -(-self.max_seq // self.page_size)
             pool = dict(layers=cfg.layers, num_pages=self.kv_pages or self.batch * per_seq, page_size=self.page_size,
