@@ -229,3 +229,24 @@ def test_generation_past_max_seq_with_a_budget():
 def test_runner_refuses_bad_windows(bad):
     with pytest.raises(ValueError, match="kv_window|kv_sinks"):
         _runner(kv_bits=8, kv_budget=64, **bad)
+
+
+def test_capture_of_a_full_cache():
+    """capture() runs a step, so it makes room first: page 0, which is another sequence's, keeps what it has."""
+    cfg, r = _runner(kv_bits=8, kv_budget=64, kv_recent=16)
+    _, e = _runner(kv_bits=8, kv_budget=64, kv_recent=16)
+    ids = _ids(cfg, 2, 60, 10)
+    r.prefill(ids)
+    e.prefill(ids)
+    while r.cached < 80:
+        r.decode_step()
+        e.decode_step()
+    r.capture()
+    _clean()
+    for _ in range(10):
+        r.step()
+        e.decode_step()
+    assert torch.equal(r.generated, e.generated) and r.cached == e.cached
+    for i in range(cfg.layers):
+        assert torch.equal(r.paged.k[i], e.paged.k[i]) and torch.equal(r.paged.k_scale[i], e.paged.k_scale[i])
+    _clean()

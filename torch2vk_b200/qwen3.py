@@ -470,6 +470,7 @@ class Qwen3Runner:
         piece of step state is saved before and restored after (the KV-cache row
         they write is rewritten by the first replay).
         """
+        self._make_room()
         saved = [t.clone() for t in self._step_state()]
         side = torch.cuda.Stream(device=self.device)
         side.wait_stream(torch.cuda.current_stream(self.device))
@@ -486,9 +487,9 @@ class Qwen3Runner:
             t.copy_(v)
 
     def step(self) -> None:
-        self._make_room()
         if self._graph is None:
             self.capture()
+        self._make_room()
         self._graph.replay()
         self._count_step()
 
