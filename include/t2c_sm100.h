@@ -566,7 +566,8 @@ int t2c_linear_allreduce(int wtype, const void *x, const void *w, const void *re
  * head_stride, row_stride, multiples of 16, shared by k and v; unit stride along head_dim), with one fp16 scale
  * for each `block` consecutive tokens of a KV head, k_scale / v_scale [num_pages][n_kv][page_size / block]
  * (strides scale_page_stride, scale_head_stride; unit last).  A code c in -127..127 stands for c * scale.
- * page_size: a power of two from 16 up; block: 16, 32 or 64, at most page_size; head_dim 64 or 128.
+ * page_size: a power of two from 16 up; block: 16, 32 or 64, at most page_size; head_dim 64 or 128.  Here and below the
+ * stride of a dimension of one entry does not count.
  * block_table int32 [B, bt_width] (row stride bt_stride) maps a sequence's logical pages to physical ones; an
  * entry outside [0, num_pages) is reported through t2c_device_status (T2C_EINVAL): writes skip those rows,
  * attention and eviction read page 0 in their place, the read back gives zeros.

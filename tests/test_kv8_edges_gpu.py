@@ -165,3 +165,70 @@ def test_nan_values_in_a_short_cache():
     clean()
     _seen_nan(out.unsqueeze(1), lse.unsqueeze(-1), want, poisoned)
     check_weights(w, before, want, positions, 1, NK)
+
+
+# ------------------------------------------------------------------ views
+def _loose(x, dims):
+    """x on the GPU, with a stride of 5 along its dimensions of one entry, where no stride counts."""
+    x = x.cuda()
+    strides = [5 if d in dims else s for d, s in enumerate(x.stride())]
+    y = torch.as_strided(x, x.shape, strides)
+    assert y.shape == x.shape and all(x.shape[d] == 1 for d in dims)
+    return y
+
+
+def test_strides_of_dimensions_of_one_entry_do_not_count():
+    """One sequence, one token, one head or one page: what their strides say is no reason to refuse a call."""
+    from torch2vk_b200 import kernels
+
+    NH, NK, dim, page, block, T = 4, 1, 64, 64, 16, 5
+    cache, table = ref.pool(1, NK, page, dim, block, seed=231), torch.zeros(1, 1, dtype=torch.int32)
+    g = torch.Generator().manual_seed(232)
+    pages = kernels.Q8Pages(_loose(cache["k"], (0, 1)), _loose(cache["v"], (0, 1)), cache["ks"].cuda(), cache["vs"].cuda())
+    bt = _loose(table, (0,))
+    k, v = (torch.randn(1, T, NK, dim, generator=g).half() for _ in range(2))
+    q = torch.randn(1, T, NH, dim, generator=g).half()
+    kernels.kv_cache_write_q8(pages, _loose(k, (0, 2)), _loose(v, (0, 2)), i32([20]), bt)
+    ref.write(cache, k, v, [20], table)
+    clean()
+    same_cache(pages, cache)
+    want = ref.attention(cache, q, [20], table, dim ** -0.5)
+    out, lse = kernels.attn_prefill_q8(_loose(q, (0,)), pages, i32([20]), bt, return_lse=True,
+                                       out=_loose(torch.zeros_like(q), (0,)))
+    before = torch.rand(1, NK, page, generator=g)
+    w = _loose(before, (0, 1))
+    kernels.attn_key_weights_q8(_loose(q, (0,)), lse, pages, i32([20]), bt, weights=w, weights_out=w)
+    clean()
+    check_attention(out, lse, want)
+    check_weights(w, before, want, [20], T, NK)
+    for t in (0, 4):
+        one = kernels.attn_decode_q8(_loose(q[:, t], (0,)), pages, i32([20 + t]), bt, out=_loose(torch.zeros(1, NH, dim).half(), (0,)))
+        clean()
+        check_attention(one.unsqueeze(1), None, {n: (x[:, t: t + 1] if n in ("out", "spread") else x[:, :, t: t + 1])
+                                                 for n, x in want.items() if n != "probs"})
+    w = _weights(1, NK, page, 233)
+    wd = _loose(w, (0, 1))
+    kept, left = kernels.kv_cache_evict_q8(pages, wd, i32([60]), bt, keep=21, sinks=2, recent=3)
+    clean()
+    chosen, want_left = ref.evict(cache, w, [60], table, table, keep=21, sinks=2, recent=3)
+    assert left.cpu().tolist() == want_left
+    _check_kept(kept, wd, chosen, w, 21)
+    same_cache(pages, cache)
+    k1, _ = kernels.kv_cache_read_q8(pages, i32([0]), left, bt, tokens=21)
+    assert torch.equal(k1[0].cpu(), ref.rows(cache, table[0], 21)[0].transpose(0, 1).half())
+
+
+def test_evict_one_sequence_through_a_view_of_the_table():
+    """One row of the table: in place whatever the rows' strides."""
+    from torch2vk_b200 import kernels
+
+    NK, page, dim, block, keep = 2, 32, 64, 16, 40
+    cache, table = ref.pool(6, NK, page, dim, block, seed=235), ref.tables(1, 6, 0, seed=236)
+    w = _weights(1, NK, 6 * page, 237)
+    pages, bt, wd = device_pages(cache), table.cuda(), w.cuda()
+    kept, left = kernels.kv_cache_evict_q8(pages, wd, i32([190]), bt, keep=keep, sinks=2, recent=8, out_table=_loose(bt, (0,))[:, :2])
+    clean()
+    chosen, want_left = ref.evict(cache, w, [190], table, table, keep=keep, sinks=2, recent=8)
+    assert left.cpu().tolist() == want_left
+    _check_kept(kept, wd, chosen, w, keep)
+    same_cache(pages, cache)

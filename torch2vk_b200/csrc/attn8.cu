@@ -705,7 +705,7 @@ extern "C" int t2c_attn_decode_q8(const t2c_q8_pages *pages, const void *q, int6
     AttnArgs &a = p.a;
     int rc = kv8_attn_check(pages, "attn_decode_q8", a.pg, block_table, bt_stride, bt_width, positions, B, 1, NH, max_len);
     if (rc != T2C_OK) return rc;
-    if (!kv8_strides(q, q_sb, q_sh, 0) || !kv8_strides(out, o_sb, o_sh, 0))
+    if (!kv8_strides(q, B, q_sb, NH, q_sh, 1, 0) || !kv8_strides(out, B, o_sb, NH, o_sh, 1, 0))
         return set_error(T2C_EINVAL, "attn_decode_q8: q and out rows must be 16-byte aligned");
     if (splits < 0) return set_error(T2C_EINVAL, "attn_decode_q8: splits %lld", (long long)splits);
     const int64_t D = pages->head_dim, group = NH / a.pg.n_kv;

@@ -352,7 +352,7 @@ extern "C" int t2c_attn_key_weights_q8(const t2c_q8_pages *pages, const void *q,
     WeightArgs a = {};
     int rc = kv8_attn_check(pages, "attn_key_weights_q8", a.pg, block_table, bt_stride, bt_width, positions, B, T, NH, max_len);
     if (rc != T2C_OK) return rc;
-    if (!kv8_strides(q, q_sb, q_st, q_sh)) return set_error(T2C_EINVAL, "attn_key_weights_q8: q rows must be 16-byte aligned");
+    if (!kv8_strides(q, B, q_sb, T, q_st, NH, q_sh)) return set_error(T2C_EINVAL, "attn_key_weights_q8: q rows must be 16-byte aligned");
     if (!lse || !weights_out) return set_error(T2C_EINVAL, "attn_key_weights_q8: NULL pointer");
     const int64_t group = NH / a.pg.n_kv, D = pages->head_dim;
     if (group > kWRows) return set_error(T2C_EUNSUPPORTED, "attn_key_weights_q8: group %lld", (long long)group);

@@ -680,7 +680,7 @@ extern "C" int t2c_attn_prefill_q8(const t2c_q8_pages *pages, const void *q, int
     PrefillArgs a = {};
     int rc = kv8_attn_check(pages, "attn_prefill_q8", a.pg, block_table, bt_stride, bt_width, positions, B, T, NH, max_len);
     if (rc != T2C_OK) return rc;
-    if (!kv8_strides(q, q_sb, q_st, q_sh) || !kv8_strides(out, o_sb, o_st, o_sh))
+    if (!kv8_strides(q, B, q_sb, T, q_st, NH, q_sh) || !kv8_strides(out, B, o_sb, T, o_st, NH, o_sh))
         return set_error(T2C_EINVAL, "attn_prefill_q8: q and out rows must be 16-byte aligned");
     if (splits < 0) return set_error(T2C_EINVAL, "attn_prefill_q8: splits %lld", (long long)splits);
     const int64_t D = pages->head_dim;

@@ -23,8 +23,8 @@ int kv8_view(const t2c_q8_pages *p, const char *what, KvPages &out) {
         return set_error(T2C_EINVAL, "%s: bad pool shape", what);
     if (p->head_dim != 64 && p->head_dim != 128)
         return set_error(T2C_EUNSUPPORTED, "%s: head_dim %lld", what, (long long)p->head_dim);
-    if (!kv8_aligned(p->k, 16) || !kv8_aligned(p->v, 16) || p->page_stride % 16 || p->head_stride % 16 ||
-        p->row_stride % 16 || !kv8_aligned(p->k_scale, 2) || !kv8_aligned(p->v_scale, 2))
+    if (!kv8_aligned(p->k, 16) || !kv8_aligned(p->v, 16) || (p->num_pages > 1 && p->page_stride % 16) ||
+        (p->n_kv > 1 && p->head_stride % 16) || p->row_stride % 16 || !kv8_aligned(p->k_scale, 2) || !kv8_aligned(p->v_scale, 2))
         return set_error(T2C_EINVAL, "%s: page rows must be 16-byte aligned", what);
     out.k = static_cast<int8_t *>(p->k);
     out.v = static_cast<int8_t *>(p->v);
@@ -42,10 +42,10 @@ int kv8_view(const t2c_q8_pages *p, const char *what, KvPages &out) {
     return T2C_OK;
 }
 
-int kv8_table(const t2c_q8_pages *p, const int32_t *table, int64_t stride, int64_t width, const char *what,
+int kv8_table(const t2c_q8_pages *p, const int32_t *table, int64_t B, int64_t stride, int64_t width, const char *what,
               int64_t &capacity) {
     if (!table) return set_error(T2C_EINVAL, "%s: NULL block table", what);
-    if (width <= 0 || stride < width || width > (INT32_MAX - 65536) / p->page_size)
+    if (width <= 0 || (B > 1 && stride < width) || width > (INT32_MAX - 65536) / p->page_size)
         return set_error(T2C_EINVAL, "%s: bad block table", what);
     capacity = width * p->page_size;
     return T2C_OK;
@@ -55,7 +55,7 @@ int kv8_attn_check(const t2c_q8_pages *pages, const char *what, KvPages &pg, con
           int64_t bt_width, const int32_t *positions, int64_t B, int64_t T, int64_t NH, int64_t &max_len) {
     int64_t capacity = 0;
     int rc = kv8_view(pages, what, pg);
-    if (rc == T2C_OK) rc = kv8_table(pages, table, bt_stride, bt_width, what, capacity);
+    if (rc == T2C_OK) rc = kv8_table(pages, table, B, bt_stride, bt_width, what, capacity);
     if (rc != T2C_OK) return rc;
     if (!positions) return set_error(T2C_EINVAL, "%s: NULL positions", what);
     if (B <= 0 || T <= 0 || NH <= 0 || NH % pg.n_kv || B > 65535 || B * T * NH > INT32_MAX)
@@ -81,8 +81,10 @@ bool kv8_maps(const t2c_q8_pages *p, int rows, CUtensorMap &k_map, CUtensorMap &
     if (!encode) return false;
     const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p->head_dim), static_cast<cuuint64_t>(p->page_size),
                                 static_cast<cuuint64_t>(p->n_kv), static_cast<cuuint64_t>(p->num_pages)};
-    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(p->row_stride), static_cast<cuuint64_t>(p->head_stride),
-                                   static_cast<cuuint64_t>(p->page_stride)};
+    // a dimension of one entry may have any stride: give the driver one it takes
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(p->row_stride),
+                                   static_cast<cuuint64_t>(p->n_kv > 1 ? p->head_stride : p->row_stride),
+                                   static_cast<cuuint64_t>(p->num_pages > 1 ? p->page_stride : p->row_stride)};
     const cuuint32_t box[4] = {static_cast<cuuint32_t>(p->head_dim), static_cast<cuuint32_t>(rows), 1, 1};
     const cuuint32_t es[4] = {1, 1, 1, 1};
     const CUtensorMapSwizzle swizzle = p->head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
@@ -544,11 +546,11 @@ extern "C" int t2c_kv_cache_write_q8(const t2c_q8_pages *pages, const void *k, i
     KvPages pg;
     int64_t capacity = 0;
     int rc = kv8_view(pages, "kv_cache_write_q8", pg);
-    if (rc == T2C_OK) rc = kv8_table(pages, block_table, bt_stride, bt_width, "kv_cache_write_q8", capacity);
+    if (rc == T2C_OK) rc = kv8_table(pages, block_table, B, bt_stride, bt_width, "kv_cache_write_q8", capacity);
     if (rc != T2C_OK) return rc;
     if (!k || !v || !positions) return set_error(T2C_EINVAL, "kv_cache_write_q8: NULL pointer");
     if (B <= 0 || T <= 0 || T > INT32_MAX - 128) return set_error(T2C_EINVAL, "kv_cache_write_q8: bad shape");
-    if (!kv8_aligned(k, 16) || !kv8_aligned(v, 16) || k_sb % 8 || k_st % 8 || k_sh % 8 || v_sb % 8 || v_st % 8 || v_sh % 8)
+    if (!kv8_strides(k, B, k_sb, T, k_st, pg.n_kv, k_sh) || !kv8_strides(v, B, v_sb, T, v_st, pg.n_kv, v_sh))
         return set_error(T2C_EINVAL, "kv_cache_write_q8: rows must be 16-byte aligned");
     const int64_t groups = (T + 62) / 64 + 1;  // 64-row groups that T rows from any position can touch
     if (B * groups > INT32_MAX || pg.n_kv > 32767) return set_error(T2C_EINVAL, "kv_cache_write_q8: bad shape");
@@ -565,7 +567,7 @@ extern "C" int t2c_kv_cache_read_q8(const t2c_q8_pages *pages, void *k_out, void
     KvPages pg;
     int64_t capacity = 0;
     int rc = kv8_view(pages, "kv_cache_read_q8", pg);
-    if (rc == T2C_OK) rc = kv8_table(pages, block_table, bt_stride, bt_width, "kv_cache_read_q8", capacity);
+    if (rc == T2C_OK) rc = kv8_table(pages, block_table, B, bt_stride, bt_width, "kv_cache_read_q8", capacity);
     if (rc != T2C_OK) return rc;
     if (!k_out || !v_out || !first || !lengths) return set_error(T2C_EINVAL, "kv_cache_read_q8: NULL pointer");
     if (B <= 0 || T <= 0 || T > INT32_MAX) return set_error(T2C_EINVAL, "kv_cache_read_q8: bad shape");
@@ -589,8 +591,8 @@ extern "C" int t2c_kv_cache_evict_q8(const t2c_q8_pages *pages, const float *wei
     KvPages pg;
     int64_t capacity = 0, out_capacity = 0;
     int rc = kv8_view(pages, "kv_cache_evict_q8", pg);
-    if (rc == T2C_OK) rc = kv8_table(pages, block_table, bt_stride, bt_width, "kv_cache_evict_q8", capacity);
-    if (rc == T2C_OK) rc = kv8_table(pages, out_table, ot_stride, ot_width, "kv_cache_evict_q8", out_capacity);
+    if (rc == T2C_OK) rc = kv8_table(pages, block_table, B, bt_stride, bt_width, "kv_cache_evict_q8", capacity);
+    if (rc == T2C_OK) rc = kv8_table(pages, out_table, B, ot_stride, ot_width, "kv_cache_evict_q8", out_capacity);
     if (rc != T2C_OK) return rc;
     if (!weights || !lengths || !weights_out || !kept || !new_lengths)
         return set_error(T2C_EINVAL, "kv_cache_evict_q8: NULL pointer");
@@ -601,7 +603,7 @@ extern "C" int t2c_kv_cache_evict_q8(const t2c_q8_pages *pages, const float *wei
         return set_error(T2C_EINVAL, "kv_cache_evict_q8: keep %lld exceeds the %lld positions of out_table", (long long)keep,
                          (long long)out_capacity);
     const bool in_place = out_table == block_table;
-    if (in_place && ot_stride != bt_stride) return set_error(T2C_EINVAL, "kv_cache_evict_q8: one table with two strides");
+    if (in_place && B > 1 && ot_stride != bt_stride) return set_error(T2C_EINVAL, "kv_cache_evict_q8: one table with two strides");
     if (!in_place && weights == weights_out)
         return set_error(T2C_EINVAL, "kv_cache_evict_q8: weights in place need the codes in place");
     if (weights == weights_out && ((B > 1 && w_sb != wo_sb) || (pg.n_kv > 1 && w_sh != wo_sh)))

@@ -26,7 +26,7 @@ struct KvPages {
 // Checks the pool's description; fills `out`.  `what` names the entry point in messages.
 int kv8_view(const t2c_q8_pages *pages, const char *what, KvPages &out);
 // Checks a block table against the pool: returns T2C_OK and the capacity in positions.
-int kv8_table(const t2c_q8_pages *pages, const int32_t *table, int64_t stride, int64_t width, const char *what,
+int kv8_table(const t2c_q8_pages *pages, const int32_t *table, int64_t B, int64_t stride, int64_t width, const char *what,
               int64_t &capacity);
 
 // What the attention entry points check alike; max_len becomes the bound in positions.
@@ -182,9 +182,10 @@ int kv8_configure(Kernel kern, int smem, int slot, const char *what) {
 
 inline bool kv8_aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
-// An fp16 tensor whose rows are 16-byte aligned.
-inline bool kv8_strides(const void *p, int64_t a, int64_t b, int64_t c) {
-    return p && kv8_aligned(p, 16) && a % 8 == 0 && b % 8 == 0 && c % 8 == 0;
+// An fp16 tensor whose rows are 16-byte aligned: (entries, stride) of its dimensions but the last.  One entry has no stride.
+inline bool kv8_strides(const void *p, int64_t na, int64_t a, int64_t nb, int64_t b, int64_t nc, int64_t c) {
+    const auto fits = [](int64_t n, int64_t stride) { return n == 1 || stride % 8 == 0; };
+    return p && kv8_aligned(p, 16) && fits(na, a) && fits(nb, b) && fits(nc, c);
 }
 
 }  // namespace t2c

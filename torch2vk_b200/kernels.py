@@ -812,6 +812,12 @@ def row_mean_f32(x: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
 
 
 # ------------------------------------------------ paged KV cache in 8 bits
+def _one_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """One shape and one layout; a dimension of one entry may have any stride."""
+    return a.shape == b.shape and (a.stride() == b.stride()
+                                   or all(n == 1 or x == y for n, x, y in zip(a.shape, a.stride(), b.stride())))
+
+
 class Q8Pages:
     """One layer's pool of the 8-bit paged cache: int8 codes k / v [num_pages, n_kv, page_size, head_dim] (any page,
     head and row strides that are multiples of 16, the same for both) and one fp16 scale for each `block`
@@ -822,11 +828,11 @@ class Q8Pages:
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
         shape, strides = k.shape, k.stride()
-        if k.dtype != torch.int8 or v.dtype != torch.int8 or len(shape) != 4 or v.shape != shape or v.stride() != strides:
+        if k.dtype != torch.int8 or v.dtype != torch.int8 or len(shape) != 4 or not _one_layout(k, v):
             raise ValueError("k / v must be int8 [num_pages, n_kv, page_size, head_dim] of one layout")
         s_shape, s_strides = k_scale.shape, k_scale.stride()
         if (k_scale.dtype != torch.float16 or v_scale.dtype != torch.float16 or len(s_shape) != 3
-                or v_scale.shape != s_shape or v_scale.stride() != s_strides or s_shape[:2] != shape[:2]
+                or not _one_layout(k_scale, v_scale) or s_shape[:2] != shape[:2]
                 or s_shape[2] == 0 or shape[2] % s_shape[2]):
             raise ValueError("k_scale / v_scale must be float16 [num_pages, n_kv, page_size / block] of one layout")
         if strides[3] != 1 or (s_strides[2] != 1 and s_shape[2] > 1):
@@ -842,7 +848,7 @@ class Q8Pages:
 
 def _q8_table(table: torch.Tensor, batch: int) -> tuple[int, int, int]:
     shape = table.shape
-    if table.dtype != torch.int32 or len(shape) != 2 or shape[0] < batch or table.stride(1) != 1:
+    if table.dtype != torch.int32 or len(shape) != 2 or shape[0] < batch or (table.stride(1) != 1 and shape[1] > 1):
         raise ValueError("block_table must be int32 [sequences, pages] with unit last stride")
     return _lib.ptr(table), table.stride(0), shape[1]
 
@@ -911,8 +917,7 @@ def _q8_weights(weights: torch.Tensor | None, weights_out: torch.Tensor, batch: 
     if weights_out.dtype != torch.float32 or weights_out.dim() != 3 or weights_out.stride(2) != 1 \
             or weights_out.shape[0] < batch or weights_out.shape[1] != heads or weights_out.shape[2] < positions:
         raise ValueError(f"weights_out must be float32 [batch, {heads}, at least {positions}] with unit last stride")
-    if weights is not None and (weights.dtype != torch.float32 or weights.shape != weights_out.shape
-                                or weights.stride() != weights_out.stride()):
+    if weights is not None and (weights.dtype != torch.float32 or not _one_layout(weights, weights_out)):
         raise ValueError("weights must have weights_out's type, shape and strides")
     return (None if weights is None else _lib.ptr(weights)), _lib.ptr(weights_out), *weights_out.stride()[:2]
 
