@@ -50,3 +50,25 @@ def test_join_makes_no_index_of_a_record_that_was_not_written(part_count):
             for last in edges + [rng.randrange(-(1 << 31), 1 << 31) for _ in range(20)]:
                 n = part_count(first, last, ctas, most)
                 assert n == (last - first + 1 if 0 <= first <= last < ctas and last - first < most else 0)
+
+
+def test_workspace_sizes_are_kept_per_device(monkeypatch):
+    """A workspace's size goes by the device's SMs: what was asked on one device is no answer for another."""
+    from types import SimpleNamespace
+
+    from torch2vk_b200 import kernels
+
+    now = {"device": 0}
+    floats = {0: 1000, 1: 2000}
+    monkeypatch.setattr(kernels.torch.cuda, "current_device", lambda: now["device"])
+    monkeypatch.setattr(kernels._lib, "lib", lambda: SimpleNamespace(raw=lambda name: lambda *args: floats[now["device"]]))
+    pages = SimpleNamespace(n_kv=8, head_dim=128, page_size=64)
+    table = SimpleNamespace(shape=(4, 100))
+    kernels._q8_workspace_floats.cache_clear()
+    try:
+        for device in (0, 1, 0, 1):
+            now["device"] = device
+            assert kernels.attn_decode_q8_workspace(pages, table, batch=4, n_heads=32) == floats[device]
+            assert kernels.attn_prefill_q8_workspace(pages, table, batch=4, tokens=5, n_heads=32) == floats[device]
+    finally:
+        kernels._q8_workspace_floats.cache_clear()

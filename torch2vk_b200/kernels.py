@@ -940,8 +940,8 @@ def _q8_max_len(max_len: int | None, table: torch.Tensor, pages: Q8Pages) -> int
 
 
 @functools.lru_cache(maxsize=1024)
-def _q8_workspace_floats(name: str, n_kv: int, head_dim: int, page_size: int, *args: int) -> int:
-    """The library's answer for a pool of this shape (it depends on nothing else)."""
+def _q8_workspace_floats(name: str, device: int, n_kv: int, head_dim: int, page_size: int, *args: int) -> int:
+    """The library's answer for a pool of this shape on this device, the current one (its SMs count, nothing else does)."""
     ref = _lib.Q8_PAGES.pack(0, 0, 0, 0, 0, 0, 0, 0, 0, 1, n_kv, page_size, head_dim, 16)
     return int(_lib.lib().raw(name)(ref, *args))
 
@@ -949,7 +949,7 @@ def _q8_workspace_floats(name: str, n_kv: int, head_dim: int, page_size: int, *a
 def _q8_workspace(workspace: torch.Tensor | None, like: torch.Tensor, pages: Q8Pages, name: str,
                   *args: int) -> tuple[torch.Tensor | None, int]:
     if workspace is None:
-        need = _q8_workspace_floats(name, pages.n_kv, pages.head_dim, pages.page_size, *args)
+        need = _q8_workspace_floats(name, torch.cuda.current_device(), pages.n_kv, pages.head_dim, pages.page_size, *args)
         if need <= 0:
             return None, 0
         return like.new_empty(need, dtype=torch.float32), need
@@ -961,8 +961,8 @@ def _q8_workspace(workspace: torch.Tensor | None, like: torch.Tensor, pages: Q8P
 def attn_decode_q8_workspace(pages: Q8Pages, block_table: torch.Tensor, *, batch: int, n_heads: int,
                              max_len: int | None = None, splits: int = 0, with_weights: bool = False) -> int:
     """Floats of workspace that attn_decode_q8 needs with these arguments."""
-    return _q8_workspace_floats("t2c_attn_decode_q8_workspace", pages.n_kv, pages.head_dim, pages.page_size,
-                                block_table.shape[1], batch, n_heads, _q8_max_len(max_len, block_table, pages), splits,
+    return _q8_workspace_floats("t2c_attn_decode_q8_workspace", torch.cuda.current_device(), pages.n_kv, pages.head_dim,
+                                pages.page_size, block_table.shape[1], batch, n_heads, _q8_max_len(max_len, block_table, pages), splits,
                                 1 if with_weights else 0)
 
 
@@ -1002,8 +1002,8 @@ def attn_decode_q8(q: torch.Tensor, pages: Q8Pages, positions: torch.Tensor, blo
 def attn_prefill_q8_workspace(pages: Q8Pages, block_table: torch.Tensor, *, batch: int, tokens: int, n_heads: int,
                               max_len: int | None = None, splits: int = 0) -> int:
     """Floats of workspace that attn_prefill_q8 needs with these arguments."""
-    return _q8_workspace_floats("t2c_attn_prefill_q8_workspace", pages.n_kv, pages.head_dim, pages.page_size,
-                                block_table.shape[1], batch, tokens, n_heads, _q8_max_len(max_len, block_table, pages), splits)
+    return _q8_workspace_floats("t2c_attn_prefill_q8_workspace", torch.cuda.current_device(), pages.n_kv, pages.head_dim,
+                                pages.page_size, block_table.shape[1], batch, tokens, n_heads, _q8_max_len(max_len, block_table, pages), splits)
 
 
 def attn_prefill_q8(q: torch.Tensor, pages: Q8Pages, positions: torch.Tensor, block_table: torch.Tensor, *,
