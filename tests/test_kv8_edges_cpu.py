@@ -72,3 +72,15 @@ def test_workspace_sizes_are_kept_per_device(monkeypatch):
             assert kernels.attn_prefill_q8_workspace(pages, table, batch=4, tokens=5, n_heads=32) == floats[device]
     finally:
         kernels._q8_workspace_floats.cache_clear()
+
+
+def test_stream_handle_without_torch_internals(monkeypatch):
+    """A torch without the raw-handle function: its current stream is asked instead."""
+    from types import SimpleNamespace
+
+    from torch2vk_b200 import _lib
+
+    monkeypatch.setattr(_lib.torch.cuda, "current_stream", lambda: SimpleNamespace(cuda_stream=77))
+    monkeypatch.setattr(_lib, "_raw_stream", None)
+    assert _lib.stream_ptr() == 77
+    assert _lib.stream_ptr(SimpleNamespace(cuda_stream=5)) == 5

@@ -184,9 +184,15 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr()
 
 
+# torch's own, not part of its interface: the current stream's handle without a Stream object around it, where there is one
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr(stream: torch.cuda.Stream | None = None) -> int:
-    if stream is None:  # the raw handle, without building a Stream object
-        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    if stream is None:
+        if _raw_stream is not None:
+            return _raw_stream(torch.cuda.current_device())
+        stream = torch.cuda.current_stream()
     return stream.cuda_stream
 
 
