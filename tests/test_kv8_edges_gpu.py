@@ -71,6 +71,17 @@ def test_evict_refuses_one_tensor_with_two_strides():
                                   weights_out=buf[:128].view(2, 2, 32))
 
 
+@pytest.mark.parametrize("bad", [dict(keep=0), dict(keep=10, sinks=-1), dict(keep=10, recent=-1), dict(keep=10, sinks=6, recent=5)])
+def test_evict_says_what_it_needs(bad):
+    """No sinks and no recent window are fine; what is refused is what the message says."""
+    from torch2vk_b200 import kernels
+
+    cache, table = ref.pool(9, 2, 16, 64, 16, seed=207), ref.tables(2, 4, 1, seed=208)
+    w = torch.zeros(2, 2, 64, device="cuda")
+    with pytest.raises(RuntimeError, match="keep > 0, sinks >= 0, recent >= 0 and sinks \\+ recent <= keep"):
+        kernels.kv_cache_evict_q8(device_pages(cache), w, i32([60, 60]), table.cuda(), **bad)
+
+
 def test_evict_in_place_through_a_view_of_the_table():
     """A view that begins where the block table does names the same pages: the move is in place, the weights too."""
     from torch2vk_b200 import kernels

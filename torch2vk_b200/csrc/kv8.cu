@@ -598,7 +598,7 @@ extern "C" int t2c_kv_cache_evict_q8(const t2c_q8_pages *pages, const float *wei
         return set_error(T2C_EINVAL, "kv_cache_evict_q8: NULL pointer");
     if (lengths == new_lengths) return set_error(T2C_EINVAL, "kv_cache_evict_q8: new_lengths must not be lengths");
     if (B <= 0 || sinks < 0 || recent < 0 || keep <= 0 || sinks + recent > keep)
-        return set_error(T2C_EINVAL, "kv_cache_evict_q8: needs 0 < sinks + recent <= keep");
+        return set_error(T2C_EINVAL, "kv_cache_evict_q8: needs keep > 0, sinks >= 0, recent >= 0 and sinks + recent <= keep");
     if (keep > out_capacity)
         return set_error(T2C_EINVAL, "kv_cache_evict_q8: keep %lld exceeds the %lld positions of out_table", (long long)keep,
                          (long long)out_capacity);
