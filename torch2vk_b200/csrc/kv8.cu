@@ -594,11 +594,12 @@ extern "C" int t2c_kv_cache_evict_q8(const t2c_q8_pages *pages, const float *wei
     if (rc == T2C_OK) rc = kv8_table(pages, block_table, B, bt_stride, bt_width, "kv_cache_evict_q8", capacity);
     if (rc == T2C_OK) rc = kv8_table(pages, out_table, B, ot_stride, ot_width, "kv_cache_evict_q8", out_capacity);
     if (rc != T2C_OK) return rc;
+    if (B <= 0) return set_error(T2C_EINVAL, "kv_cache_evict_q8: bad shape");
+    if (sinks < 0 || recent < 0 || keep <= 0 || sinks + recent > keep)
+        return set_error(T2C_EINVAL, "kv_cache_evict_q8: needs keep > 0, sinks >= 0, recent >= 0 and sinks + recent <= keep");
     if (!weights || !lengths || !weights_out || !kept || !new_lengths)
         return set_error(T2C_EINVAL, "kv_cache_evict_q8: NULL pointer");
     if (lengths == new_lengths) return set_error(T2C_EINVAL, "kv_cache_evict_q8: new_lengths must not be lengths");
-    if (B <= 0 || sinks < 0 || recent < 0 || keep <= 0 || sinks + recent > keep)
-        return set_error(T2C_EINVAL, "kv_cache_evict_q8: needs keep > 0, sinks >= 0, recent >= 0 and sinks + recent <= keep");
     if (keep > out_capacity)
         return set_error(T2C_EINVAL, "kv_cache_evict_q8: keep %lld exceeds the %lld positions of out_table", (long long)keep,
                          (long long)out_capacity);
