@@ -15,19 +15,19 @@ namespace {
 struct AttnArgs {
     KvPages pg;
     const __half *q;
-    int64_t q_sb, q_st, q_sh;
+    int64_t q_sb, q_sh;
     __half *out;
-    int64_t o_sb, o_st, o_sh;
-    float *lse;  // [B, NH, T]
+    int64_t o_sb, o_sh;
+    float *lse;  // [B, NH]
     const int32_t *positions, *table;
     int64_t t_stride, max_len;
-    int B, T, NH;
+    int B, NH;
     float scale_log2;
 };
 
-// Number of keys query t of sequence b sees.
-__device__ __forceinline__ int64_t visible(const int32_t *positions, int b, int t, int64_t max_len) {
-    const int64_t n = static_cast<int64_t>(positions[b]) + t + 1;
+// Number of keys the query of sequence b sees.
+__device__ __forceinline__ int64_t visible(const int32_t *positions, int b, int64_t max_len) {
+    const int64_t n = static_cast<int64_t>(positions[b]) + 1;
     if (n > max_len) {
         report_device_error(T2C_EINVAL);
         return max_len;
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kDThreads, 4) attn8_decode_kernel(const __grid
     do {
         const int head = unit / p.head_chunks, chunk = unit % p.head_chunks;
         const int heads = min(8, group - 8 * chunk), h0 = head * group + 8 * chunk;
-        const int64_t n = visible(a.positions, b, 0, a.max_len);
+        const int64_t n = visible(a.positions, b, a.max_len);
         const int t1 = min(t0 + left, unit_tiles);
         const int64_t k0 = min(static_cast<int64_t>(t0) * kDTile, n), k1 = min(static_cast<int64_t>(t1) * kDTile, n);
         const int32_t *bt = a.table + b * a.t_stride;
@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(kDThreads, 4) attn8_decode_kernel(const __grid
     // ---- the cluster's CTAs hold all of the unit's keys: join through distributed shared memory
     const int head = unit / p.head_chunks, chunk = unit % p.head_chunks;
     const int heads = min(8, group - 8 * chunk), h0 = head * group + 8 * chunk;
-    const int64_t n = visible(a.positions, b, 0, a.max_len);
+    const int64_t n = visible(a.positions, b, a.max_len);
     const int C = p.splits;
     constexpr int kPitch = D + 4;
     float *part = reinterpret_cast<float *>(smem);
@@ -720,7 +720,7 @@ extern "C" int t2c_attn_decode_q8(const t2c_q8_pages *pages, const void *q, int6
     a.out = static_cast<__half *>(out), a.o_sb = o_sb, a.o_sh = o_sh;
     a.lse = lse;
     a.positions = positions, a.table = block_table, a.t_stride = bt_stride, a.max_len = max_len;
-    a.B = static_cast<int>(B), a.T = 1, a.NH = static_cast<int>(NH);
+    a.B = static_cast<int>(B), a.NH = static_cast<int>(NH);
     a.scale_log2 = scale * 1.4426950408889634f;
     const int64_t tiles = (max_len + kDTile - 1) / kDTile;
     p.splits = plan.splits, p.head_chunks = plan.head_chunks, p.ctas = plan.ctas;

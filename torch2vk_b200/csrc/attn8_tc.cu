@@ -22,7 +22,8 @@
 // scale joins as log2 vs, and the softmax sum takes P / vs.  One reference m per row serves all tiles until the P of
 // 16 keys sum to more than 2^14: then the row's m moves to those keys' maximum - 8 (a whole number, so that rescaling
 // by 2^(old - new) is exact) and O, l and the tile's P are rescaled.  So no pass looks for the maximum; P's rounding
-// to fp16 (what the tensor core takes) is the only one before the output's.
+// to fp16 (what the tensor core takes) is the only one before the output's, but for P that a move brings below fp16's
+// normal numbers: those round once more, by at most 2^-25 where the row's largest P is 2^8 or more.
 //
 // Within groups of four dims K and Q rows are held in the order 0, 2, 1, 3 (as the expansion leaves them; the product
 // does not see it), V's columns too, which the epilogue undoes.

@@ -334,10 +334,7 @@ class Qwen3Runner:
         _, lse = kernels.attn_prefill_q8(q, pages, self.slots, bt, max_len=end, return_lse=True, out=out)
         w = min(self.kv_window, tokens_per_seq)
         last = self.slots + (tokens_per_seq - w)
-        if self.cached:  # keys of an earlier prompt keep what they had; this prompt's start from its own queries
-            weights[:, :, self.cached:end] = 0.0
-        else:
-            weights[:, :, :end] = 0.0
+        weights[:, :, self.cached:end] = 0.0  # earlier keys keep what they had; this prompt's start from its own queries
         kernels.attn_key_weights_q8(q[:, tokens_per_seq - w:], lse[:, :, tokens_per_seq - w:].contiguous(), pages, last, bt,
                                     max_len=end, weights=weights, weights_out=weights)
 
