@@ -243,3 +243,124 @@ def test_evict_one_sequence_through_a_view_of_the_table():
     assert left.cpu().tolist() == want_left
     _check_kept(kept, wd, chosen, w, keep)
     same_cache(pages, cache)
+
+
+# ------------------------------------------------------------------ eviction: entries, lengths, layouts, NaN, and what follows it
+def _evict_case(B, NK, page, dim, block, width, keep, seed):
+    out = -(-keep // page)
+    cache, both = ref.pool(B * (width + out) + 1, NK, page, dim, block, seed=seed), ref.tables(B, width + out, 0, seed=seed + 1) + 1  # page 0 is nobody's
+    return cache, both[:, :width].contiguous(), both[:, width:].contiguous(), _weights(B, NK, width * page, seed + 2)
+
+
+@pytest.mark.parametrize("layout", ["head_major", "token_major"])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_nan_blocks_and_layouts(in_place, layout):
+    """Rows of a block that reads as NaN make the block they move to read as NaN; pages in either order in memory."""
+    from torch2vk_b200 import kernels
+
+    B, NK, page, dim, block, width, keep = 2, 3, 32, 128, 16, 10, 150
+    cache, table, to, w = _evict_case(B, NK, page, dim, block, width, keep, 241)
+    cache["ks"][table[0, 4], 1, 1], cache["vs"][table[1, 9], 2, 0] = math.nan, math.nan
+    lengths = [320, 311]
+    pages, bt, wd = device_pages(cache, layout), table.cuda(), w.cuda()
+    wo = wd if in_place else torch.zeros(B, NK, keep, device="cuda")
+    kept, left = kernels.kv_cache_evict_q8(pages, wd, i32(lengths), bt, keep=keep, sinks=4, recent=40,
+                                           out_table=None if in_place else to.cuda(), weights_out=wo)
+    clean()
+    chosen, want_left = ref.evict(cache, w, lengths, table, table if in_place else to, keep=keep, sinks=4, recent=40)
+    assert left.cpu().tolist() == want_left
+    _check_kept(kept, wo, chosen, w, keep)
+    same_cache(pages, cache)
+    k, v = kernels.kv_cache_read_q8(pages, i32([0, 0]), left, bt if in_place else to.cuda(), tokens=keep)
+    assert bool(torch.isnan(k[0, :, 1]).any()) and bool(torch.isnan(v[1, :, 2]).any()) and not torch.isnan(k[1]).any()
+
+
+def test_evict_reports_bad_entries():
+    """A source entry outside the pool is reported and read as page 0; rows of a destination entry outside it are skipped."""
+    from torch2vk_b200 import kernels
+
+    B, NK, page, dim, block, width, keep = 2, 2, 32, 64, 16, 5, 70
+    cache, table, to, w = _evict_case(B, NK, page, dim, block, width, keep, 251)
+    assert not (table == 0).any() and not (to == 0).any()
+    lengths = [160, 133]
+    bad, zero = table.clone(), table.clone()
+    bad[0, 1], bad[1, 3], zero[0, 1], zero[1, 3] = 1 << 20, -7, 0, 0
+    pages, wd, wo = device_pages(cache), w.cuda(), torch.zeros(B, NK, keep, device="cuda")
+    kept, left = kernels.kv_cache_evict_q8(pages, wd, i32(lengths), bad.cuda(), keep=keep, sinks=4, recent=40, out_table=to.cuda(),
+                                           weights_out=wo)
+    assert kernels.device_status(clear=True) == 1 << 1
+    chosen, _ = ref.evict(cache, w, lengths, zero, to, keep=keep, sinks=4, recent=40)
+    _check_kept(kept, wo, chosen, w, keep)
+    same_cache(pages, cache)
+    was = {n: x.clone() for n, x in cache.items()}
+    bad = to.clone()
+    bad[0, 1] = cache["k"].shape[0]
+    kept, _ = kernels.kv_cache_evict_q8(pages, wd, i32(lengths), table.cuda(), keep=keep, sinks=4, recent=40, out_table=bad.cuda(),
+                                        weights_out=wo)
+    assert kernels.device_status(clear=True) == 1 << 1
+    chosen, _ = ref.evict(cache, w, lengths, table, to, keep=keep, sinks=4, recent=40)
+    for n in cache:
+        cache[n][to[0, 1]] = was[n][to[0, 1]]
+    same_cache(pages, cache)
+    assert kept[0, 0].cpu().tolist() == chosen[0][0]
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_reports_lengths_out_of_range(in_place):
+    """A length past the table counts as the table's positions, a negative one as none; both are reported."""
+    from torch2vk_b200 import kernels
+
+    B, NK, page, dim, block, width, keep = 3, 2, 32, 64, 16, 4, 50
+    cache, table, to, w = _evict_case(B, NK, page, dim, block, width, keep, 261)
+    pages, bt, wd = device_pages(cache), table.cuda(), w.cuda()
+    wo = wd if in_place else torch.zeros(B, NK, keep, device="cuda")
+    kept, left = kernels.kv_cache_evict_q8(pages, wd, i32([width * page + 9, -4, 60]), bt, keep=keep, sinks=1, recent=9,
+                                           out_table=None if in_place else to.cuda(), weights_out=wo)
+    assert kernels.device_status(clear=True) == 1 << 1
+    lengths = [width * page, 0, 60]
+    chosen, want_left = ref.evict(cache, w, lengths, table, table if in_place else to, keep=keep, sinks=1, recent=9)
+    assert left.cpu().tolist() == want_left
+    _check_kept(kept, wo, chosen, w, keep)
+    same_cache(pages, cache)
+
+
+@pytest.mark.parametrize("page,block", [(64, 64), (32, 16)])
+def test_append_after_an_eviction(page, block):
+    """Rows appended to the block that an eviction left partly filled: its scale grows from the evicted rows' one."""
+    from torch2vk_b200 import kernels
+
+    B, NK, dim, width, keep = 3, 2, 128, 320 // page, 101
+    cache = ref.pool(B * width, NK, page, dim, block, seed=271)
+    table = ref.tables(B, width, 0, seed=272)
+    w = _weights(B, NK, width * page, 273)
+    pages, bt, wd = device_pages(cache), table.cuda(), w.cuda()
+    g = torch.Generator().manual_seed(274)
+    lengths = [300, 90, 102]
+    for T, gain in ((1, 0.2), (1, 4.0), (30, 9.0)):
+        _, left = kernels.kv_cache_evict_q8(pages, wd, i32(lengths), bt, keep=keep, sinks=4, recent=16)
+        _, want = ref.evict(cache, w, lengths, table, table, keep=keep, sinks=4, recent=16)
+        w = wd.cpu()
+        assert left.cpu().tolist() == want
+        k, v = (torch.randn(B, T, NK, dim, generator=g).half() * gain for _ in range(2))
+        kernels.kv_cache_write_q8(pages, k.cuda(), v.cuda(), left, bt)
+        clean()
+        ref.write(cache, k, v, want, table)
+        same_cache(pages, cache)
+        lengths = [n + T for n in want]
+
+
+@pytest.mark.parametrize("B,n,keep", [(1, 30000, 9000), (2, 9001, 2500), (1, 70000, 40000)])
+def test_evict_long_moves_the_weights(B, n, keep):
+    """In place, several rounds a head: a round's weights are read before an earlier round's stores reach them."""
+    from torch2vk_b200 import kernels
+
+    NK, page, dim, block = 2, 64, 64, 16
+    width = -(-n // page)
+    cache, table = ref.pool(B * width, NK, page, dim, block, seed=281), ref.tables(B, width, 0, seed=282)
+    w = torch.exp(2 * torch.randn(B, NK, width * page, generator=torch.Generator().manual_seed(283)))
+    pages, bt, wd = device_pages(cache), table.cuda(), w.cuda()
+    kept, left = kernels.kv_cache_evict_q8(pages, wd, i32([n - 31 * b for b in range(B)]), bt, keep=keep, sinks=4, recent=100)
+    clean()
+    assert left.cpu().tolist() == [keep] * B
+    assert torch.equal(wd[:, :, :keep].cpu(), torch.gather(w, 2, kept.long().cpu()))
+    assert bool((kept[:, :, 1:] > kept[:, :, :-1]).all()) and bool((kept[:, :, :4].cpu() == torch.arange(4)).all())

@@ -250,3 +250,94 @@ def test_capture_of_a_full_cache():
     for i in range(cfg.layers):
         assert torch.equal(r.paged.k[i], e.paged.k[i]) and torch.equal(r.paged.k_scale[i], e.paged.k_scale[i])
     _clean()
+
+
+def _rows(r, tokens):
+    from torch2vk_b200 import kernels
+
+    n = torch.full((2,), tokens, dtype=torch.int32, device="cuda")
+    return [x.float() for x in kernels.kv_cache_read_q8(r.paged.layer(0), torch.zeros_like(n), n, r.paged.block_table, tokens=tokens)]
+
+
+def test_cut_keeps_sinks_and_the_recent_window():
+    """After a cut the first rows of each head are the prompt's first, the last its last, to half a step of the block they
+    moved to; 2e-3 of the value is the fp16 rounding of both reads and of the scale."""
+    cfg, free = _runner(kv_bits=8)
+    _, tight = _runner(kv_bits=8, kv_budget=64, kv_sinks=4, kv_recent=16)
+    ids = _ids(cfg, 2, 100, 11)
+    free.prefill(ids)
+    tight.prefill(ids)
+    assert tight.cached == 64
+    for was, now in zip(_rows(free, 100), _rows(tight, 64)):
+        step = was.abs().amax((1, 3), keepdim=True) / 127  # of a head
+        for a, b in ((slice(0, 4), slice(0, 4)), (slice(84, 100), slice(48, 64))):
+            assert bool(((now[:, b] - was[:, a]).abs() <= 0.51 * step + 2e-3 * was[:, a].abs()).all())
+        assert not torch.equal(now[:, 4:48], was[:, 4:48])
+    _clean()
+
+
+def test_continued_prompt_after_a_cut():
+    """prefill(append=True) on a cache that was cut, rows and positions apart: the weights grow by what the window's
+    queries pay, and the layer outputs are those of the same tokens fed one by one."""
+    def bounded():
+        cfg, r = _runner(kv_bits=8, kv_budget=128, kv_sinks=4, kv_recent=32, kv_window=8)
+        r.prefill(_ids(cfg, 2, 200, 12))
+        for _ in range(3):
+            r.decode_step()
+        return cfg, r
+
+    cfg, r = bounded()
+    _, one = bounded()
+    assert r.cached == 131 and r.length == 203 and r.slots.tolist() == [131, 131] and r.positions.tolist() == [203, 203]
+    held = [w[:, :, :131].double().clone() for w in r.paged.weights]
+    ids = _ids(cfg, 2, 10, 13)
+    outs = []
+    r.prefill(ids, append=True, layer_outputs=outs)
+    assert r.cached == 141 and r.length == 213 and r.slots.tolist() == [141, 141] and r.positions.tolist() == [213, 213]
+    group = cfg.heads // cfg.kv_heads
+    for w, was in zip(r.paged.weights, held):
+        now = w[:, :, :141].double()
+        assert bool((now[:, :, :131] >= was - 1e-6).all()) and bool((now[:, :, 131:] >= 0).all())
+        paid = now.sum(-1) - was.sum(-1)
+        assert bool((paid - 8 * group).abs().max() < 1e-3 * 8 * group)
+    for t in range(10):
+        step = []
+        one.next_token.copy_(ids[:, t])
+        one.decode_step(layer_outputs=step)
+        for x, y in zip(outs, step):
+            assert _near(x.view(2, 10, -1)[:, t], y, 0.03)
+    r.step()
+    _clean()
+
+
+def test_tensor_parallel_runner_on_the_8_bit_pool():
+    """make_tp_runner takes the cache's settings; one rank gives the plain runner's tokens."""
+    import os
+    import subprocess
+    import sys
+
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = f"""
+import sys
+sys.path[:0] = [{here!r}, {os.path.dirname(here)!r}]
+from datetime import timedelta
+import torch, torch.distributed as dist
+from test_kv8_runner_gpu import _ids, _runner
+from torch2vk_b200.tp import make_tp_runner
+torch.cuda.set_device(0)
+dist.init_process_group("nccl", init_method="tcp://127.0.0.1:29577", rank=0, world_size=1, timeout=timedelta(seconds=60))
+kw = dict(kv_bits=8, kv_budget=64, kv_recent=16)
+cfg, plain = _runner(**kw)
+tp = make_tp_runner(cfg, _runner.weights, rank=0, tp=1, batch=2, max_seq=256, max_new_tokens=120, page_size=16, decode_splits=4, **kw)
+ids = _ids(cfg, 2, 100, 14)
+for r in (plain, tp):
+    r.prefill(ids)
+    for _ in range(40):
+        r.decode_step()
+assert torch.equal(plain.generated[:, :41], tp.generated[:, :41]) and plain.cached == tp.cached
+torch.cuda.synchronize()
+dist.destroy_process_group()
+print("tp ok")
+"""
+    run = subprocess.run(["timeout", "-k", "30", "240", sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "tp ok" in run.stdout, (run.stdout + run.stderr)[-3000:]
