@@ -605,7 +605,8 @@ int t2c_kv_cache_read_q8(const t2c_q8_pages *pages, void *k_out, void *v_out, co
  *   out = softmax(scale * q k^T) v, lse = log sum exp of the scaled scores (natural log; NULL: not stored).
  * A query that sees nothing (negative position) gives out 0 and lse -inf.  A V block that reads as NaN makes out NaN where
  * it is seen, and neither lse nor the weights below; a K block of NaN makes all three NaN for its head.
- * q, out fp16 with element strides (multiples of 8, unit along head_dim); lse fp32 [B, NH, T].
+ * q, out fp16 with element strides (multiples of 8, unit along head_dim); lse fp32 [B, NH, T].  Scores, softmax statistics
+ * and weights are fp32; the probabilities that meet V are rounded to fp16 (2^-11 of each), as the tensor cores take them.
  * max_len > 0: no sequence has more than max_len positions (longer ones are cut to it and reported).
  * splits: CTAs that share one sequence's keys, 0 = chosen by the library; workspace: at least
  * t2c_attn_*_q8_workspace(...) floats for the same arguments (-1: arguments out of range).

@@ -369,7 +369,7 @@ extern "C" int t2c_attn_key_weights_q8(const t2c_q8_pages *pages, const void *q,
     // SM (the next tile's codes arrive under this one).  Where many do, one, and a cluster of up to 8 CTAs shares out the
     // query tiles of the first keys, which every query sees, until the longest share is under 3/4 of the mean of an SM's
     // slot; 32 query tiles a CTA at least, which its beginning costs about 4 of (6000 queries of 16 heads on 8: 150 us
-    // alone, 116 in pairs, 139 in fours; 4096 queries of 16 heads of 64 on 16: 53, 62, 84).  32 queries on 2 x 16007
+    // alone, 117 in pairs, 139 in fours; 4096 queries of 16 heads of 64 on 16: 53, 62, 84).  32 queries on 2 x 16007
     // positions: 7 key tiles a CTA 26 us, one 39.
     const int64_t nq = (T + tokens - 1) / tokens, tiles = (max_len + 127) / 128, units = B * a.pg.n_kv, slots = 2 * sm_count();
     int64_t per = nq >= 8 ? 1 : (units * tiles + slots - 1) / slots;
