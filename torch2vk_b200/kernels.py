@@ -814,8 +814,8 @@ def row_mean_f32(x: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
 # ------------------------------------------------ paged KV cache in 8 bits
 def _one_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
     """One shape and one layout; a dimension of one entry may have any stride."""
-    return a.shape == b.shape and (a.stride() == b.stride()
-                                   or all(n == 1 or x == y for n, x, y in zip(a.shape, a.stride(), b.stride())))
+    shape, strides, others = a.shape, a.stride(), b.stride()
+    return shape == b.shape and (strides == others or all(n == 1 or x == y for n, x, y in zip(shape, strides, others)))
 
 
 class Q8Pages:
